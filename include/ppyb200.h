@@ -241,6 +241,140 @@ int32_t ppyb200_attention_causal_vt_bf16(const uint16_t *qkv, const uint16_t *vt
 int32_t ppyb200_attention_causal_bf16(const uint16_t *qkv, uint16_t *out, int64_t batch,
                                       int64_t length, int64_t heads, int64_t head_dim);
 
+/* ---------------------------------------------------------------- decoding with a cache */
+
+/* Element types of the decoding entry points. */
+#define PPYB200_F32 0
+#define PPYB200_BF16 1
+#define PPYB200_F16 2
+
+/* Limits: nodes of a tree with parents (a chain may be longer), steps of an accepted path, and
+ * steps x query heads a key head of one. */
+#define PPYB200_TREE_NODES 256
+#define PPYB200_PATH_STEPS 64
+#define PPYB200_PATH_ROWS 512
+
+/* Attention of drafted nodes over a cache, and their append to it. Sequence b has lengths[b]
+ * entries in its cache and counts[b] nodes (`nodes` for all when counts is NULL); node i attends
+ * to every entry, to its ancestors (parents[b][i] < i, -1 for a child of the last entry; NULL
+ * for a chain, parent i - 1) and to itself, with scores scale * q . k. Node i's key and value
+ * are written to slot lengths[b] + i. Query heads share key heads in order: heads / kv_heads
+ * each. Tensors are given by their first element and strides in elements, unit stride along
+ * head_dim: q, k_new, v_new and out by (batch, node, head), keys and values by (batch, head,
+ * slot); parents by its batch stride (0: one tree for all). out has q's type; lse (may be NULL)
+ * is f32 [batch][heads][nodes], the natural log of each row's sum of e^score. Rows of nodes at
+ * and behind counts[b] are left as they were, and so are the slots behind the last node.
+ * bf16 or f16, head_dim a multiple of 8 up to 128, rows on 16-byte boundaries. A length or count
+ * outside the buffers is held inside them, a parent that is no earlier node is taken for -1; both
+ * raise *status (may be NULL) to 2. q, k_new and v_new do not overlap the cache or out. No
+ * counterpart in the reference beyond its prompt attention (examples/46_gpt2/gpt2.ppy:52). */
+typedef struct ppyb200_tree_attention_args {
+  const void *q, *k_new, *v_new;
+  void *keys, *values;
+  const int32_t *lengths, *parents, *counts;
+  void *out;
+  float *lse;
+  int32_t *status;
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t dtype, batch, nodes, heads, kv_heads, head_dim, capacity;
+  int64_t q_strides[3], k_new_strides[3], v_new_strides[3];
+  int64_t keys_strides[3], values_strides[3], out_strides[3];
+  int64_t parents_stride;
+  double scale;
+} ppyb200_tree_attention_args;
+
+/* Device pointers; enqueued on the current stream. The workspace (16-byte aligned, at least
+ * ppyb200_tree_attention_workspace bytes, which only the sizes, the type and the device decide;
+ * it may be NULL when that is 0) is the caller's until the call's work is done: calls that may
+ * overlap, captured graphs among them, take one each. */
+int64_t ppyb200_tree_attention_workspace(const ppyb200_tree_attention_args *args);
+int32_t ppyb200_tree_attention(const ppyb200_tree_attention_args *args);
+
+/* A verified path joins the cache. path[b][0 .. accepted[b]) are nodes of the last attention in
+ * ascending order; q and lse are that attention's (layer by layer), its nodes at slots
+ * lengths[b] + node. For every layer and key head: weights of the lengths[b] entries grow by the
+ * sum of e^(score - lse) over the path's rows and the key head's query heads; entry
+ * lengths[b] + t (t < accepted[b]) gets the sum over the rows of steps t and later, the keys and
+ * values of node path[b][t], and the position seen[b] + t. lengths and seen are left to the
+ * caller. Strides in elements: q by (layer, batch, node, head), keys and values by (layer, batch,
+ * head, slot), weights and positions by (layer, batch, head) with unit stride along slots; lse
+ * [layers][batch][heads][nodes], path [batch][steps]. weights may be NULL (rows move only; q and
+ * lse are not read then), positions may be NULL. A path that is not in order is cut before the
+ * first such step, a length or count outside the buffers held inside them; both raise *status
+ * (may be NULL) to 2. */
+typedef struct ppyb200_accept_args {
+  const void *q;
+  const float *lse;
+  void *keys, *values;
+  float *weights;
+  int32_t *positions;
+  const int32_t *lengths, *seen, *path, *accepted;
+  int32_t *status;
+  int64_t dtype, layers, batch, nodes, steps, heads, kv_heads, head_dim, capacity;
+  int64_t q_strides[4], keys_strides[4], values_strides[4], weights_strides[3];
+  double scale;
+} ppyb200_accept_args;
+
+int32_t ppyb200_accept(const ppyb200_accept_args *args);
+
+/* Every key head of sequences longer than `budget` keeps `budget` entries: those with a position
+ * of at least seen[b] - recent first, then by weight from the largest, NaN last; the lowest slot
+ * first among equals. Kept entries in slots below the budget stay; those behind it fill the
+ * holes, both in ascending order, keys and values in place. weights_out and positions_out (slots
+ * 0 .. min(length, budget) are written; they may be weights and positions themselves, and
+ * overlap them in no other way) get the kept entries' values, kept [layers][batch][kv_heads]
+ * [budget] the slot each came from (-1 behind the length). lengths are left to the caller: they
+ * become min(length, budget). Strides in elements as for ppyb200_accept; weights and positions
+ * share theirs, and so do weights_out and positions_out. 16-bit elements, head_dim a multiple of
+ * 8, rows on 16-byte boundaries. A length outside the buffers is held inside them and raises
+ * *status (may be NULL) to 2. The workspace as for ppyb200_tree_attention. */
+typedef struct ppyb200_evict_args {
+  void *keys, *values;
+  const float *weights;
+  const int32_t *positions;
+  float *weights_out;
+  int32_t *positions_out;
+  int32_t *kept;
+  const int32_t *lengths, *seen;
+  int32_t *status;
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t layers, batch, kv_heads, head_dim, capacity, budget, recent;
+  int64_t keys_strides[4], values_strides[4], weights_strides[3], out_strides[3];
+} ppyb200_evict_args;
+
+int64_t ppyb200_evict_workspace(const ppyb200_evict_args *args);
+int32_t ppyb200_evict(const ppyb200_evict_args *args);
+
+/* The embedding of a tree's nodes: x[b, i] = wte[ids[b, i]] + wpe[seen[b] + depth(i)], depth the
+ * number of ancestors (parents as for ppyb200_tree_attention, parents_stride between
+ * sequences). Nodes at and behind counts[b] (NULL: none) get zeros. An id outside [0, vocab), a
+ * position outside [0, context) or a parent that is no earlier node gives zeros and raises
+ * *status (may be NULL) to 2. width % 8 == 0, 16-byte aligned tables and x. */
+int32_t ppyb200_gpt2_embed_tree(const int64_t *ids, const int32_t *parents,
+                                int64_t parents_stride, const int32_t *counts,
+                                const int32_t *seen, const uint16_t *wte, const uint16_t *wpe,
+                                float *x, int64_t batch, int64_t nodes, int64_t width,
+                                int64_t vocab, int64_t context, int32_t *status);
+
+/* ---------------------------------------------------------------- scoring logits */
+
+#define PPYB200_TOP_LIMIT 64
+
+/* For each of `rows` rows of `vocab` logits (dtype PPYB200_F32, _BF16 or _F16; rows `pitch`
+ * elements apart, at any element): logprobs[r][i] = x[tokens[r][i]] - log sum e^x for `given`
+ * tokens a row (a token outside [0, vocab) gives NaN), entropy[r] = - sum p log p (may be NULL),
+ * and the `top` (0 .. 64, at most vocab) largest logits: their log probabilities and indices,
+ * largest first, the lowest index first among equals, NaN above every number. -inf logits have
+ * probability 0; a row with a NaN or +inf, or with no logit above -inf, has NaN log probabilities
+ * and entropy. f32 sums. Device pointers; enqueued on the current stream. No counterpart in the
+ * reference, which returns GPT-2's logits (examples/46_gpt2/gpt2.ppy:241). */
+int32_t ppyb200_token_logprobs(const void *logits, int64_t dtype, int64_t rows, int64_t vocab,
+                               int64_t pitch, const int64_t *tokens, int64_t given, int64_t top,
+                               float *logprobs, float *entropy, float *top_logprobs,
+                               int64_t *top_tokens);
+
 /* ---------------------------------------------------------------- tensor parallel over NVLink */
 
 /* Bytes of the handle ppyb200_shared_alloc writes (a cudaIpcMemHandle_t). */

@@ -75,6 +75,58 @@ __global__ void __launch_bounds__(256) embed_kernel(const int64_t* __restrict__ 
   dst[1] = hi;
 }
 
+// x[b, i] = wte[ids[b, i]] + wpe[seen[b] + depth(i)] for the nodes of drafted trees; zeros behind
+// a sequence's nodes and where an index is out of range. The depth is a walk up the parents (few
+// steps: a drafted tree is shallow), done by each of a node's threads for itself.
+__global__ void __launch_bounds__(256)
+embed_tree_kernel(const int64_t* __restrict__ ids, const int32_t* __restrict__ parents,
+                  int64_t parents_stride, const int32_t* __restrict__ counts,
+                  const int32_t* __restrict__ seen, const __nv_bfloat16* __restrict__ wte,
+                  const __nv_bfloat16* __restrict__ wpe, float* __restrict__ x, int64_t batch,
+                  int64_t nodes, int64_t width, int64_t vocab, int64_t context,
+                  int32_t* status) {
+  ppyb200::pdl_wait();  // the previous kernel may still read x
+  const int64_t groups = width / 8;
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (at >= batch * nodes * groups) return;
+  const int64_t t = at / groups, c = (at % groups) * 8, b = t / nodes, i = t % nodes;
+  float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+  if (counts == nullptr || i < counts[b]) {
+    int64_t depth = i;
+    bool good = true;
+    if (parents != nullptr) {
+      const int32_t* up = parents + b * parents_stride;
+      depth = 0;
+      for (int64_t n = i;;) {
+        const int32_t p = up[n];
+        if (p < 0 || p >= n) {
+          good = p == -1;
+          break;
+        }
+        n = p;
+        ++depth;
+      }
+    }
+    const int64_t id = ids[t], position = seen[b] + depth;
+    if (good && id >= 0 && id < vocab && position >= 0 && position < context) {
+      const uint4 te = __ldg(reinterpret_cast<const uint4*>(wte + id * width + c));
+      const uint4 pe = __ldg(reinterpret_cast<const uint4*>(wpe + position * width + c));
+      const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(&te);
+      const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&pe);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = __bfloat162float(p[k]) + __bfloat162float(q[k]);
+      lo = make_float4(v[0], v[1], v[2], v[3]);
+      hi = make_float4(v[4], v[5], v[6], v[7]);
+    } else if (status != nullptr) {
+      atomicMax(status, PPYB200_DEVICE_RAISED);
+    }
+  }
+  float4* dst = reinterpret_cast<float4*>(x + t * width + c);
+  dst[0] = lo;
+  dst[1] = hi;
+}
+
 // ---------------------------------------------------------------- linear epilogues
 
 // tanh on the SFU (PTX tanh.approx.f32, max relative error about 2^-11): the GELU output is
@@ -345,6 +397,25 @@ int32_t ppyb200_gpt2_embed(const int64_t* ids, const uint16_t* wte, const uint16
       reinterpret_cast<const __nv_bfloat16*>(wte), reinterpret_cast<const __nv_bfloat16*>(wpe), x,
       tokens, length, width, vocab, status);
   return finish(e, "ppyb200_gpt2_embed", 1);
+}
+
+int32_t ppyb200_gpt2_embed_tree(const int64_t* ids, const int32_t* parents,
+                                int64_t parents_stride, const int32_t* counts,
+                                const int32_t* seen, const uint16_t* wte, const uint16_t* wpe,
+                                float* x, int64_t batch, int64_t nodes, int64_t width,
+                                int64_t vocab, int64_t context, int32_t* status) {
+  if (batch <= 0 || nodes <= 0) return PPYB200_OK;
+  if (width <= 0 || width % 8 != 0 || !aligned16(wte) || !aligned16(wpe) || !aligned16(x)) {
+    ppyb200_set_error("ppyb200_gpt2_embed_tree: width % 8 == 0 and 16-byte aligned tables "
+                      "required");
+    return PPYB200_RAISED;
+  }
+  const int64_t work = batch * nodes * (width / 8);
+  const cudaError_t e = ppyb200::launch_pdl(
+      embed_tree_kernel, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, stream_now(), ids,
+      parents, parents_stride, counts, seen, reinterpret_cast<const __nv_bfloat16*>(wte),
+      reinterpret_cast<const __nv_bfloat16*>(wpe), x, batch, nodes, width, vocab, context, status);
+  return finish(e, "ppyb200_gpt2_embed_tree", 1);
 }
 
 int32_t ppyb200_linear_bf16(const uint16_t* a, const uint16_t* w, const float* bias,

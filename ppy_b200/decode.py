@@ -1,0 +1,359 @@
+"""Decoding with a cache: attention of drafted trees, acceptance, eviction.
+
+    cache = KVCache(layers, batch, heads, head_dim, capacity)
+    out, lse = tree_attention(q, k, v, cache.keys[i], cache.values[i], cache.lengths, parents)
+    cache.accept(path, accepted)        # the verified path of the last attention joins the cache
+    cache.evict(budget, recent=64)      # entries of least accumulated attention weight give way
+
+`tree_attention`, `accept_nodes` and `evict` are the operators, on torch CUDA tensors (storage
+only: the work is this package's kernels, through ppyb200_tree_attention, ppyb200_accept and
+ppyb200_evict); `KVCache` holds the state that belongs together. A single token is a tree of one
+node, and a piece of a prompt is a chain (`parents=None`).
+
+Calls are asynchronous on the thread's stream (`runtime.set_stream`), ordered with torch's current
+stream (`runtime.launches_beside_torch`), and read sequence lengths on the device, so that they can
+be captured into a CUDA graph and replayed as the cache grows. Each call's workspace is a torch
+allocation of its own: calls on several streams and captured graphs share none.
+"""
+
+from __future__ import annotations
+
+import functools
+import math
+import struct
+
+from . import runtime
+from .runtime import B200Error
+
+__all__ = ["KVCache", "accept_nodes", "evict", "tree_attention"]
+
+#: The header's limits (include/ppyb200.h).
+TREE_NODES, PATH_STEPS, PATH_ROWS = 256, 64, 512
+
+_ATTENTION = struct.Struct("=39qd")  # ppyb200_tree_attention_args
+_ACCEPT = struct.Struct("=35qd")  # ppyb200_accept_args
+_EVICT = struct.Struct("=33q")  # ppyb200_evict_args
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+@functools.cache
+def _kinds() -> dict:
+    torch = _torch()
+    return {torch.bfloat16: 1, torch.float16: 2}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise B200Error(what)
+
+
+def _element_rows(name: str, t, shape, dtype, device) -> None:
+    """A tensor of `shape` and `dtype` on `device` with unit stride along its last axis."""
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or (
+            t.stride(-1) != 1 and shape[-1] > 1):
+        raise B200Error(f"{name}: {dtype} {list(shape)} on {device}, unit stride along the last "
+                        f"axis (not {t.dtype} {list(t.shape)} on {t.device}, strides "
+                        f"{list(t.stride())})")
+
+
+def _whole(name: str, t, shape, dtype, device) -> None:
+    """A contiguous tensor of `shape` and `dtype` on `device`."""
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or (
+            not t.is_contiguous()):
+        raise B200Error(f"{name}: contiguous {dtype} {list(shape)} on {device} (not {t.dtype} "
+                        f"{list(t.shape)} on {t.device}, strides {list(t.stride())})")
+
+
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(device, dtype, batch, nodes, heads, kv_heads, head_dim,
+                         capacity) -> int:
+    return runtime.library().ppyb200_tree_attention_workspace(_ATTENTION.pack(
+        *(0,) * 13, dtype, batch, nodes, heads, kv_heads, head_dim, capacity, *(0,) * 19, 1.0))
+
+
+def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=None, scale=None,
+                   out=None, lse=None, status=None):
+    """Attend from drafted nodes to their sequences' caches and to their own ancestors, and append
+    the nodes to the caches. Returns (out, lse).
+
+    q [batch, nodes, heads, head_dim], k_new and v_new [batch, nodes, kv_heads, head_dim]; keys and
+    values [batch, kv_heads, capacity, head_dim], any strides (a view of a token-major cache, one
+    layer of a KVCache); lengths int32 [batch], the entries of each cache; parents int32 [batch,
+    nodes] or [nodes]: parents[b, i] < i is node i's parent, -1 hangs it off the last entry; None
+    makes the nodes a chain. counts int32 [batch] gives each sequence's real nodes (all without
+    it). Scores are scale * q . k (1 / sqrt(head_dim) by default).
+
+    out [batch, nodes, heads, head_dim] of q's type and lse f32 [batch, heads, nodes], the natural
+    log of the sum of e^score of each row (made here unless given; behind a sequence's nodes they
+    are left as they were, zeros when made here). Node i is written to slot lengths[b] + i of keys
+    and values; `lengths` stay as they are (`accept_nodes` says which nodes join).
+
+    bf16 or f16; head_dim a multiple of 8 up to 128; rows on 16-byte boundaries; up to 256 nodes with
+    parents. `status` (int32 [1], optional) is raised to 2 when a length, count or parent is out of
+    range: the call then keeps to the buffers, and takes such a parent for -1."""
+    torch = _torch()
+    kind, device = _kinds().get(q.dtype), q.device
+    _need(kind is not None and q.is_cuda and q.dim() == 4 and keys.dim() == 4,
+          "q: bf16 or f16 [batch, nodes, heads, head_dim], keys [batch, kv_heads, capacity, "
+          "head_dim], on a CUDA device")
+    batch, nodes, heads, d = q.shape
+    kv_heads, capacity = keys.shape[1], keys.shape[2]
+    _element_rows("q", q, (batch, nodes, heads, d), q.dtype, device)
+    _element_rows("k_new", k_new, (batch, nodes, kv_heads, d), q.dtype, device)
+    _element_rows("v_new", v_new, (batch, nodes, kv_heads, d), q.dtype, device)
+    _element_rows("keys", keys, (batch, kv_heads, capacity, d), q.dtype, device)
+    _element_rows("values", values, (batch, kv_heads, capacity, d), q.dtype, device)
+    _whole("lengths", lengths, (batch,), torch.int32, device)
+    parents_stride = 0
+    if parents is not None:
+        shared = parents.dim() == 1
+        _whole("parents", parents, (nodes,) if shared else (batch, nodes), torch.int32, device)
+        parents_stride = 0 if shared else nodes
+    if counts is not None:
+        _whole("counts", counts, (batch,), torch.int32, device)
+    if status is not None:
+        _whole("status", status, (1,), torch.int32, device)
+    with runtime.launches_beside_torch(device.index) as launch:
+        make = torch.empty if counts is None else torch.zeros
+        made = []
+        if out is None:
+            out = make((batch, nodes, heads, d), dtype=q.dtype, device=device)
+            made.append(out)
+        else:
+            _element_rows("out", out, (batch, nodes, heads, d), q.dtype, device)
+        if lse is None:
+            lse = make((batch, heads, nodes), dtype=torch.float32, device=device)
+            made.append(lse)
+        else:
+            _whole("lse", lse, (batch, heads, nodes), torch.float32, device)
+        if launch.side is not None and made:  # zeros were written on torch's stream
+            launch.side.wait_stream(torch.cuda.current_stream())
+        size = _attention_workspace(device.index, kind, batch, nodes, heads, kv_heads, d,
+                                    capacity)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        args = _ATTENTION.pack(
+            q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), keys.data_ptr(), values.data_ptr(),
+            lengths.data_ptr(), _address(parents), _address(counts), out.data_ptr(),
+            lse.data_ptr(), _address(status), _address(workspace), size, kind, batch, nodes,
+            heads, kv_heads, d, capacity, *q.stride()[:3], *k_new.stride()[:3],
+            *v_new.stride()[:3], *keys.stride()[:3], *values.stride()[:3], *out.stride()[:3],
+            parents_stride, 1.0 / math.sqrt(d) if scale is None else scale)
+        if runtime.library().ppyb200_tree_attention(args) != runtime.STATUS_OK:
+            raise B200Error(runtime.last_error())
+        if launch.side is not None:
+            for t in (*made, workspace):
+                if t is not None:
+                    t.record_stream(launch.side)
+    return out, lse
+
+
+def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, accepted,
+                 scale=None, status=None) -> None:
+    """The verified path of the last attention joins the caches of every layer, in place.
+
+    q [layers, batch, nodes, heads, head_dim] and lse f32 [layers, batch, heads, nodes] are that
+    attention's; keys and values [layers, batch, kv_heads, capacity, head_dim] hold its nodes
+    behind `lengths` (int32 [batch]). path int32 [batch, steps]: the accepted nodes in ascending
+    order, the first accepted[b] (int32 [batch]) of row b; up to 64 steps, steps times query heads
+    a key head up to 512 (`KVCache.accept` takes longer ones in pieces).
+
+    weights f32 [layers, batch, kv_heads, capacity] (None: not kept) grow by the attention that
+    the path's rows paid to each entry, summed over the query heads of the key head; the path's
+    keys and values move to slots lengths[b], lengths[b] + 1, ..., their weights start with what
+    the path paid them, and positions (int32, laid out as weights; None: not kept) get seen[b],
+    seen[b] + 1, ... (`seen` int32 [batch]: the tokens before them). lengths and seen are the
+    caller's to advance. `status` as in tree_attention: raised when the path is not in order (it is
+    cut there) or a length or count is out of range."""
+    torch = _torch()
+    kind, device = _kinds().get(keys.dtype), keys.device
+    _need(kind is not None and keys.is_cuda and keys.dim() == 5 and q.dim() == 5,
+          "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim], q [layers, batch, "
+          "nodes, heads, head_dim], on a CUDA device")
+    layers, batch, kv_heads, capacity, d = keys.shape
+    nodes, heads = q.shape[2], q.shape[3]
+    steps = path.shape[-1]
+    _element_rows("q", q, (layers, batch, nodes, heads, d), keys.dtype, device)
+    _element_rows("keys", keys, tuple(keys.shape), keys.dtype, device)
+    _element_rows("values", values, tuple(keys.shape), keys.dtype, device)
+    if weights is not None:
+        _whole("lse", lse, (layers, batch, heads, nodes), torch.float32, device)
+    for name, t in (("lengths", lengths), ("seen", seen), ("accepted", accepted)):
+        _whole(name, t, (batch,), torch.int32, device)
+    _whole("path", path, (batch, steps), torch.int32, device)
+    tables = weights if weights is not None else positions
+    strides = (0, 0, 0)
+    for name, t, kept in (("weights", weights, torch.float32),
+                          ("positions", positions, torch.int32)):
+        if t is not None:
+            _element_rows(name, t, (layers, batch, kv_heads, capacity), kept, device)
+            _need(t.stride() == tables.stride(), "weights and positions are laid out alike")
+            strides = t.stride()[:3]
+    if status is not None:
+        _whole("status", status, (1,), torch.int32, device)
+    with runtime.launches_beside_torch(device.index):
+        args = _ACCEPT.pack(
+            q.data_ptr(), lse.data_ptr(), keys.data_ptr(), values.data_ptr(), _address(weights),
+            _address(positions), lengths.data_ptr(), seen.data_ptr(), path.data_ptr(),
+            accepted.data_ptr(), _address(status), kind, layers, batch, nodes, steps, heads,
+            kv_heads, d, capacity, *q.stride()[:4], *keys.stride()[:4], *values.stride()[:4],
+            *strides, 1.0 / math.sqrt(d) if scale is None else scale)
+        if runtime.library().ppyb200_accept(args) != runtime.STATUS_OK:
+            raise B200Error(runtime.last_error())
+
+
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(layers, batch, kv_heads, head_dim, capacity, budget) -> int:
+    return runtime.library().ppyb200_evict_workspace(_EVICT.pack(
+        *(0,) * 12, layers, batch, kv_heads, head_dim, capacity, budget, *(0,) * 15))
+
+
+def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, weights_out=None,
+          positions_out=None, status=None):
+    """Cut every key head's cache to `budget` entries, keys and values in place. Returns `kept`,
+    int32 [layers, batch, kv_heads, budget]: the slot that each entry came from, -1 behind a
+    sequence's entries.
+
+    keys and values [layers, batch, kv_heads, capacity, head_dim]; weights f32 and positions int32
+    [layers, batch, kv_heads, capacity]; lengths, seen int32 [batch]. Entries at positions
+    seen[b] - recent and later stay first, then those of largest weight (NaN last; the lowest
+    slot first among equals). Kept entries in slots below the budget stay where they are; those
+    behind it move into the holes, both in ascending order, so slots are in no order of position
+    afterwards. The kept entries' weights and positions go to weights_out and positions_out
+    [layers, batch, kv_heads, at least budget], the tables themselves by default. Sequences of up to `budget` entries
+    keep them all. lengths are the caller's to set to min(lengths, budget)."""
+    torch = _torch()
+    device = keys.device
+    _need(keys.dtype in _kinds() and keys.is_cuda and keys.dim() == 5,
+          "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim] on a CUDA device")
+    layers, batch, kv_heads, capacity, d = keys.shape
+    budget, recent = int(budget), int(recent)
+    _need(0 < budget <= capacity and recent >= 0,
+          "a budget of 1 up to the capacity, and recent not negative")
+    _element_rows("keys", keys, tuple(keys.shape), keys.dtype, device)
+    _element_rows("values", values, tuple(keys.shape), keys.dtype, device)
+    _element_rows("weights", weights, (layers, batch, kv_heads, capacity), torch.float32, device)
+    _element_rows("positions", positions, (layers, batch, kv_heads, capacity), torch.int32,
+                  device)
+    _need(weights.stride() == positions.stride(), "weights and positions are laid out alike")
+    weights_out = weights if weights_out is None else weights_out
+    positions_out = positions if positions_out is None else positions_out
+    width = weights_out.shape[-1]
+    _need(width >= budget, "weights_out: at least budget entries a head")
+    _element_rows("weights_out", weights_out, (layers, batch, kv_heads, width), torch.float32,
+                  device)
+    _element_rows("positions_out", positions_out, (layers, batch, kv_heads, width), torch.int32,
+                  device)
+    _need(weights_out.stride() == positions_out.stride(),
+          "weights_out and positions_out are laid out alike")
+    for name, t in (("lengths", lengths), ("seen", seen)):
+        _whole(name, t, (batch,), torch.int32, device)
+    if status is not None:
+        _whole("status", status, (1,), torch.int32, device)
+    with runtime.launches_beside_torch(device.index) as launch:
+        kept = torch.empty((layers, batch, kv_heads, budget), dtype=torch.int32, device=device)
+        size = _evict_workspace(layers, batch, kv_heads, d, capacity, budget)
+        workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
+        if launch.side is not None:
+            kept.record_stream(launch.side)
+            workspace.record_stream(launch.side)
+        args = _EVICT.pack(
+            keys.data_ptr(), values.data_ptr(), weights.data_ptr(), positions.data_ptr(),
+            weights_out.data_ptr(), positions_out.data_ptr(), kept.data_ptr(),
+            lengths.data_ptr(), seen.data_ptr(), _address(status), workspace.data_ptr(),
+            workspace.numel(), layers, batch, kv_heads, d, capacity, budget, recent,
+            *keys.stride()[:4], *values.stride()[:4], *weights.stride()[:3],
+            *weights_out.stride()[:3])
+        if runtime.library().ppyb200_evict(args) != runtime.STATUS_OK:
+            raise B200Error(runtime.last_error())
+    return kept
+
+
+class KVCache:
+    """Keys and values of `batch` sequences over `layers` layers, with what decoding keeps beside
+    them, as plain torch tensors:
+
+        keys, values   [layers, batch, heads, capacity, head_dim]
+        weights        f32 [layers, batch, heads, capacity], accumulated attention weights
+                       (None with weights=False: nothing is accumulated or evicted)
+        positions      int32, laid out as weights: the token position of each entry
+        lengths, seen  int32 [batch]: entries in the cache, and tokens accepted so far
+
+    `pending` is what the last extension left for `accept`: its queries [layers, batch, nodes,
+    query heads, head_dim] and log-sum-exps f32 [layers, batch, query heads, nodes]."""
+
+    def __init__(self, layers: int, batch: int, heads: int, head_dim: int, capacity: int,
+                 dtype=None, device="cuda", weights: bool = True) -> None:
+        torch = _torch()
+        dtype = torch.bfloat16 if dtype is None else dtype
+        _need(dtype in _kinds(), "a cache of bf16 or f16")
+        shape = (layers, batch, heads, capacity)
+        self.keys = torch.zeros(*shape, head_dim, dtype=dtype, device=device)
+        self.values = torch.zeros_like(self.keys)
+        self.weights = torch.zeros(shape, dtype=torch.float32, device=device) if weights else None
+        self.positions = torch.zeros(shape, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.seen = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.pending = None
+        self.buffers: dict = {}  # an extension's activations, by its shape
+
+    @property
+    def capacity(self) -> int:
+        return self.keys.shape[3]
+
+    def reset(self) -> None:
+        """Forget every sequence."""
+        self.lengths.zero_()
+        self.seen.zero_()
+        self.status.zero_()
+        self.pending = None
+
+    def check(self) -> None:
+        """Raise if an index given to a call since the last check was out of range (syncs)."""
+        if int(self.status.item()) != 0:
+            self.status.zero_()
+            raise B200Error("a length, count, parent, path, position or token id was out of range")
+
+    def accept(self, path=None, accepted=None) -> None:
+        """The nodes path[b, :accepted[b]] of the last extension (int32 [batch, steps] and
+        [batch], as `accept_nodes`; all nodes without a path, each sequence's first accepted[b]
+        of them) join the cache: lengths and seen grow by `accepted`. Paths longer than
+        accept_nodes takes go in pieces."""
+        torch = _torch()
+        _need(self.pending is not None, "accept follows an extension")
+        q, lse = self.pending
+        batch, nodes, heads = q.shape[1], q.shape[2], q.shape[3]
+        device = self.keys.device
+        if path is None:
+            path = torch.arange(nodes, dtype=torch.int32, device=device).expand(batch, nodes)
+        if accepted is None:
+            accepted = torch.full((batch,), path.shape[1], dtype=torch.int32, device=device)
+        most = min(PATH_STEPS, PATH_ROWS // (heads // self.keys.shape[2]))
+        for at in range(0, path.shape[1], most):
+            part = path[:, at:at + most] - at
+            count = (accepted - at).clamp(0, part.shape[1])
+            # the nodes from `at` on: a path ascends, so its step `at` is node `at` or later
+            part_lse = lse[..., at:].contiguous() if self.weights is not None else lse
+            accept_nodes(q[:, :, at:], part_lse, self.keys, self.values,
+                         self.weights, self.positions, self.lengths, self.seen,
+                         part.contiguous(), count, status=self.status)
+            self.lengths += count
+            self.seen += count
+        self.pending = None
+
+    def evict(self, budget: int, recent: int = 0):
+        """Cut every sequence to `budget` entries (see `evict`); returns `kept`."""
+        _need(self.weights is not None, "eviction takes a cache with weights")
+        kept = evict(self.keys, self.values, self.weights, self.positions, self.lengths,
+                     self.seen, budget, recent, status=self.status)
+        self.lengths.clamp_(max=budget)
+        return kept

@@ -27,7 +27,7 @@ import ctypes
 from dataclasses import dataclass
 from pathlib import Path
 
-from . import runtime
+from . import decode, runtime, scoring
 
 __all__ = ["Config", "GPT2", "GPT2_124M", "GraphedForward"]
 
@@ -55,6 +55,7 @@ def _bind(lib) -> None:
         return
     p, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
     lib.ppyb200_gpt2_embed.argtypes = [p, p, p, p, i64, i64, i64, i64, p]
+    lib.ppyb200_gpt2_embed_tree.argtypes = [p, p, i64, p, p, p, p, p, i64, i64, i64, i64, i64, p]
     lib.ppyb200_linear_bf16.argtypes = [p, p, p, p, i64, i64, i64, i32, p]
     lib.ppyb200_linear_residual.argtypes = [p, p, p, p, i64, i64, i64, p]
     lib.ppyb200_linear_qkv_bf16.argtypes = [p, p, p, p, p, i64, i64, i64, i64, p]
@@ -62,7 +63,7 @@ def _bind(lib) -> None:
     lib.ppyb200_attention_causal_vt_bf16.argtypes = [p, p, p, i64, i64, i64, i64, p]
     lib.ppyb200_matmul_bf16_kmajor.argtypes = [p, p, p, p, i64, i64, i64]
     lib.ppyb200_matmul_bf16_kmajor_ld.argtypes = [p, p, p, p, i64, i64, i64, i64]
-    for name in ("ppyb200_gpt2_embed", "ppyb200_linear_bf16", "ppyb200_linear_residual",
+    for name in ("ppyb200_gpt2_embed", "ppyb200_gpt2_embed_tree", "ppyb200_linear_bf16", "ppyb200_linear_residual",
                  "ppyb200_linear_qkv_bf16", "ppyb200_attention_causal_bf16",
                  "ppyb200_attention_causal_vt_bf16", "ppyb200_matmul_bf16_kmajor",
                  "ppyb200_matmul_bf16_kmajor_ld"):
@@ -207,6 +208,115 @@ class GPT2:
                                                       logits.data_ptr(), pitch, tokens, v, c),
                     "lm head")
         return logits
+
+    def new_cache(self, batch: int, capacity: int | None = None,
+                  weights: bool = True) -> decode.KVCache:
+        """An empty cache for `batch` sequences (`capacity` entries each, the context by default),
+        with accumulated attention weights for eviction unless weights=False."""
+        cfg = self.config
+        return decode.KVCache(cfg.layers, batch, cfg.heads, cfg.head_dim,
+                              cfg.context if capacity is None else capacity,
+                              device=self.device, weights=weights)
+
+    def extend(self, cache: decode.KVCache, ids, parents=None, counts=None, logits=None):
+        """Logits [batch, nodes, vocab] (f32, laid out as forward's) of drafted tokens `ids` (int64
+        [batch, nodes]) behind the sequences of `cache`: a tree by `parents` (int32 [batch, nodes]
+        or [nodes], as `decode.tree_attention`), or a chain -- the next token of each sequence, or a
+        prompt (piece) of any length. counts int32 [batch]: each sequence's real nodes; the logits
+        of the others mean nothing. The nodes sit behind the cache's entries until
+        `cache.accept` takes a path of them in; another extension in its place overwrites them.
+        An index out of range shows in `cache.check()`."""
+        import torch
+
+        cfg = self.config
+        batch, nodes = ids.shape
+        tokens, c, v = batch * nodes, cfg.width, cfg.vocab
+        if cfg.head_dim != cache.keys.shape[4] or cache.keys.shape[:3] != (
+                cfg.layers, batch, cfg.heads) or cache.keys.dtype != torch.bfloat16:
+            raise runtime.B200Error("a bf16 cache of this model's layers, heads and head size, and "
+                                    "of as many sequences as ids")
+        if ids.dtype != torch.int64 or ids.device != cache.keys.device or tokens == 0:
+            raise runtime.B200Error("ids: int64 [batch, nodes] on the cache's device, not empty")
+        ids = ids.contiguous()
+        stride = 0
+        if parents is not None:
+            shared = parents.dim() == 1
+            decode._whole("parents", parents, (nodes,) if shared else (batch, nodes),
+                          torch.int32, ids.device)
+            stride = 0 if shared else nodes
+        if counts is not None:
+            decode._whole("counts", counts, (batch,), torch.int32, ids.device)
+        s = cache.buffers.get((batch, nodes))
+        if s is None:
+            d = ids.device
+            layers = cfg.layers if cache.weights is not None else 1
+            s = {"x": torch.empty(tokens, c, dtype=torch.float32, device=d),
+                 "h": torch.empty(tokens, c, dtype=torch.bfloat16, device=d),
+                 "qkv": torch.empty(layers, tokens, 3 * c, dtype=torch.bfloat16, device=d),
+                 "lse": torch.zeros(layers, batch, cfg.heads, nodes, device=d),
+                 # rows behind a sequence's nodes are left alone: zeros from the start
+                 "att": torch.zeros(tokens, c, dtype=torch.bfloat16, device=d),
+                 "f": torch.empty(tokens, 4 * c, dtype=torch.bfloat16, device=d)}
+            cache.buffers[(batch, nodes)] = s
+        x, h, att, f, lib = s["x"], s["h"], s["att"], s["f"], self.lib
+        if logits is None:
+            logits = self.new_logits(batch, nodes)
+        pitch = self._row_pitch(logits, batch, nodes, v)
+        ln = self.layernorm.device.layernorm_bf16
+        heads = (batch, nodes, 3, cfg.heads, cfg.head_dim)
+        with runtime.launches_beside_torch(ids.device.index) as launch:
+            if launch.side is not None:
+                logits.record_stream(launch.side)
+                ids.record_stream(launch.side)
+            st = cache.status.data_ptr()
+            self._check(lib.ppyb200_gpt2_embed_tree(
+                ids.data_ptr(), parents.data_ptr() if parents is not None else None, stride,
+                counts.data_ptr() if counts is not None else None, cache.seen.data_ptr(),
+                self.wte.data_ptr(), self.wpe.data_ptr(), x.data_ptr(), batch, nodes, c, v,
+                cfg.context, st), "embed")
+            for i, blk in enumerate(self.blocks):
+                qkv = s["qkv"][i % len(s["qkv"])]
+                lse = s["lse"][i % len(s["lse"])]
+                self._check(ln(x, blk["ln1_g"], blk["ln1_b"], h).status, "layernorm")
+                self._check(lib.ppyb200_linear_bf16(h.data_ptr(), blk["w_qkv"].data_ptr(),
+                                                    blk["b_qkv"].data_ptr(), qkv.data_ptr(),
+                                                    tokens, 3 * c, c, 0, st), "qkv")
+                q, k, value = qkv.view(heads).unbind(2)
+                decode.tree_attention(q, k, value, cache.keys[i], cache.values[i], cache.lengths,
+                                      parents, counts, out=att.view(batch, nodes, cfg.heads, -1),
+                                      lse=lse, status=cache.status)
+                self._check(lib.ppyb200_linear_residual(att.data_ptr(), blk["w_o"].data_ptr(),
+                                                        blk["b_o"].data_ptr(), x.data_ptr(),
+                                                        tokens, c, c, st), "out projection")
+                self._check(ln(x, blk["ln2_g"], blk["ln2_b"], h).status, "layernorm")
+                self._check(lib.ppyb200_linear_bf16(h.data_ptr(), blk["w_fc"].data_ptr(),
+                                                    blk["b_fc"].data_ptr(), f.data_ptr(),
+                                                    tokens, 4 * c, c, 1, st), "fc")
+                self._check(lib.ppyb200_linear_residual(f.data_ptr(), blk["w_proj"].data_ptr(),
+                                                        blk["b_proj"].data_ptr(), x.data_ptr(),
+                                                        tokens, c, 4 * c, st), "proj")
+            self._check(ln(x, self.lnf_g, self.lnf_b, h).status, "layernorm")
+            self._check(lib.ppyb200_matmul_bf16_kmajor_ld(h.data_ptr(), self.wte.data_ptr(), None,
+                                                          logits.data_ptr(), pitch, tokens, v, c),
+                        "lm head")
+        # without weights one layer's queries stand for all: `accept` only moves rows then
+        queries = s["qkv"].view(-1, *heads)[:, :, :, 0]
+        lse = s["lse"]
+        cache.pending = (queries.expand(cfg.layers, *queries.shape[1:]),
+                         lse.expand(cfg.layers, *lse.shape[1:]))
+        return logits
+
+    def score(self, ids, top: int = 0, logits=None) -> scoring.TokenLogprobs:
+        """Log probabilities of tokens 1, 2, ... of `ids` [batch, length] given those before them,
+        the entropy of each prediction and its `top` alternatives (`scoring.token_logprobs`), all
+        [batch, length - 1, ...], from one forward (`logits` as for it)."""
+        import torch
+
+        logits = self.forward(ids, logits)
+        following = torch.full_like(ids, -1, memory_format=torch.contiguous_format)
+        following[:, :-1] = ids[:, 1:]
+        scored = scoring.token_logprobs(logits, following, top)
+        return scoring.TokenLogprobs(*(t[:, :-1] for t in scored))
 
     def profile(self, ids, logits=None) -> dict:
         """One forward with CUDA events around every call: {kernel: [launches, ms, flops]}.

@@ -76,6 +76,17 @@ def library() -> ctypes.CDLL:
         lib.ppyb200_device_buffer.restype = ctypes.c_void_p
         lib.ppyb200_device_buffer.argtypes = [ctypes.c_int64]
         lib.ppyb200_release_buffer.argtypes = [ctypes.c_void_p]
+        # decoding and scoring: arguments packed as the header's structures (bytes)
+        for name in ("ppyb200_tree_attention", "ppyb200_accept", "ppyb200_evict"):
+            getattr(lib, name).argtypes = [ctypes.c_char_p]
+            getattr(lib, name).restype = ctypes.c_int32
+        for name in ("ppyb200_tree_attention_workspace", "ppyb200_evict_workspace"):
+            getattr(lib, name).argtypes = [ctypes.c_char_p]
+            getattr(lib, name).restype = ctypes.c_int64
+        lib.ppyb200_token_logprobs.argtypes = (
+            [ctypes.c_void_p] + [ctypes.c_int64] * 4 + [ctypes.c_void_p]
+            + [ctypes.c_int64] * 2 + [ctypes.c_void_p] * 4)
+        lib.ppyb200_token_logprobs.restype = ctypes.c_int32
         _library = lib
         return lib
 
@@ -102,6 +113,47 @@ def set_stream(stream) -> None:
         return
     handle = int(getattr(stream, "cuda_stream", stream) or 0)
     library().ppyb200_set_stream(ctypes.c_void_p(handle or _LEGACY_STREAM))
+
+
+class launches_beside_torch:
+    """Context of a call that launches on this thread's stream (set_stream) with torch tensors
+    of device `index`: the thread's device has to be theirs (a thread without one is bound to
+    it), and is the current one inside. Where torch's current stream is another than the
+    thread's, the call waits for the work already on torch's stream and torch's stream for the
+    call's, so the tensors are the caller's to use as if the call had run on it; `side` is the
+    thread's stream then, for tensors made inside (record_stream), else None."""
+
+    __slots__ = ("_guard", "_stream", "side")
+
+    def __init__(self, index: int) -> None:
+        import torch
+
+        lib = library()
+        bound = lib.ppyb200_current_device()
+        self._guard = None
+        if bound != index and bound >= 0:
+            raise B200Error(f"tensors on cuda:{index}, but this thread's device is {bound} "
+                            "(runtime.init)")
+        if torch.cuda.current_device() != index:
+            self._guard = torch.cuda.device(index)
+            self._guard.__enter__()
+        if bound < 0:
+            init(index)
+        self._stream, self.side = torch.cuda.current_stream(index), None
+        handle = lib.ppyb200_stream() or 0
+        if handle != (self._stream.cuda_stream or _LEGACY_STREAM):
+            self.side = (torch.cuda.default_stream(index) if handle == _LEGACY_STREAM
+                         else torch.cuda.ExternalStream(handle, index))
+            self.side.wait_stream(self._stream)
+
+    def __enter__(self) -> "launches_beside_torch":
+        return self
+
+    def __exit__(self, *exc) -> None:
+        if self.side is not None:
+            self._stream.wait_stream(self.side)
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
 
 
 def device_allocations() -> int:

@@ -1,0 +1,90 @@
+"""Scoring logits: log probabilities of given tokens, entropy, and the likeliest alternatives.
+
+`token_logprobs` reads each row of logits once (ppyb200_token_logprobs): rows as the LM head writes
+them (`GPT2.new_logits`, `GPT2.forward`, `GPT2.extend`), or any evenly spaced rows of f32, bf16 or
+f16."""
+
+from __future__ import annotations
+
+import functools
+from typing import NamedTuple
+
+from . import runtime
+from .runtime import B200Error
+
+__all__ = ["TokenLogprobs", "token_logprobs"]
+
+TOP_LIMIT = 64  # PPYB200_TOP_LIMIT
+
+
+class TokenLogprobs(NamedTuple):
+    """logprobs f32, shaped as the tokens; entropy f32 [...]; top_logprobs f32 and top_tokens int64
+    [..., top], the largest first."""
+
+    logprobs: object
+    entropy: object
+    top_logprobs: object
+    top_tokens: object
+
+
+@functools.cache
+def _kinds() -> dict:
+    import torch
+
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows(logits) -> tuple[int, int]:
+    """(rows, distance between rows) of [..., vocab] logits with evenly spaced rows."""
+    shape, strides = logits.shape, logits.stride()
+    rows, pitch = 1, 0
+    for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if size != 1:
+            if rows > 1 and stride != pitch * rows:
+                return logits.numel() // shape[-1], -1
+            pitch = stride if rows == 1 else pitch
+        rows *= size
+    return rows, pitch if rows > 1 else shape[-1]
+
+
+def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of `tokens` under `logits` [..., vocab], each row's entropy (nats), and its
+    `top` likeliest tokens (0 to 64) with their log probabilities.
+
+    tokens int64 [...] (one a row) or [..., given] (several a row); a token outside the vocabulary
+    (-1 where none is asked for) gives NaN. Alternatives come largest first, the lowest index
+    first among equals, NaN above every number. A logit of -inf has probability 0; a row with a NaN
+    or +inf, or with nothing above -inf, has NaN log probabilities and entropy."""
+    import torch
+
+    kind = _kinds().get(logits.dtype)
+    if kind is None or not logits.is_cuda or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise B200Error("logits: f32, bf16 or f16 [..., vocab] on a CUDA device")
+    leading, vocab, device = tuple(logits.shape[:-1]), logits.shape[-1], logits.device
+    rows, pitch = _rows(logits)
+    if pitch < vocab or (logits.stride(-1) != 1 and vocab > 1):
+        raise B200Error("logits: unit stride along the vocabulary, rows evenly spaced and at least "
+                        "vocab elements apart")
+    several = tokens.dim() == len(leading) + 1
+    if (tokens.dtype != torch.int64 or tokens.device != device or not tokens.is_contiguous()
+            or tuple(tokens.shape[:len(leading)]) != leading
+            or not (several or tokens.dim() == len(leading))):
+        raise B200Error(f"tokens: contiguous int64 {list(leading)} or {list(leading)} + [given], "
+                        f"on {device}")
+    if not 0 <= top <= min(TOP_LIMIT, vocab):
+        raise B200Error(f"top: 0 up to {TOP_LIMIT} and the vocabulary")
+    given = tokens.shape[-1] if several else 1
+    with runtime.launches_beside_torch(device.index) as launch:
+        result = TokenLogprobs(
+            torch.empty(tokens.shape, dtype=torch.float32, device=device),
+            torch.empty(leading, dtype=torch.float32, device=device),
+            torch.empty((*leading, top), dtype=torch.float32, device=device),
+            torch.empty((*leading, top), dtype=torch.int64, device=device))
+        if launch.side is not None:
+            for t in result:
+                t.record_stream(launch.side)
+        if runtime.library().ppyb200_token_logprobs(
+                logits.data_ptr(), kind, rows, vocab, pitch, tokens.data_ptr(), given, top,
+                *(t.data_ptr() for t in result)) != runtime.STATUS_OK:
+            raise B200Error(runtime.last_error())
+    return result
