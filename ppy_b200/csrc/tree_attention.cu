@@ -6,10 +6,11 @@
 //   s_ij = scale q_i . k_j,  lse_i = log sum_visible e^{s_ij},  out_i = sum e^{s_ij - lse_i} v_j
 //
 // The rows of one key head (nodes x the query heads that share it) form the M side of the
-// products; tiles of 64 keys stream through shared memory once per 16, 32, 64 or 128 rows with
-// a running maximum and sum (f32). A long axis of keys is split over CTAs: each leaves its
-// unnormalised f32 output with its maximum and sum in the workspace, and a second kernel joins
-// them in split order, so results do not depend on timing.
+// products. Two kernels: the one here streams tiles of 64 keys through shared memory for 16 (or
+// 64) rows a CTA with warp-level products, and tree_attention_sm100.cuh holds the tensor-core
+// kernel for many rows. Both keep a running maximum and sum (f32). The key tiles of all sequences
+// are dealt to the CTAs in parts of equal size; a sequence of several parts is joined by a
+// second kernel in the order of its parts, so results do not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -20,42 +21,23 @@
 #include "../../include/ppyb200.h"
 #include "mma16.cuh"
 #include "ppyb200_device.cuh"
+#include "tree_attention.cuh"
+#include "tree_attention_sm100.cuh"
 
 namespace {
 
 using namespace ppyb200::mma16;
+using ppyb200::tree::Args;
+using ppyb200::tree::Deal;
+using ppyb200::tree::Part;
+using ppyb200::tree::Results;
+using ppyb200::tree::WideRows;
+using ppyb200::tree::raise;
+using ppyb200::tree::sequence_extent;
 
 constexpr int kTile = 64;       // keys a tile
 constexpr int kStages = 3;      // tiles in flight
 constexpr int kTreeWords = PPYB200_TREE_NODES / 32;
-
-struct Shape {
-  int splits;     // CTAs along the keys
-  int row_tiles;  // CTAs along the rows of one key head
-  int group;      // query heads a key head
-};
-
-__device__ __forceinline__ void raise(int32_t* status) {
-  if (status != nullptr) atomicMax(status, PPYB200_DEVICE_RAISED);
-}
-
-// The cache length and node count of a sequence, held inside the buffers whatever the device
-// arrays say: nodes that do not fit behind the length are dropped, and the status raised.
-__device__ __forceinline__ void sequence_extent(const ppyb200_tree_attention_args& a, int b,
-                                                int64_t& length, int& count, int32_t* status) {
-  int64_t l = a.lengths[b];
-  int64_t n = a.counts != nullptr ? a.counts[b] : (int32_t)a.nodes;
-  bool bad = l < 0 || l > a.capacity || n < 0 || n > a.nodes;
-  l = l < 0 ? 0 : (l > a.capacity ? a.capacity : l);
-  n = n < 0 ? 0 : (n > a.nodes ? a.nodes : n);
-  if (l + n > a.capacity) {
-    n = a.capacity - l;
-    bad = true;
-  }
-  if (bad) raise(status);
-  length = l;
-  count = (int)n;
-}
 
 // Shared memory rows of D elements: 16-byte pieces XORed with the row's low bits, so that the
 // eight rows an ldmatrix reads lie in different banks.
@@ -66,8 +48,8 @@ __device__ __forceinline__ uint32_t row_piece(int row, int piece) {
 
 // WM warps along the rows (16 each), WK warps along a tile's keys.
 template <class T, int D, int WM, int WK>
-__global__ void __launch_bounds__(32 * WM * WK)
-tree_attention_kernel(const ppyb200_tree_attention_args a, const Shape shape, float* partial) {
+__global__ void __launch_bounds__(32 * WM * WK, WK == 1 ? 1 : D == 64 ? 4 : 2)
+narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_tiles) {
   constexpr int kThreads = 32 * WM * WK, kRows = 16 * WM, kPieces = D / 8;
   constexpr int kKeys = kTile / WK;      // keys of a tile that one warp takes
   constexpr int kTileBytes = kTile * D * 2;
@@ -79,19 +61,15 @@ tree_attention_kernel(const ppyb200_tree_attention_args a, const Shape shape, fl
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wm = warp / WK, wk = warp % WK;
   const int gid = lane >> 2, tig = lane & 3;
-  const int b = blockIdx.z;
-  const int kvh = blockIdx.y / shape.row_tiles, rt = blockIdx.y % shape.row_tiles;
-  const int group = shape.group, d = (int)a.head_dim;
-  int64_t length;
-  int count;
-  sequence_extent(a, b, length, count, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0
-                                           ? a.status : nullptr);
-  const int rows = count * group, row0 = rt * kRows;
-  if (row0 >= rows) return;
-  const int64_t total = length + count;
-  const int64_t tiles = (total + kTile - 1) / kTile;
-  const int64_t per = (tiles + shape.splits - 1) / shape.splits;
-  const int64_t t0 = blockIdx.x * per, t1 = min(tiles, t0 + per);
+  const Part part = ppyb200::tree::part_of<kTile, false>(
+      a, deal, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0 ? a.status : nullptr);
+  const int kvh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
+  const int group = (int)(a.heads / a.kv_heads), d = (int)a.head_dim, b = part.b;
+  const int64_t length = part.length;
+  const int rows = part.count * group, row0 = rt * kRows;
+  if (b < 0 || row0 >= rows) return;
+  const int64_t total = length + part.count;
+  const int64_t t0 = part.first, t1 = t0 + part.tiles;
 
   const T* q = static_cast<const T*>(a.q) + b * a.q_strides[0];
   const T* k_new = static_cast<const T*>(a.k_new) + b * a.k_new_strides[0] +
@@ -386,7 +364,7 @@ tree_attention_kernel(const ppyb200_tree_attention_args a, const Shape shape, fl
     if (r >= rows) continue;
     const float m = half == 0 ? m0 : m1, l = half == 0 ? l0 : l1;
     const int node = r / group, head = kvh * group + r % group;
-    if (shape.splits == 1) {
+    if (part.parts == 1) {
       T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
                (int64_t)head * a.out_strides[2];
       const float inv = 1.f / l;
@@ -400,48 +378,55 @@ tree_attention_kernel(const ppyb200_tree_attention_args a, const Shape shape, fl
       if (tig == 0 && a.lse != nullptr)
         a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
     } else {
-      // partial [batch][heads][nodes][splits][D + 2]
-      float* to = partial + ((((int64_t)b * a.heads + head) * a.nodes + node) * shape.splits +
-                             blockIdx.x) * (D + 2);
+      const Results results(a.workspace, a, deal, D);
+      const int64_t at = results.at(blockIdx.x, kvh, r);
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(to + n * 8 + tig * 2) =
+        *reinterpret_cast<float2*>(results.out + at * D + n * 8 + tig * 2) =
             make_float2(o[n][2 * half], o[n][2 * half + 1]);
-      if (tig == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m, l);
+      if (tig == 0) results.top[at] = make_float2(m, l);
     }
   }
 }
 
-// One warp a row: joins the splits' unnormalised outputs in split order.
-template <class T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const ppyb200_tree_attention_args a,
-                                                   const int splits, const float* partial) {
+// One warp a row: joins the parts' unnormalised outputs in their order.
+template <class T, int D, int TILE, bool APART>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a,
+                                                   const Deal deal) {
   ppyb200::pdl_wait();
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= a.batch * a.heads * a.nodes) return;
-  const int node = (int)(row % a.nodes);
-  const int head = (int)(row / a.nodes % a.heads), b = (int)(row / a.nodes / a.heads);
+  const Results results(a.workspace, a, deal, D);
+  const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, group = (int)(a.heads / a.kv_heads);
+  if (index >= a.batch * a.kv_heads * results.rows) return;
+  const int64_t row = index % results.rows;
+  const int kvh = (int)(index / results.rows % a.kv_heads);
+  const int b = (int)(index / results.rows / a.kv_heads);
+  const int node = (int)(row / group), head = kvh * group + (int)(row % group);
   int64_t length;
   int count;
   sequence_extent(a, b, length, count, nullptr);
   if (node >= count) return;
-  const float* from = partial + row * splits * (D + 2);
+  const int2 parts = ppyb200::tree::parts_of<TILE, APART>(a, deal, b);
+  if (deal.streams == 1 && parts.y == 1) return;  // written by its CTA
+  const int64_t first = (int64_t)parts.x * deal.streams, end = first + parts.y * deal.streams;
   float m = -INFINITY;
-  for (int s = lane; s < splits; s += 32) m = fmaxf(m, from[s * (D + 2) + D]);
+  for (int64_t s = first + lane; s < end; s += 32)
+    m = fmaxf(m, results.top[results.at(s, kvh, row)].x);
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
   const float u = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float* p = from + s * (D + 2);
-    const float f = exp2_sfu(p[D] - u);
-    l += f * p[D + 1];
+#pragma unroll 4
+  for (int64_t s = first; s < end; ++s) {
+    const int64_t at = results.at(s, kvh, row);
+    const float2 top = results.top[at];
+    const float f = exp2_sfu(top.x - u);
+    l += f * top.y;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
-      const float2 v = *reinterpret_cast<const float2*>(p + i * 64 + lane * 2);
+      const float2 v = *reinterpret_cast<const float2*>(results.out + at * D + i * 64 + lane * 2);
       o[2 * i] += f * v.x;
       o[2 * i + 1] += f * v.y;
     }
@@ -455,71 +440,126 @@ __global__ void __launch_bounds__(128) join_kernel(const ppyb200_tree_attention_
     if (col < a.head_dim)
       *reinterpret_cast<uint32_t*>(out + col) = Kind<T>::pack(o[2 * i] * inv, o[2 * i + 1] * inv);
   }
-  if (lane == 0 && a.lse != nullptr) a.lse[row] = (m + log2f(l)) * kLn2;
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- host
 
 struct Plan {
-  int wm, wk;  // warps along rows and keys
-  Shape shape;
+  bool wide;
+  WideRows rows;  // wide
+  int wm;         // narrow: warps along the rows
+  int row_tiles;
+  Deal deal;
+  bool join;  // some sequence may have several results
   int64_t workspace;
 };
 
 int padded_dim(int64_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
-Plan plan_for(const ppyb200_tree_attention_args& a, int sm_count) {
-  Plan p;
-  p.shape.group = (int)(a.heads / a.kv_heads);
-  const int64_t rows = a.nodes * p.shape.group;
-  p.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
-  p.wk = p.wm == 1 ? 4 : p.wm == 2 ? 2 : 1;
-  p.shape.row_tiles = (int)((rows + 16 * p.wm - 1) / (16 * p.wm));
-  const int64_t ctas = a.batch * a.kv_heads * p.shape.row_tiles;
-  const int64_t tiles = (a.capacity + kTile - 1) / kTile;
-  // enough CTAs for four on every SM, each with at least two tiles of a full cache
-  int64_t splits = (4 * (int64_t)sm_count + ctas - 1) / ctas;
-  splits = splits < 1 ? 1 : splits > (tiles + 1) / 2 ? (tiles + 1) / 2 : splits;
-  p.shape.splits = (int)splits;
-  p.workspace = splits == 1 ? 0 : a.batch * a.heads * a.nodes * splits *
-                                      (padded_dim(a.head_dim) + 2) * 4;
+// What the tensor-core kernel takes: a positive scale (it keeps maxima of unscaled scores), tensors
+// that tensor maps can describe, and more rows than one 16-row tile of the narrow kernel.
+bool wide_fits(const Args& a) {
+  const int64_t group = a.heads / a.kv_heads;
+  return a.nodes * group > 16 && group <= 128 && a.head_dim > 32;
+}
+bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int64_t n2) {
+  const int64_t n[3] = {n0, n1, n2};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (strides[i] <= 0 || strides[i] >= (1ll << 39))) return false;
+  return true;
+}
+bool wide_takes(const Args& a) {
+  return wide_fits(a) && a.scale > 0 && strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
+         strides_fit(a.k_new_strides, a.batch, a.nodes, a.kv_heads) &&
+         strides_fit(a.v_new_strides, a.batch, a.nodes, a.kv_heads) &&
+         strides_fit(a.keys_strides, a.batch, a.kv_heads, a.capacity) &&
+         strides_fit(a.values_strides, a.batch, a.kv_heads, a.capacity);
+}
+
+Plan plan_for(const Args& a, bool wide, int sm_count) {
+  Plan p = {};
+  p.wide = wide;
+  const int64_t rows = a.nodes * (a.heads / a.kv_heads);
+  int64_t slots;
+  if (wide) {
+    // one CTA an SM: as many parts as make the last wave of CTAs a full one, by the time of a
+    // full cache: waves x (tiles a part + 3 for a CTA's start and end)
+    p.rows = ppyb200::tree::wide_rows(a);
+    p.deal.streams = p.rows.share ? 1 : 2;
+    p.deal.least = 2;
+    const int64_t unit = a.kv_heads * p.rows.pairs;
+    const int64_t tiles = a.batch * ((a.capacity + 127) / 128 + (a.nodes + 127) / 128);
+    int64_t best = INT64_MAX;
+    slots = a.batch;
+    for (int64_t s = a.batch; s <= a.batch + (tiles + 1) / 2 &&
+                              s * unit <= 8 * (int64_t)sm_count + a.batch * unit; ++s) {
+      const int64_t waves = (s * unit + sm_count - 1) / sm_count;
+      const int64_t spare = s - a.batch + 1;
+      const int64_t cost = waves * ((tiles + spare - 1) / spare + 3);
+      if (cost < best) {
+        best = cost;
+        slots = s;
+      }
+    }
+  } else {
+    p.wm = rows <= 16 ? 1 : 4;
+    p.row_tiles = (int)((rows + 16 * p.wm - 1) / (16 * p.wm));
+    p.deal.streams = 1;
+    p.deal.least = 2;
+    // four CTAs an SM, and at least two parts a sequence on average, so that long ones are split
+    const int64_t unit = a.kv_heads * p.row_tiles;
+    const int64_t tiles = (a.capacity + kTile - 1) / kTile;
+    const int64_t most = a.batch * ((tiles + 1) / 2);
+    slots = 4 * (int64_t)sm_count / unit;
+    slots = slots < 2 * a.batch ? 2 * a.batch : slots;
+    slots = slots > most ? most : slots;
+    slots = slots < a.batch ? a.batch : slots;
+  }
+  p.deal.slots = (int)slots;
+  p.join = p.deal.streams == 2 || slots > a.batch;
+  p.workspace = p.join ? Results::bytes(a, p.deal, padded_dim(a.head_dim)) : 0;
   return p;
 }
 
+template <class T, int D, int TILE, bool APART>
+cudaError_t join(const Args& a, const Plan& p, cudaStream_t stream) {
+  const int64_t rows = a.batch * a.heads * a.nodes;
+  return ppyb200::launch_pdl(join_kernel<T, D, TILE, APART>, dim3((unsigned)((rows + 3) / 4)),
+                             dim3(128), 0, stream, a, p.deal);
+}
+
 template <class T, int D, int WM, int WK>
-cudaError_t launch_rows(const ppyb200_tree_attention_args& a, const Plan& p, cudaStream_t stream) {
+cudaError_t launch_narrow(const Args& a, const Plan& p, cudaStream_t stream) {
   static ppyb200::DeviceOnce once;
   constexpr int smem = kStages * 2 * kTile * D * 2;
   int ready = 0;
-  auto kernel = tree_attention_kernel<T, D, WM, WK>;
-  cudaError_t e = once.get([&](int* value) {
+  auto kernel = narrow_kernel<T, D, WM, WK>;
+  const cudaError_t e = once.get([&](int* value) {
     *value = 1;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   }, &ready);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)p.shape.splits, (unsigned)(a.kv_heads * p.shape.row_tiles),
-                  (unsigned)a.batch);
-  e = ppyb200::launch_pdl(kernel, grid, dim3(32 * WM * WK), smem, stream, a, p.shape,
-                          static_cast<float*>(a.workspace));
-  if (e != cudaSuccess || p.shape.splits == 1) return e;
-  const int64_t rows = a.batch * a.heads * a.nodes;
-  return ppyb200::launch_pdl(join_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0,
-                             stream, a, p.shape.splits, static_cast<const float*>(a.workspace));
+  return ppyb200::launch_pdl(kernel,
+                             dim3((unsigned)p.deal.slots, (unsigned)(a.kv_heads * p.row_tiles)),
+                             dim3(32 * WM * WK), smem, stream, a, p.deal, p.row_tiles);
 }
 
 template <class T, int D>
-cudaError_t launch_dim(const ppyb200_tree_attention_args& a, const Plan& p, cudaStream_t stream) {
-  switch (p.wm) {
-    case 1: return launch_rows<T, D, 1, 4>(a, p, stream);
-    case 2: return launch_rows<T, D, 2, 2>(a, p, stream);
-    case 4: return launch_rows<T, D, 4, 1>(a, p, stream);
-    default: return launch_rows<T, D, 8, 1>(a, p, stream);
+cudaError_t launch_dim(const Args& a, const Plan& p, cudaStream_t stream) {
+  cudaError_t e;
+  if (p.wide) {
+    e = ppyb200::tree::launch_wide<T, D>(a, p.deal, p.rows, stream);
+    return e == cudaSuccess && p.join ? join<T, D, ppyb200::tree::kKeysTile, true>(a, p, stream)
+                                      : e;
   }
+  e = p.wm == 1 ? launch_narrow<T, D, 1, 4>(a, p, stream) : launch_narrow<T, D, 4, 1>(a, p, stream);
+  return e == cudaSuccess && p.join ? join<T, D, kTile, false>(a, p, stream) : e;
 }
 
 template <class T>
-cudaError_t launch_type(const ppyb200_tree_attention_args& a, const Plan& p,
-                        cudaStream_t stream) {
+cudaError_t launch_type(const Args& a, const Plan& p, cudaStream_t stream) {
   return a.head_dim <= 64 ? launch_dim<T, 64>(a, p, stream) : launch_dim<T, 128>(a, p, stream);
 }
 
@@ -539,8 +579,8 @@ const char* refusal(const ppyb200_tree_attention_args& a) {
   if (a.parents != nullptr && a.nodes > PPYB200_TREE_NODES)
     return "a tree has at most PPYB200_TREE_NODES nodes (a chain may be longer)";
   if (a.batch > 65535 || a.capacity > INT32_MAX || a.nodes * (a.heads / a.kv_heads) > INT32_MAX ||
-      a.kv_heads * ((a.nodes * (a.heads / a.kv_heads) + 127) / 128) > 65535)
-    return "batch up to 65535, kv_heads x row tiles of 128 up to 65535, capacity below 2^31";
+      a.kv_heads * ((a.nodes * (a.heads / a.kv_heads) + 15) / 16) > 65535)
+    return "batch up to 65535, kv_heads x row tiles of 16 up to 65535, capacity below 2^31";
   if (!rows16(a.q, a.q_strides) || !rows16(a.k_new, a.k_new_strides) ||
       !rows16(a.v_new, a.v_new_strides) || !rows16(a.keys, a.keys_strides) ||
       !rows16(a.values, a.values_strides) || !rows16(a.out, a.out_strides))
@@ -555,7 +595,11 @@ extern "C" {
 int64_t ppyb200_tree_attention_workspace(const ppyb200_tree_attention_args* args) {
   if (args == nullptr || refusal(*args) != nullptr || args->batch == 0 || args->nodes == 0)
     return 0;
-  return plan_for(*args, ppyb200_sm_count()).workspace;
+  // enough for either kernel: strides and scale, which choose one, are not among the sizes
+  const int sm_count = ppyb200_sm_count();
+  const int64_t narrow = plan_for(*args, false, sm_count).workspace;
+  const int64_t wide = wide_fits(*args) ? plan_for(*args, true, sm_count).workspace : 0;
+  return narrow > wide ? narrow : wide;
 }
 
 int32_t ppyb200_tree_attention(const ppyb200_tree_attention_args* args) {
@@ -573,7 +617,7 @@ int32_t ppyb200_tree_attention(const ppyb200_tree_attention_args* args) {
   }
   if (a.batch == 0 || a.nodes == 0) return PPYB200_OK;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(ppyb200_stream());
-  const Plan p = plan_for(a, ppyb200_sm_count());
+  const Plan p = plan_for(a, wide_takes(a), ppyb200_sm_count());
   if (p.workspace > 0 && (a.workspace == nullptr || a.workspace_bytes < p.workspace ||
                           (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0)) {
     ppyb200_set_error("ppyb200_tree_attention: a 16-byte aligned workspace of "
@@ -583,7 +627,7 @@ int32_t ppyb200_tree_attention(const ppyb200_tree_attention_args* args) {
   const cudaError_t e = a.dtype == PPYB200_BF16 ? launch_type<__nv_bfloat16>(a, p, stream)
                                                 : launch_type<__half>(a, p, stream);
   if (e != cudaSuccess) return ppyb200_check((int32_t)e, "ppyb200_tree_attention");
-  ppyb200_count_launches(p.shape.splits == 1 ? 1 : 2);
+  ppyb200_count_launches(p.join ? 2 : 1);
   return PPYB200_OK;
 }
 

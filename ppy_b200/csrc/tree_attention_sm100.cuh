@@ -1,0 +1,711 @@
+// The tree attention's tensor-core kernel, for key heads with many query rows (nodes x the
+// query heads that share the key head): tcgen05 products with TMEM accumulators, fed by TMA.
+//
+// A CTA takes a part of one sequence's key tiles (128 keys each: the cache's, then the nodes' own)
+// and walks it with two streams, each a query tile of 128 rows with its own softmax warpgroup and
+// MMA issuer, so that one stream's products run while the other's softmax does:
+//   rows > 128   the streams hold two row tiles and share every key tile (read once for 256 rows)
+//   rows <= 128  the streams hold the same rows and take the key tiles in turn, two results
+//   rows <= 64   as before, the second stream's rows in lanes 64-127: the four warps with rows sit
+//                on four SM sub-partitions instead of two
+// Per key tile and stream:
+//   S = Q K^T   M = 128, N = 128, both operands K-major with the 128-byte swizzle; the query rows
+//               of a tile come as one box [nodes][heads of the group][64 columns]
+//   softmax     a row a thread, f32, the running maximum moved only when a score exceeds it by
+//               2^8 (the weights of the tile are at most 2^8 then, exact for the quotient)
+//   O += P V    P from TMEM in the values' type (rounded to half a step, as the prompt
+//               attention's), V as it lies in the cache: [keys][64 columns] boxes are the
+//               MN-major form of the operand, no transposed copy
+// TMEM: D = 64: S 2 x 128 columns, O 2 x 64, P 2 x 64, and S of the next tile runs during the
+// softmax. D = 128: S 2 x 128, O 2 x 128, and P lies over its S; S of the next tile follows the
+// product that reads P (MMAs of one thread run in order).
+//
+// Tiles with masked keys (the cache's last, and the nodes') have their hidden values cleaned in
+// shared memory before the product: rows behind the sequence are zeroed, and so are single
+// values of nodes that are not finite, which the last step adds to the rows that see them.
+//
+//   warps 0-7  softmax (warpgroup t = stream t; warp w reads TMEM lanes 32 (w % 4) ...)
+//   warp 8     one thread: TMA loads of Q, K and V (a ring of K and V tiles in turn)
+//   warps 9,10 one thread each: the MMAs of stream 0 and 1; warp 9 owns the TMEM
+//   warp 11    appends the nodes to the cache, a share of them each CTA
+//
+// Every mbarrier wait is bounded: on giving up the CTA raises the status, every role leaves its
+// loop, copies and MMAs in flight are drained and the TMEM is freed.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "gemm_sm100.cuh"
+#include "mma16.cuh"
+#include "tmem.cuh"
+#include "tree_attention.cuh"
+
+namespace ppyb200 {
+namespace tree {
+
+using namespace tmem;
+using gemm::mbar_arrive;
+using gemm::mbar_drain_wait;
+using gemm::mbar_expect_tx;
+using gemm::mbar_init;
+using gemm::mbar_try_wait;
+using gemm::tc_fence_after;
+using gemm::tc_fence_before;
+using mma16::exp2_sfu;
+using mma16::Kind;
+
+constexpr int kRowsTile = 128;  // rows a stream
+constexpr int kKeysTile = 128;  // keys a tile
+constexpr int kWideThreads = 384;
+// Registers a thread after the split (setmaxnreg): the softmax warpgroups hold a row of 128 scores
+// and take what the third warpgroup gives up. The launch holds kLaunchRegs x 384, and the split
+// must not ask for more: launch_wide checks the compiled count, since a split that the pool
+// cannot meet would never return.
+constexpr uint32_t kLaunchRegs = 168, kSoftmaxRegs = 224, kSupportRegs = 56;
+static_assert(2 * 128 * kSoftmaxRegs + 128 * kSupportRegs <= kWideThreads * kLaunchRegs,
+              "register split above the launch's registers");
+constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr float kMoveLog2 = 8.f;
+constexpr int kBox = 128 * 64 * 2;  // 128 rows of 64 16-bit columns: one TMA box
+
+template <int D>
+struct WideShape {
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kTileBytes = kBoxes * kBox;  // a K, V or Q tile
+  static constexpr int kSlots = D == 64 ? 10 : 5;   // K and V tiles in the ring
+  static constexpr bool kOver = D == 128;           // P lies over S
+  static constexpr uint32_t kOCol = 256;
+  static constexpr uint32_t kPCol = kOver ? 0 : 384;
+  static constexpr uint32_t kPStep = kOver ? 128 : 64;
+};
+
+template <int D>
+struct WideShared {
+  alignas(1024) uint8_t q[2][WideShape<D>::kTileBytes];
+  alignas(1024) uint8_t ring[WideShape<D>::kSlots][WideShape<D>::kTileBytes];
+  alignas(8) uint64_t q_full, full[WideShape<D>::kSlots], empty[WideShape<D>::kSlots];
+  alignas(8) uint64_t s_full[2], s_free[2], p_full[2], o_done[2], drain[2];
+  uint32_t tmem_base;
+  int abort;
+  int spoiled[2];  // stream t met a value that is not finite among its node tiles
+};
+
+__device__ __forceinline__ void support_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSupportRegs));
+}
+__device__ __forceinline__ void softmax_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+}
+
+// The launch's tensor maps: [columns][slots or nodes][key heads][batch], and for q [columns]
+// [heads][nodes][batch].
+struct WideMaps {
+  CUtensorMap q, keys, values, k_new, v_new;
+};
+
+struct WideRows {
+  int tile_nodes;  // nodes of a row tile (tile_nodes x group <= 128, or <= 64 when half)
+  int pairs;       // CTAs along the rows
+  bool share;      // two row tiles a CTA, sharing the key tiles; else two streams over the keys
+  bool half;       // not share, at most 64 rows: stream 1's rows in lanes 64-127
+  int group;
+};
+
+template <class Layout>
+__device__ __forceinline__ bool wide_wait(Layout& s, uint64_t* bar, uint32_t parity,
+                                          int32_t* status) {
+  for (uint32_t tries = 0; tries < kWaitLimit; ++tries) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*(volatile int*)&s.abort) return false;
+  }
+  *(volatile int*)&s.abort = 1;
+  raise(status);
+  return false;
+}
+template <class Layout>
+__device__ __forceinline__ bool wide_warp_wait(Layout& s, uint64_t* bar, uint32_t parity,
+                                               int32_t* status) {
+  return __all_sync(0xffffffffu, wide_wait(s, bar, parity, status)) != 0;
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// An MN-major tile with the 128-byte swizzle: 64-column boxes kBox bytes apart (leading offset),
+// 1024 bytes between groups of eight keys (stride offset).
+__device__ __forceinline__ uint64_t smem_desc_mn(const void* tile) {
+  const uint64_t addr = smem_u32(tile);
+  return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(kBox >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <class T>
+constexpr uint32_t type_bits() {  // a and b format: 0 f16, 1 bf16
+  return sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+}
+template <class T>
+constexpr uint32_t idesc_s() {
+  return (1u << 4) | type_bits<T>() | ((uint32_t)(kKeysTile >> 3) << 17) |
+         ((uint32_t)(kRowsTile >> 4) << 24);
+}
+template <class T, int D>
+constexpr uint32_t idesc_o() {  // B (the values) MN-major
+  return (1u << 4) | type_bits<T>() | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
+         ((uint32_t)(kRowsTile >> 4) << 24);
+}
+
+// Which keys of a tile a row sees, a bit each.
+struct Sight {
+  uint64_t lo, hi;
+  __device__ __forceinline__ static Sight first(int64_t n) {  // keys 0 .. n - 1
+    Sight s;
+    s.lo = n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+    n -= 64;
+    s.hi = n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+    return s;
+  }
+  __device__ __forceinline__ void add(int key) {
+    if (key < 64) lo |= 1ull << key;
+    else hi |= 1ull << (key - 64);
+  }
+  __device__ __forceinline__ bool has(int key) const {
+    return (((key < 64 ? lo : hi) >> (key & 63)) & 1ull) != 0;
+  }
+};
+
+// What node `node` sees of the node tile that starts at node n0.
+__device__ __forceinline__ Sight node_sight(const int32_t* parents, int node, int n0, int count,
+                                            int32_t* status) {
+  if (parents == nullptr) return Sight::first(min(node + 1, count) - n0);
+  Sight s = Sight::first(0);
+  for (int i = node;;) {
+    if (i >= n0 && i < n0 + kKeysTile) s.add(i - n0);
+    const int p = parents[i];
+    if (p < 0 || p >= i) {  // a root; an index that is no earlier node raises
+      if (p != -1) raise(status);
+      break;
+    }
+    i = p;
+  }
+  return s;
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kWideThreads, 1)
+wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args a,
+            const Deal deal, const WideRows wide) {
+  using Shape = WideShape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  WideShared<D>& s = *reinterpret_cast<WideShared<D>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  const Part part = part_of<kKeysTile, true>(
+      a, deal, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0 ? a.status : nullptr);
+  const int kvh = blockIdx.y / wide.pairs, pair = blockIdx.y % wide.pairs;
+  const int group = wide.group, d = (int)a.head_dim, b = part.b;
+  // row tiles: stream t starts at node node0[t]
+  const int node0 = wide.share ? pair * 2 * wide.tile_nodes : 0;
+  if (b < 0 || node0 >= part.count) return;  // the whole CTA
+  const bool both = !wide.share || node0 + wide.tile_nodes < part.count;
+  const int64_t cache_tiles = (part.length + kKeysTile - 1) / kKeysTile;
+  int64_t tiles = part.tiles;
+  if (a.parents == nullptr && wide.share) {
+    // a chain: node tiles behind the last row's node are hidden from every row
+    const int last = min(part.count, node0 + 2 * wide.tile_nodes);
+    const int64_t end = cache_tiles + (last + kKeysTile - 1) / kKeysTile;
+    tiles = min(tiles, end - part.first);
+    tiles = tiles < 0 ? 0 : tiles;
+  }
+  // stream t walks tiles t_first(t), + t_step, ...: t_count(t) of them
+  const int step = wide.share ? 1 : 2;
+  auto tile_count = [&](int t) -> int64_t {
+    if (wide.share) return t == 0 || both ? tiles : 0;
+    return (tiles - t + 1) / 2;
+  };
+  auto tile_index = [&](int t, int64_t k) { return wide.share ? k : 2 * k + t; };
+
+  if (threadIdx.x == 0) {
+    mbar_init(&s.q_full, 1);
+    for (int i = 0; i < Shape::kSlots; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], wide.share && both ? 2 : 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s.s_full[t], 1);
+      mbar_init(&s.s_free[t], 4);
+      mbar_init(&s.p_full[t], 4);
+      mbar_init(&s.o_done[t], 1);
+      mbar_init(&s.drain[t], 1);
+      s.spoiled[t] = 0;
+    }
+    s.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s.tmem_base)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+
+  if (warp == 8) {
+    support_registers();
+    if (lane == 0 && tiles > 0) {
+      // ---- loader: Q once, then K and V of every tile; tile i's K is ring entry 2 i, its V 2 i + 1
+      const uint32_t q_bytes = (uint32_t)(Shape::kBoxes * wide.tile_nodes * group * 128);
+      mbar_expect_tx(&s.q_full, both ? 2 * q_bytes : q_bytes);
+      for (int t = 0; t < (both ? 2 : 1); ++t)
+        for (int x = 0; x < Shape::kBoxes; ++x)
+          tma_load_4d(s.q[t] + x * kBox + (wide.half && t == 1 ? kBox / 2 : 0), &maps.q,
+                      &s.q_full, x * 64, kvh * group,
+                      node0 + (wide.share ? t * wide.tile_nodes : 0), b);
+      int64_t c = 0;
+      bool ok = true;
+      for (int64_t i = 0; i < tiles && ok; ++i) {
+        const int64_t tile = part.first + i;
+        const bool own = tile >= cache_tiles;
+        const int32_t at = (int32_t)((own ? tile - cache_tiles : tile) * kKeysTile);
+        for (int v = 0; v < 2; ++v, ++c) {
+          const int slot = (int)(c % Shape::kSlots);
+          if (!wide_wait(s, &s.empty[slot], (uint32_t)(((c / Shape::kSlots) & 1) ^ 1),
+                         a.status)) {
+            ok = false;
+            break;
+          }
+          const CUtensorMap* map = own ? (v == 0 ? &maps.k_new : &maps.v_new)
+                                       : (v == 0 ? &maps.keys : &maps.values);
+          mbar_expect_tx(&s.full[slot], Shape::kTileBytes);
+          for (int x = 0; x < Shape::kBoxes; ++x)
+            tma_load_4d(s.ring[slot] + x * kBox, map, &s.full[slot], x * 64, at, kvh, b);
+        }
+      }
+      // the copies issued here land before the CTA may leave
+      for (int64_t j = c > Shape::kSlots ? c - Shape::kSlots : 0; j < c; ++j)
+        mbar_drain_wait(&s.full[j % Shape::kSlots], (uint32_t)((j / Shape::kSlots) & 1));
+      mbar_drain_wait(&s.q_full, 0);
+    }
+  } else if (warp == 9 || warp == 10) {
+    support_registers();
+    const int t = warp - 9;
+    const int64_t mine = tile_count(t);
+    if (lane == 0 && mine > 0) {
+      // ---- MMA issuer of stream t. Each commit to `empty` frees a ring entry of this stream's.
+      const uint32_t s_col = tmem + (uint32_t)(t * kKeysTile);
+      const uint32_t o_col = tmem + Shape::kOCol + (uint32_t)(t * D);
+      const uint32_t p_col = tmem + Shape::kPCol + (uint32_t)(t * Shape::kPStep);
+      auto full = [&](int64_t c) {
+        return wide_wait(s, &s.full[c % Shape::kSlots], (uint32_t)((c / Shape::kSlots) & 1),
+                         a.status);
+      };
+      auto scores = [&](int64_t k) -> bool {  // S = Q K^T of this stream's tile k
+        const int64_t c = 2 * tile_index(t, k);
+        if (!full(c)) return false;
+        if (!Shape::kOver && k > 0 &&
+            !wide_wait(s, &s.s_free[t], (uint32_t)((k - 1) & 1), a.status))
+          return false;
+        tc_fence_after();
+        const uint8_t* key = s.ring[c % Shape::kSlots];
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int box = kk >> 2, off = (kk & 3) * 2;
+          mma(s_col, gemm::smem_desc(s.q[t] + box * kBox) + (uint64_t)off,
+              gemm::smem_desc(key + box * kBox) + (uint64_t)off, idesc_s<T>(),
+              kk > 0 ? 1u : 0u);
+        }
+        commit(&s.s_full[t]);
+        commit(&s.empty[c % Shape::kSlots]);
+        return true;
+      };
+      auto product = [&](int64_t k) -> bool {  // O += P V of tile k
+        const int64_t c = 2 * tile_index(t, k) + 1;
+        if (!full(c) || !wide_wait(s, &s.p_full[t], (uint32_t)(k & 1), a.status)) return false;
+        tc_fence_after();
+        const uint64_t value = smem_desc_mn(s.ring[c % Shape::kSlots]);
+#pragma unroll
+        for (int kk = 0; kk < kKeysTile / 16; ++kk)  // 16 keys: two groups of 1024 bytes
+          mma_ts(o_col, p_col + (uint32_t)(kk * 8), value + (uint64_t)(kk * (2048 >> 4)),
+                 idesc_o<T, D>(), k > 0 || kk > 0 ? 1u : 0u);
+        commit(&s.o_done[t]);
+        commit(&s.empty[c % Shape::kSlots]);
+        return true;
+      };
+      if (wide_wait(s, &s.q_full, 0, a.status)) {
+        bool ok = scores(0);
+        for (int64_t k = 0; k < mine && ok; ++k) {
+          if (!Shape::kOver && k + 1 < mine) ok = scores(k + 1);
+          ok = ok && product(k);
+          if (Shape::kOver && k + 1 < mine) ok = ok && scores(k + 1);
+        }
+      }
+      commit(&s.drain[t]);
+      mbar_drain_wait(&s.drain[t], 0);
+    }
+  } else if (warp == 11) {
+    support_registers();
+    // ---- append: CTA (part, pair) of this key head takes every n-th node
+    const int n = part.parts * wide.pairs;
+    const T* k_new = static_cast<const T*>(a.k_new) + b * a.k_new_strides[0] +
+                     kvh * a.k_new_strides[2];
+    const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
+                     kvh * a.v_new_strides[2];
+    T* keys = static_cast<T*>(a.keys) + b * a.keys_strides[0] + kvh * a.keys_strides[1];
+    T* values = static_cast<T*>(a.values) + b * a.values_strides[0] + kvh * a.values_strides[1];
+    // pairs without rows have left: the others are dealt with by the pairs that stay
+    const int tile2 = 2 * wide.tile_nodes;
+    const int live = wide.share ? part.parts * ((part.count + tile2 - 1) / tile2) : n;
+    for (int i = part.index + part.parts * pair; i < part.count; i += live) {
+      const int64_t j = part.length + i;
+      for (int piece = lane; piece < d / 4; piece += 32) {
+        const bool is_key = piece < d / 8;
+        const int x = (is_key ? piece : piece - d / 8) * 8;
+        if (is_key)
+          *reinterpret_cast<uint4*>(keys + j * a.keys_strides[2] + x) =
+              *reinterpret_cast<const uint4*>(k_new + i * a.k_new_strides[1] + x);
+        else
+          *reinterpret_cast<uint4*>(values + j * a.values_strides[2] + x) =
+              *reinterpret_cast<const uint4*>(v_new + i * a.v_new_strides[1] + x);
+      }
+    }
+  } else {
+    softmax_registers();
+    // ---- softmax: warpgroup t, thread = row (a TMEM lane) and, when cleaning, a key
+    const int t = warp >> 2;
+    const int lane_row = (warp & 3) * 32 + lane;
+    const int row = lane_row - (wide.half && t == 1 ? 64 : 0);  // of the row tile
+    const int node = node0 + (wide.share ? t * wide.tile_nodes : 0) + row / group;
+    const bool real = row >= 0 && row < wide.tile_nodes * group && node < part.count &&
+                      (t == 0 || both);
+    const bool busy = __any_sync(0xffffffffu, real) != 0;  // the warp has rows
+    const int64_t mine = tile_count(t);
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_addr + (uint32_t)(t * kKeysTile);
+    const uint32_t o_addr = tmem + lane_addr + Shape::kOCol + (uint32_t)(t * D);
+    const uint32_t p_addr = tmem + lane_addr + Shape::kPCol + (uint32_t)(t * Shape::kPStep);
+    const float scale_log2 = (float)a.scale * mma16::kLog2e;
+    const uint64_t scale2 = f2(scale_log2, scale_log2);
+    const int32_t* parents = a.parents == nullptr ? nullptr
+                                                  : a.parents + (int64_t)b * a.parents_stride;
+    const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
+                     kvh * a.v_new_strides[2];
+    float m = -INFINITY, l = 0.f;  // m in raw score units
+    bool ok = true;
+    for (int64_t k = 0; k < mine; ++k) {
+      if (!wide_warp_wait(s, &s.s_full[t], (uint32_t)(k & 1), a.status)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int64_t tile = part.first + tile_index(t, k);
+      const bool own = tile >= cache_tiles;
+      const int64_t left = own ? 0 : part.length - tile * kKeysTile;
+      const bool ragged = own || left < kKeysTile;
+      if (busy) {
+        float sv[kKeysTile];
+#pragma unroll
+        for (int c = 0; c < kKeysTile / 32; ++c)
+          tmem_ld32_nowait(s_addr + (uint32_t)(c * 32), sv + c * 32);
+        tmem_wait_ld();
+        if (!Shape::kOver) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.s_free[t]);
+        }
+        if (ragged) {
+          const Sight sees =
+              !own ? Sight::first(left)
+                   : real ? node_sight(parents, node, (int)(tile - cache_tiles) * kKeysTile,
+                                       part.count, a.status)
+                          : Sight::first(0);
+#pragma unroll
+          for (int c = 0; c < kKeysTile; ++c)
+            if ((((c < 64 ? sees.lo : sees.hi) >> (c & 63)) & 1ull) == 0) sv[c] = -INFINITY;
+        }
+        float mx[4] = {m, m, m, m};
+#pragma unroll
+        for (int c = 0; c < kKeysTile; c += 8) {
+          mx[0] = max3(mx[0], sv[c + 0], sv[c + 1]);
+          mx[1] = max3(mx[1], sv[c + 2], sv[c + 3]);
+          mx[2] = max3(mx[2], sv[c + 4], sv[c + 5]);
+          mx[3] = max3(mx[3], sv[c + 6], sv[c + 7]);
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // the maximum moves by more than kMoveLog2, or stays; a row that has seen nothing yet
+        // stays at -inf, its weights 2^-inf = 0
+        const bool move = top != -INFINITY && !((top - m) * scale_log2 <= kMoveLog2);
+        float alpha = 1.f;
+        if (move) {
+          alpha = m == -INFINITY ? 0.f : exp2_sfu((m - top) * scale_log2);
+          m = top;
+          l *= alpha;
+        }
+        const float shift = m == -INFINITY ? 0.f : -m * scale_log2;
+        const uint64_t shift2 = f2(shift, shift);
+        if (!Shape::kOver && k > 0) {
+          // the product before this tile's reads P, which the stores below replace
+          if (!wide_warp_wait(s, &s.o_done[t], (uint32_t)((k - 1) & 1), a.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        uint64_t sum2[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int quarter = 0; quarter < 4; ++quarter) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = quarter * 32; c < quarter * 32 + 32; c += 2) {
+            float lo, hi;
+            unf2(fma2(f2(sv[c], sv[c + 1]), scale2, shift2), lo, hi);
+            const float e0 = exp2_sfu(lo), e1 = exp2_sfu(hi);
+            sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], f2(e0, e1));
+            pk[(c >> 1) & 15] = Kind<T>::pack(e0, e1);
+          }
+          tmem_st16(p_addr + (uint32_t)(quarter * 16), pk);
+        }
+        float s0, s1, s2, s3;
+        unf2(add2(sum2[0], sum2[1]), s0, s1);
+        unf2(add2(sum2[2], sum2[3]), s2, s3);
+        l += (s0 + s1) + (s2 + s3);
+        if (k > 0 && __any_sync(0xffffffffu, move)) {
+          // scale O of the rows whose maximum moved. Every product before this tile's is
+          // complete: S of this tile was issued behind the last (D = 128), or its barrier was
+          // waited for above.
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32_nowait(o_addr + (uint32_t)(c * 32), o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= alpha;
+            tmem_st32(o_addr + (uint32_t)(c * 32), o);
+          }
+        }
+        tmem_wait_st();
+      } else {
+        // no rows in this warp: it only keeps the barriers' counts (its P rows are never read
+        // by a row that leaves the CTA), in step with the others: two arrivals of one warp in a
+        // phase of p_full would stand for another's
+        if (!Shape::kOver) {
+          if (lane == 0) mbar_arrive(&s.s_free[t]);
+          if (k > 0 && !wide_warp_wait(s, &s.o_done[t], (uint32_t)((k - 1) & 1), a.status)) {
+            ok = false;
+            break;
+          }
+        }
+      }
+      if (ragged) {
+        // clean the tile's values: thread = key
+        const int64_t c = 2 * tile_index(t, k) + 1;
+        const int slot = (int)(c % Shape::kSlots);
+        if (!wide_warp_wait(s, &s.full[slot], (uint32_t)((c / Shape::kSlots) & 1), a.status)) {
+          ok = false;
+          break;
+        }
+        const int64_t n = own ? (tile - cache_tiles) * kKeysTile + lane_row : 0;
+        uint8_t* line = s.ring[slot] + lane_row * 128;
+        if (own ? n >= part.count : lane_row >= left) {
+#pragma unroll
+          for (int x = 0; x < Shape::kBoxes; ++x)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(line + x * kBox + e * 16) = make_uint4(0, 0, 0, 0);
+        } else if (own) {
+          const T* from = v_new + n * a.v_new_strides[1];
+          for (int e = 0; e < d / 8; ++e) {
+            const uint4 w = *reinterpret_cast<const uint4*>(from + e * 8);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            uint32_t clean[4];
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = Kind<T>::unpack(words[i]);
+              const bool x = isfinite(v.x), y = isfinite(v.y);
+              bad = bad || !x || !y;
+              clean[i] = (x ? words[i] & 0xffffu : 0u) | (y ? words[i] & 0xffff0000u : 0u);
+            }
+            if (bad) {
+              *reinterpret_cast<uint4*>(line + (e >> 3) * kBox +
+                                        (((e & 7) ^ (lane_row & 7)) << 4)) =
+                  make_uint4(clean[0], clean[1], clean[2], clean[3]);
+              *(volatile int*)&s.spoiled[t] = 1;
+            }
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.p_full[t]);
+    }
+    // the row's result, once the stream's last product has completed
+    if (ok && mine > 0) {
+      ok = wide_warp_wait(s, &s.o_done[t], (uint32_t)((mine - 1) & 1), a.status);
+      tc_fence_after();
+    }
+    if (ok && busy && (t == 0 || both)) {
+      const int64_t slot = (int64_t)blockIdx.x * deal.streams + (deal.streams == 2 ? t : 0);
+      const Results results(a.workspace, a, deal, D);
+      const int64_t at = results.at(slot, kvh, (int64_t)node * group + row % group);
+      const int head = kvh * group + row % group;
+      const bool whole = deal.streams == 1 && part.parts == 1;
+      const float inv = 1.f / l;
+      T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
+               (int64_t)head * a.out_strides[2];
+      const bool spoiled = mine > 0 && *(volatile int*)&s.spoiled[t] != 0;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (mine > 0) {
+          tmem_ld32_nowait(o_addr + (uint32_t)(c * 32), o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (spoiled && real) {
+          // add what the cleaning took out, to the rows that see it
+          for (int64_t k = 0; k < mine; ++k) {
+            const int64_t tile = part.first + tile_index(t, k) - cache_tiles;
+            if (tile < 0) continue;
+            const int n0 = (int)tile * kKeysTile;
+            const Sight sees = node_sight(parents, node, n0, part.count, nullptr);
+            for (int key = 0; key < kKeysTile && n0 + key < part.count; ++key) {
+              if (!sees.has(key)) continue;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if (c * 32 + e >= d) continue;
+                const float v = (float)v_new[(n0 + key) * a.v_new_strides[1] + c * 32 + e];
+                if (!isfinite(v)) o[e] += v;
+              }
+            }
+          }
+        }
+        if (real && whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            if (c * 32 + e < d)
+              *reinterpret_cast<uint4*>(out + c * 32 + e) = make_uint4(
+                  Kind<T>::pack(o[e] * inv, o[e + 1] * inv),
+                  Kind<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
+                  Kind<T>::pack(o[e + 4] * inv, o[e + 5] * inv),
+                  Kind<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(results.out + at * D + c * 32 + e) =
+                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      const float m_log2 = m == -INFINITY ? m : m * scale_log2;
+      if (real && whole) {
+        if (a.lse != nullptr)
+          a.lse[((int64_t)b * a.heads + head) * a.nodes + node] =
+              (m_log2 + log2f(l)) * mma16::kLn2;
+      } else if (real) {
+        results.top[at] = make_float2(m_log2, l);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+// [columns][n1][n2][n3] 16-bit elements with strides s1, s2, s3 (elements) as boxes of 64 columns
+// x box1 x box2. A dimension of one gets a stride of its own, whatever the tensor's says.
+inline bool wide_map(CUtensorMap* map, const void* base, bool bf16, int64_t columns, int64_t n1,
+                     int64_t s1, int box1, int64_t n2, int64_t s2, int box2, int64_t n3,
+                     int64_t s3) {
+  gemm::EncodeTiled encode = gemm::encode_tiled();
+  if (encode == nullptr) return false;
+  const int64_t n[3] = {n1, n2, n3}, s[3] = {s1, s2, s3};
+  cuuint64_t dims[4] = {(cuuint64_t)columns, 0, 0, 0}, strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] <= 0 || n[i] > INT32_MAX) return false;
+    const int64_t stride = n[i] == 1 ? (columns + 7) / 8 * 8 : s[i];
+    if (stride <= 0 || stride * 2 >= (1ll << 40)) return false;
+    dims[i + 1] = (cuuint64_t)n[i];
+    strides[i] = (cuuint64_t)(stride * 2);
+  }
+  const cuuint32_t box[4] = {64, (cuuint32_t)box1, (cuuint32_t)box2, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                4, const_cast<void*>(base), dims, strides, box, elem,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How the rows lie in tiles; tile_nodes 0 when a key head's group does not fit a tile.
+inline WideRows wide_rows(const Args& a) {
+  WideRows w;
+  w.group = (int)(a.heads / a.kv_heads);
+  w.half = a.nodes <= 64 / w.group;
+  w.tile_nodes = w.half ? 64 / w.group : kRowsTile / w.group;
+  w.share = w.tile_nodes > 0 && a.nodes > w.tile_nodes;
+  if (w.tile_nodes > a.nodes) w.tile_nodes = (int)a.nodes;
+  w.pairs = w.share ? (int)((a.nodes + 2 * w.tile_nodes - 1) / (2 * w.tile_nodes)) : 1;
+  return w;
+}
+
+template <class T, int D>
+inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& w,
+                               cudaStream_t stream) {
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const int64_t d = a.head_dim, kv = a.kv_heads;
+  WideMaps maps;
+  if (!wide_map(&maps.q, a.q, bf16, d, a.heads, a.q_strides[2], w.group, a.nodes,
+                a.q_strides[1], w.tile_nodes, a.batch, a.q_strides[0]) ||
+      !wide_map(&maps.keys, a.keys, bf16, d, a.capacity, a.keys_strides[2], kKeysTile, kv,
+                a.keys_strides[1], 1, a.batch, a.keys_strides[0]) ||
+      !wide_map(&maps.values, a.values, bf16, d, a.capacity, a.values_strides[2], kKeysTile, kv,
+                a.values_strides[1], 1, a.batch, a.values_strides[0]) ||
+      !wide_map(&maps.k_new, a.k_new, bf16, d, a.nodes, a.k_new_strides[1], kKeysTile, kv,
+                a.k_new_strides[2], 1, a.batch, a.k_new_strides[0]) ||
+      !wide_map(&maps.v_new, a.v_new, bf16, d, a.nodes, a.v_new_strides[1], kKeysTile, kv,
+                a.v_new_strides[2], 1, a.batch, a.v_new_strides[0]))
+    return cudaErrorInvalidValue;
+  static DeviceOnce once;
+  constexpr int smem = (int)sizeof(WideShared<D>) + 1024;
+  auto kernel = wide_kernel<T, D>;
+  int ready = 0;
+  const cudaError_t e = once.get(
+      [&](int* value) {
+        cudaFuncAttributes attributes;
+        cudaError_t r = cudaFuncGetAttributes(&attributes, kernel);
+        if (r != cudaSuccess) return r;
+        // the register split needs the launch's full count (setmaxnreg would wait for good)
+        *value = attributes.numRegs == (int)kLaunchRegs ? 1 : 2;
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      },
+      &ready);
+  if (e != cudaSuccess) return e;
+  if (ready != 1) return cudaErrorInvalidKernelImage;
+  return launch_pdl(kernel, dim3((unsigned)deal.slots, (unsigned)(a.kv_heads * w.pairs)),
+                    dim3(kWideThreads), smem, stream, maps, a, deal, w);
+}
+
+}  // namespace tree
+}  // namespace ppyb200
