@@ -29,14 +29,17 @@ namespace {
 using namespace ppyb200::mma16;
 using ppyb200::tree::Args;
 using ppyb200::tree::Deal;
-using ppyb200::tree::Part;
 using ppyb200::tree::Results;
+using ppyb200::tree::Segment;
+using ppyb200::tree::Walk;
 using ppyb200::tree::WideRows;
 using ppyb200::tree::raise;
 using ppyb200::tree::sequence_extent;
 
 constexpr int kTile = 64;       // keys a tile
 constexpr int kStages = 3;      // tiles in flight
+constexpr int kRows = 16;       // rows a CTA
+constexpr int kWarps = 4;       // along a tile's keys
 constexpr int kTreeWords = PPYB200_TREE_NODES / 32;
 
 // Shared memory rows of D elements: 16-byte pieces XORed with the row's low bits, so that the
@@ -46,12 +49,30 @@ __device__ __forceinline__ uint32_t row_piece(int row, int piece) {
   return (uint32_t)(row * D * 2 + ((piece ^ (row & 7)) << 4));
 }
 
-// WM warps along the rows (16 each), WK warps along a tile's keys.
-template <class T, int D, int WM, int WK>
-__global__ void __launch_bounds__(32 * WM * WK, WK == 1 ? 1 : D == 64 ? 4 : 2)
-narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_tiles) {
-  constexpr int kThreads = 32 * WM * WK, kRows = 16 * WM, kPieces = D / 8;
-  constexpr int kKeys = kTile / WK;      // keys of a tile that one warp takes
+// A row's result from its sums, by a warp: lane l holds columns 64 i + 2 l, +1.
+template <class T, int D>
+__device__ __forceinline__ void write_row(const Args& a, int b, int node, int head, int lane,
+                                          float m, float l, const float (&sum)[D / 32]) {
+  const float inv = 1.f / l;
+  T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
+           (int64_t)head * a.out_strides[2];
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const int col = i * 64 + lane * 2;
+    if (col < a.head_dim)
+      *reinterpret_cast<uint32_t*>(out + col) =
+          Kind<T>::pack(sum[2 * i] * inv, sum[2 * i + 1] * inv);
+  }
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
+}
+
+// Sixteen rows a CTA; the four warps take sixteen keys each of every tile and are joined at the end.
+template <class T, int D>
+__global__ void __launch_bounds__(32 * kWarps, D == 64 ? 4 : 2)
+narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
+  constexpr int kThreads = 32 * kWarps, kPieces = D / 8;
+  constexpr int kKeys = kTile / kWarps;  // keys of a tile that one warp takes
   constexpr int kTileBytes = kTile * D * 2;
   extern __shared__ __align__(128) uint8_t smem[];  // kStages x (K tile, V tile)
   __shared__ uint32_t below[kRows][kTreeWords];     // ancestors of each row's node, by bit
@@ -59,25 +80,27 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
 
   ppyb200::pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wm = warp / WK, wk = warp % WK;
   const int gid = lane >> 2, tig = lane & 3;
-  const Part part = ppyb200::tree::part_of<kTile, false>(
-      a, deal, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0 ? a.status : nullptr);
-  const int kvh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
-  const int group = (int)(a.heads / a.kv_heads), d = (int)a.head_dim, b = part.b;
-  const int64_t length = part.length;
-  const int rows = part.count * group, row0 = rt * kRows;
-  if (b < 0 || row0 >= rows) return;
-  const int64_t total = length + part.count;
-  const int64_t t0 = part.first, t1 = t0 + part.tiles;
+  const int group = deal.group, d = (int)a.head_dim;
+  Walk<kTile, false> walk;
+  walk.measure(a, deal, blockIdx.x == 0 ? a.status : nullptr);
+  walk.enter(a, deal, blockIdx.x);
+  Segment seg;
+  while (walk.next(a, deal, seg)) {
+  const int b = seg.b, kvh = seg.kvh;
+  const int64_t length = seg.length, total = length + seg.count;
+  const int row0 = seg.row0, rows = seg.count * group;
+  const int64_t t0 = seg.first, t1 = t0 + seg.tiles;
+  __syncthreads();  // the last segment's shared memory has been read
 
   const T* q = static_cast<const T*>(a.q) + b * a.q_strides[0];
   const T* k_new = static_cast<const T*>(a.k_new) + b * a.k_new_strides[0] +
                    kvh * a.k_new_strides[2];
   const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
                    kvh * a.v_new_strides[2];
-  T* keys = static_cast<T*>(a.keys) + b * a.keys_strides[0] + kvh * a.keys_strides[1];
-  T* values = static_cast<T*>(a.values) + b * a.values_strides[0] + kvh * a.values_strides[1];
+  const T* keys = static_cast<T*>(a.keys) + b * a.keys_strides[0] + kvh * a.keys_strides[1];
+  const T* values =
+      static_cast<T*>(a.values) + b * a.values_strides[0] + kvh * a.values_strides[1];
 
   const uint32_t base = shared_address(smem);
   auto load_tile = [&](int64_t tile, int stage) {
@@ -108,22 +131,10 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
     copies_commit();
   }
 
-  // append: the CTAs of the first row tile write the nodes whose slots they read
-  if (rt == 0 && t1 * kTile > length) {
-    const int64_t first = max(t0 * kTile, length), last = min(t1 * kTile, total);
-    const int pieces = d / 8;
-    for (int64_t i = tid; i < (last - first) * pieces; i += kThreads) {
-      const int64_t j = first + i / pieces, n = j - length;
-      const int piece = (int)(i % pieces);
-      *reinterpret_cast<uint4*>(keys + j * a.keys_strides[2] + piece * 8) =
-          *reinterpret_cast<const uint4*>(k_new + n * a.k_new_strides[1] + piece * 8);
-      *reinterpret_cast<uint4*>(values + j * a.values_strides[2] + piece * 8) =
-          *reinterpret_cast<const uint4*>(v_new + n * a.v_new_strides[1] + piece * 8);
-    }
-  }
+  ppyb200::tree::append<T>(a, deal, seg, tid, kThreads);
 
-  // query fragments: this warp's 16 rows, zero beyond the rows and the head size
-  const int ra = row0 + wm * 16 + gid, rb = ra + 8;
+  // query fragments: the 16 rows, zero beyond the rows and the head size
+  const int ra = row0 + gid, rb = ra + 8;
   uint32_t qf[D / 16][4];
   {
     const T* qa = ra < rows ? q + (ra / group) * a.q_strides[1] +
@@ -185,7 +196,7 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
 #pragma unroll
     for (int n = 0; n < kKeys / 8; ++n) {
       s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      const int row = wk * kKeys + n * 8 + (lane & 7);
+      const int row = warp * kKeys + n * 8 + (lane & 7);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {  // 32 columns: four 8 x 8 tiles
         uint32_t kf[4];
@@ -224,8 +235,8 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
       for (int c = 0; c < 4; ++c) {
         s[n][c] *= scale;
         if (tail) {
-          const int64_t j = t * kTile + wk * kKeys + n * 8 + tig * 2 + (c & 1);
-          if (!sees(wm * 16 + gid + (c >> 1) * 8, j)) s[n][c] = -INFINITY;
+          const int64_t j = t * kTile + warp * kKeys + n * 8 + tig * 2 + (c & 1);
+          if (!sees(gid + (c >> 1) * 8, j)) s[n][c] = -INFINITY;
         }
         if (c < 2) x0 = fmaxf(x0, s[n][c]);
         else x1 = fmaxf(x1, s[n][c]);
@@ -266,7 +277,7 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
           Kind<T>::pack(s[2 * kk][0], s[2 * kk][1]), Kind<T>::pack(s[2 * kk][2], s[2 * kk][3]),
           Kind<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]),
           Kind<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3])};
-      const int row = wk * kKeys + kk * 16 + (lane & 15);
+      const int row = warp * kKeys + kk * 16 + (lane & 15);
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {  // 16 columns: keys 0-7 and 8-15 of two 8-wide tiles
         uint32_t vf[4];
@@ -276,11 +287,11 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
       }
     }
     if (tail && spoiled != 0) {
-      for (int key = wk * kKeys; key < (wk + 1) * kKeys; ++key) {
+      for (int key = warp * kKeys; key < (warp + 1) * kKeys; ++key) {
         if (((spoiled >> key) & 1ull) == 0) continue;
         const int64_t j = t * kTile + key;
         const T* v = v_new + (j - length) * a.v_new_strides[1];
-        const bool see0 = sees(wm * 16 + gid, j), see1 = sees(wm * 16 + gid + 8, j);
+        const bool see0 = sees(gid, j), see1 = sees(gid + 8, j);
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -306,163 +317,136 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal, const int row_til
     l1 += __shfl_xor_sync(0xffffffffu, l1, w);
   }
 
-  // join the warps along the keys in shared memory
-  if (WK > 1) {
-    float* box = reinterpret_cast<float*>(smem);  // [WK][kRows][D + 2]
-    constexpr int kLine = D + 2;
-    __syncthreads();
-    float* mine = box + (wk * kRows + wm * 16 + gid) * kLine;
+  // join the warps in shared memory: [kWarps][kRows][D + 2]
+  float* box = reinterpret_cast<float*>(smem);
+  constexpr int kLine = D + 2;
+  __syncthreads();
+  float* mine = box + (warp * kRows + gid) * kLine;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      const int col = n * 8 + tig * 2;
-      mine[col] = o[n][0];
-      mine[col + 1] = o[n][1];
-      mine[8 * kLine + col] = o[n][2];
-      mine[8 * kLine + col + 1] = o[n][3];
-    }
-    if (tig == 0) {
-      mine[D] = m0;
-      mine[D + 1] = l0;
-      mine[8 * kLine + D] = m1;
-      mine[8 * kLine + D + 1] = l1;
-    }
-    __syncthreads();
-    if (wk != 0) return;
-    float y0 = -INFINITY, y1 = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      const float* from = box + (w * kRows + wm * 16 + gid) * kLine;
-      y0 = fmaxf(y0, from[D]);
-      y1 = fmaxf(y1, from[8 * kLine + D]);
-    }
-    const float z0 = y0 == -INFINITY ? 0.f : y0, z1 = y1 == -INFINITY ? 0.f : y1;
-    l0 = l1 = 0.f;
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      const float* from = box + (w * kRows + wm * 16 + gid) * kLine;
-      const float f0 = exp2_sfu(from[D] - z0), f1 = exp2_sfu(from[8 * kLine + D] - z1);
-      l0 += f0 * from[D + 1];
-      l1 += f1 * from[8 * kLine + D + 1];
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        const int col = n * 8 + tig * 2;
-        o[n][0] += f0 * from[col];
-        o[n][1] += f0 * from[col + 1];
-        o[n][2] += f1 * from[8 * kLine + col];
-        o[n][3] += f1 * from[8 * kLine + col + 1];
-      }
-    }
-    m0 = y0;
-    m1 = y1;
+  for (int n = 0; n < D / 8; ++n) {
+    const int col = n * 8 + tig * 2;
+    *reinterpret_cast<float2*>(mine + col) = make_float2(o[n][0], o[n][1]);
+    *reinterpret_cast<float2*>(mine + 8 * kLine + col) = make_float2(o[n][2], o[n][3]);
   }
-
+  if (tig == 0) {
+    *reinterpret_cast<float2*>(mine + D) = make_float2(m0, l0);
+    *reinterpret_cast<float2*>(mine + 8 * kLine + D) = make_float2(m1, l1);
+  }
+  __syncthreads();
+  // a warp a row at a time, a lane two columns of every 64
+  const Results results(a, deal, D);
+  for (int r = warp; r < kRows && row0 + r < rows; r += kWarps) {
+    float m = -INFINITY, l = 0.f, sum[D / 32];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = half == 0 ? ra : rb;
-    if (r >= rows) continue;
-    const float m = half == 0 ? m0 : m1, l = half == 0 ? l0 : l1;
-    const int node = r / group, head = kvh * group + r % group;
-    if (part.parts == 1) {
-      T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
-               (int64_t)head * a.out_strides[2];
-      const float inv = 1.f / l;
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, box[(w * kRows + r) * kLine + D]);
+    const float u = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        const int col = n * 8 + tig * 2;
-        if (col < d)
-          *reinterpret_cast<uint32_t*>(out + col) =
-              Kind<T>::pack(o[n][2 * half] * inv, o[n][2 * half + 1] * inv);
+    for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* from = box + (w * kRows + r) * kLine;
+      const float f = exp2_sfu(from[D] - u);
+      l += f * from[D + 1];
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const float2 v = *reinterpret_cast<const float2*>(from + i * 64 + lane * 2);
+        sum[2 * i] += f * v.x;
+        sum[2 * i + 1] += f * v.y;
       }
-      if (tig == 0 && a.lse != nullptr)
-        a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
-    } else {
-      const Results results(a.workspace, a, deal, D);
-      const int64_t at = results.at(blockIdx.x, kvh, r);
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(results.out + at * D + n * 8 + tig * 2) =
-            make_float2(o[n][2 * half], o[n][2 * half + 1]);
-      if (tig == 0) results.top[at] = make_float2(m, l);
     }
+    const int node = (row0 + r) / group, head = kvh * group + (row0 + r) % group;
+    if (seg.whole) {
+      write_row<T, D>(a, b, node, head, lane, m, l, sum);
+    } else {
+      const int64_t at = results.at(seg.result, r);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        *reinterpret_cast<float2*>(results.out + at * D + i * 64 + lane * 2) =
+            make_float2(sum[2 * i], sum[2 * i + 1]);
+      if (lane == 0) results.top[at] = make_float2(m, l);
+    }
+  }
   }
 }
 
-// One warp a row: joins the parts' unnormalised outputs in their order.
+// One warp a row: joins the unnormalised results of an item's segments in their order.
 template <class T, int D, int TILE, bool APART>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a,
                                                    const Deal deal) {
   ppyb200::pdl_wait();
-  const Results results(a.workspace, a, deal, D);
-  const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, group = (int)(a.heads / a.kv_heads);
-  if (index >= a.batch * a.kv_heads * results.rows) return;
-  const int64_t row = index % results.rows;
-  const int kvh = (int)(index / results.rows % a.kv_heads);
-  const int b = (int)(index / results.rows / a.kv_heads);
-  const int node = (int)(row / group), head = kvh * group + (int)(row % group);
-  int64_t length;
-  int count;
+  const int group = deal.group, rows = (int)a.nodes * group, kv_heads = (int)a.kv_heads;
+  const int index = (int)(blockIdx.x * 4 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  if (index >= (int)a.batch * kv_heads * rows) return;
+  const int row = index % rows, kvh = index / rows % kv_heads, b = index / rows / kv_heads;
+  const int node = row / group, head = kvh * group + row % group;
+  int length, count;
   sequence_extent(a, b, length, count, nullptr);
   if (node >= count) return;
-  const int2 parts = ppyb200::tree::parts_of<TILE, APART>(a, deal, b);
-  if (deal.streams == 1 && parts.y == 1) return;  // written by its CTA
-  const int64_t first = (int64_t)parts.x * deal.streams, end = first + parts.y * deal.streams;
+  // the item's place on the axis, and the CTAs whose shares hold it
+  Walk<TILE, APART> walk;
+  walk.measure(a, deal, nullptr);
+  const int item = b * deal.items + row / deal.item_rows;
+  int64_t start = 0;
+  for (int i = lane; i < item; i += 32) {
+    int other, nodes;
+    sequence_extent(a, i / deal.items, other, nodes, nullptr);
+    start += ppyb200::tree::item_tiles<TILE, APART>(a, deal, other, nodes, i % deal.items);
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) start += __shfl_xor_sync(0xffffffffu, start, w);
+  start += kvh * walk.span;
+  const int tiles =
+      ppyb200::tree::item_tiles<TILE, APART>(a, deal, length, count, item % deal.items);
+  const int c0 = walk.cta_of(a, start), c1 = walk.cta_of(a, start + tiles - 1);
+  if (deal.streams == 1 && c0 == c1) return;  // whole: written by its CTA
+  const Results results(a, deal, D);
+  // the first segment starts the item, the others continue it
+  auto place = [&](int i) {
+    const int c = c0 + i / deal.streams;
+    return results.at(walk.result_of(a, deal, c, kvh, item, c == c0) + i % deal.streams,
+                      row % deal.item_rows);
+  };
+  const int parts = (c1 - c0 + 1) * deal.streams;
   float m = -INFINITY;
-  for (int64_t s = first + lane; s < end; s += 32)
-    m = fmaxf(m, results.top[results.at(s, kvh, row)].x);
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, results.top[place(i)].x);
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
   const float u = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[D / 32];
+  float l = 0.f, sum[D / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+  for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
 #pragma unroll 4
-  for (int64_t s = first; s < end; ++s) {
-    const int64_t at = results.at(s, kvh, row);
+  for (int i = 0; i < parts; ++i) {
+    const int64_t at = place(i);
     const float2 top = results.top[at];
     const float f = exp2_sfu(top.x - u);
     l += f * top.y;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const float2 v = *reinterpret_cast<const float2*>(results.out + at * D + i * 64 + lane * 2);
-      o[2 * i] += f * v.x;
-      o[2 * i + 1] += f * v.y;
+    for (int k = 0; k < D / 64; ++k) {
+      const float2 v = *reinterpret_cast<const float2*>(results.out + at * D + k * 64 + lane * 2);
+      sum[2 * k] += f * v.x;
+      sum[2 * k + 1] += f * v.y;
     }
   }
-  const float inv = 1.f / l;
-  T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
-           (int64_t)head * a.out_strides[2];
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int col = i * 64 + lane * 2;
-    if (col < a.head_dim)
-      *reinterpret_cast<uint32_t*>(out + col) = Kind<T>::pack(o[2 * i] * inv, o[2 * i + 1] * inv);
-  }
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
+  write_row<T, D>(a, b, node, head, lane, m, l, sum);
 }
 
 // ---------------------------------------------------------------- host
 
 struct Plan {
   bool wide;
-  WideRows rows;  // wide
-  int wm;         // narrow: warps along the rows
-  int row_tiles;
+  WideRows rows;  // of the wide kernel
   Deal deal;
-  bool join;  // some sequence may have several results
+  bool join;  // some item may have several results
   int64_t workspace;
 };
 
 int padded_dim(int64_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
-// What the tensor-core kernel takes: a positive scale (it keeps maxima of unscaled scores), tensors
-// that tensor maps can describe, and more rows than one 16-row tile of the narrow kernel.
+// What the tensor-core kernel takes: a positive scale (it keeps maxima of unscaled scores), query
+// heads a key head that fit a row tile, and tensors that tensor maps describe.
 bool wide_fits(const Args& a) {
-  const int64_t group = a.heads / a.kv_heads;
-  return a.nodes * group > 16 && group <= 128 && a.head_dim > 32;
+  return a.heads / a.kv_heads <= ppyb200::tree::kRowsTile && a.head_dim > 32;
 }
 bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int64_t n2) {
   const int64_t n[3] = {n0, n1, n2};
@@ -481,44 +465,27 @@ bool wide_takes(const Args& a) {
 Plan plan_for(const Args& a, bool wide, int sm_count) {
   Plan p = {};
   p.wide = wide;
-  const int64_t rows = a.nodes * (a.heads / a.kv_heads);
-  int64_t slots;
+  const int64_t group = a.heads / a.kv_heads, rows = a.nodes * group;
+  p.deal.group = (int)group;
+  p.deal.least = 2;
   if (wide) {
-    // one CTA an SM: as many parts as make the last wave of CTAs a full one, by the time of a
-    // full cache: waves x (tiles a part + 3 for a CTA's start and end)
     p.rows = ppyb200::tree::wide_rows(a);
     p.deal.streams = p.rows.share ? 1 : 2;
-    p.deal.least = 2;
-    const int64_t unit = a.kv_heads * p.rows.pairs;
-    const int64_t tiles = a.batch * ((a.capacity + 127) / 128 + (a.nodes + 127) / 128);
-    int64_t best = INT64_MAX;
-    slots = a.batch;
-    for (int64_t s = a.batch; s <= a.batch + (tiles + 1) / 2 &&
-                              s * unit <= 8 * (int64_t)sm_count + a.batch * unit; ++s) {
-      const int64_t waves = (s * unit + sm_count - 1) / sm_count;
-      const int64_t spare = s - a.batch + 1;
-      const int64_t cost = waves * ((tiles + spare - 1) / spare + 3);
-      if (cost < best) {
-        best = cost;
-        slots = s;
-      }
-    }
+    p.deal.item_rows = (int)(p.rows.tile_nodes * group * (p.rows.share ? 2 : 1));
+    p.deal.grid = sm_count;
   } else {
-    p.wm = rows <= 16 ? 1 : 4;
-    p.row_tiles = (int)((rows + 16 * p.wm - 1) / (16 * p.wm));
     p.deal.streams = 1;
-    p.deal.least = 2;
-    // four CTAs an SM, and at least two parts a sequence on average, so that long ones are split
-    const int64_t unit = a.kv_heads * p.row_tiles;
-    const int64_t tiles = (a.capacity + kTile - 1) / kTile;
-    const int64_t most = a.batch * ((tiles + 1) / 2);
-    slots = 4 * (int64_t)sm_count / unit;
-    slots = slots < 2 * a.batch ? 2 * a.batch : slots;
-    slots = slots > most ? most : slots;
-    slots = slots < a.batch ? a.batch : slots;
+    p.deal.item_rows = kRows;
+    p.deal.grid = sm_count * (a.head_dim <= 64 ? 4 : 2);
   }
-  p.deal.slots = (int)slots;
-  p.join = p.deal.streams == 2 || slots > a.batch;
+  p.deal.items = (int)((rows + p.deal.item_rows - 1) / p.deal.item_rows);
+  // no more CTAs than a full cache has work for
+  const int64_t tile = wide ? ppyb200::tree::kKeysTile : kTile;
+  const int64_t work = a.batch * a.kv_heads * p.deal.items *
+                       ((a.capacity + tile - 1) / tile + (wide ? (a.nodes + tile - 1) / tile : 0));
+  const int64_t most = work / p.deal.least;
+  if (p.deal.grid > most) p.deal.grid = most < 1 ? 1 : (int)most;
+  p.join = p.deal.streams == 2 || p.deal.grid > 1;
   p.workspace = p.join ? Results::bytes(a, p.deal, padded_dim(a.head_dim)) : 0;
   return p;
 }
@@ -530,20 +497,19 @@ cudaError_t join(const Args& a, const Plan& p, cudaStream_t stream) {
                              dim3(128), 0, stream, a, p.deal);
 }
 
-template <class T, int D, int WM, int WK>
+template <class T, int D>
 cudaError_t launch_narrow(const Args& a, const Plan& p, cudaStream_t stream) {
   static ppyb200::DeviceOnce once;
   constexpr int smem = kStages * 2 * kTile * D * 2;
   int ready = 0;
-  auto kernel = narrow_kernel<T, D, WM, WK>;
+  auto kernel = narrow_kernel<T, D>;
   const cudaError_t e = once.get([&](int* value) {
     *value = 1;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   }, &ready);
   if (e != cudaSuccess) return e;
-  return ppyb200::launch_pdl(kernel,
-                             dim3((unsigned)p.deal.slots, (unsigned)(a.kv_heads * p.row_tiles)),
-                             dim3(32 * WM * WK), smem, stream, a, p.deal, p.row_tiles);
+  return ppyb200::launch_pdl(kernel, dim3((unsigned)p.deal.grid), dim3(32 * kWarps), smem, stream,
+                             a, p.deal);
 }
 
 template <class T, int D>
@@ -554,7 +520,7 @@ cudaError_t launch_dim(const Args& a, const Plan& p, cudaStream_t stream) {
     return e == cudaSuccess && p.join ? join<T, D, ppyb200::tree::kKeysTile, true>(a, p, stream)
                                       : e;
   }
-  e = p.wm == 1 ? launch_narrow<T, D, 1, 4>(a, p, stream) : launch_narrow<T, D, 4, 1>(a, p, stream);
+  e = launch_narrow<T, D>(a, p, stream);
   return e == cudaSuccess && p.join ? join<T, D, kTile, false>(a, p, stream) : e;
 }
 
@@ -579,8 +545,9 @@ const char* refusal(const ppyb200_tree_attention_args& a) {
   if (a.parents != nullptr && a.nodes > PPYB200_TREE_NODES)
     return "a tree has at most PPYB200_TREE_NODES nodes (a chain may be longer)";
   if (a.batch > 65535 || a.capacity > INT32_MAX || a.nodes * (a.heads / a.kv_heads) > INT32_MAX ||
-      a.kv_heads * ((a.nodes * (a.heads / a.kv_heads) + 15) / 16) > 65535)
-    return "batch up to 65535, kv_heads x row tiles of 16 up to 65535, capacity below 2^31";
+      a.batch * ((a.nodes * (a.heads / a.kv_heads) + 15) / 16) > INT32_MAX / 2 ||
+      a.batch * a.heads * a.nodes > INT32_MAX)
+    return "batch up to 65535, rows (batch x heads x nodes) and capacity below 2^31";
   if (!rows16(a.q, a.q_strides) || !rows16(a.k_new, a.k_new_strides) ||
       !rows16(a.v_new, a.v_new_strides) || !rows16(a.keys, a.keys_strides) ||
       !rows16(a.values, a.values_strides) || !rows16(a.out, a.out_strides))

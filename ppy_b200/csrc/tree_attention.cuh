@@ -20,149 +20,202 @@ __device__ __forceinline__ void raise(int32_t* status) {
 
 // The cache length and node count of a sequence, held inside the buffers whatever the device
 // arrays say: nodes that do not fit behind the length are dropped, and the status raised.
-__device__ __forceinline__ void sequence_extent(const Args& a, int b, int64_t& length,
-                                                int& count, int32_t* status) {
-  int64_t l = a.lengths[b];
-  int64_t n = a.counts != nullptr ? a.counts[b] : (int32_t)a.nodes;
-  bool bad = l < 0 || l > a.capacity || n < 0 || n > a.nodes;
-  l = l < 0 ? 0 : (l > a.capacity ? a.capacity : l);
-  n = n < 0 ? 0 : (n > a.nodes ? a.nodes : n);
-  if (l + n > a.capacity) {
-    n = a.capacity - l;
-    bad = true;
-  }
-  if (bad) raise(status);
-  length = l;
-  count = (int)n;
+__device__ __forceinline__ void sequence_extent(const Args& a, int b, int& length, int& count,
+                                                int32_t* status) {
+  const int capacity = (int)a.capacity, nodes = (int)a.nodes;
+  const int l = a.lengths[b], n = a.counts != nullptr ? a.counts[b] : nodes;
+  length = min(max(l, 0), capacity);
+  count = min(min(max(n, 0), nodes), capacity - length);
+  if (length != l || count != n) raise(status);
 }
 
-// How the key tiles of all sequences are dealt to `slots` parts (slots >= batch): parts of up to
-// C tiles, C the smallest size of at least `least` tiles that the slots suffice for whatever the
-// lengths are. Sequence b takes ceil(T_b / C) consecutive parts of nearly equal size, so long
-// and short sequences give parts alike. (sum ceil(T_b / C) < sum T_b / C + batch, so C =
-// ceil(sum T / (slots - batch + 1)) is enough.)
+// How the work is dealt to CTAs. An item is a piece of one sequence's rows (item_rows of them) under
+// one key head; its work is the key tiles it reads. All items, key head by key head, lie on one
+// axis of tiles, and CTA c of G takes the tiles [c W / G, (c + 1) W / G) of it: equal shares
+// whatever the lengths are, walked as segments of one item each. At most the first and the last
+// segment of a CTA are less than an item; those leave their unnormalised results in the workspace
+// for the join, a whole item is written out by its CTA. Where a CTA's two streams split an
+// item's keys, every segment leaves two results.
 struct Deal {
-  int slots;
+  int grid;       // CTAs at most; fewer when each would have less than `least` tiles
   int least;
-  int streams;  // results a part leaves: 2 where a CTA's two streams split its keys
+  int items;      // items a sequence and key head
+  int item_rows;
+  int group;      // query heads a key head
+  int streams;    // 2 where a CTA's two streams split an item's keys, else 1
 };
 
-struct Part {
-  int b = -1;         // -1: no work for this slot
-  int64_t length;     // the sequence's extent
-  int count;
-  int64_t first, tiles;  // key tiles of this part
-  int index, parts;      // which part of the sequence's, and how many
+struct Segment {
+  int b, kvh;
+  int row0;              // the item's first row
+  int length, count;     // the sequence's extent
+  int first, tiles;      // the key tiles to walk
+  bool whole;            // all of the item's
+  int64_t result;        // the first in the workspace, unless whole
 };
 
-// Key tiles of a sequence: the cache's, and the nodes' in tiles of their own when `apart`.
-template <int TILE, bool APART>
-__device__ __forceinline__ int64_t key_tiles(int64_t length, int count) {
-  if (count == 0) return 0;
-  return APART ? (length + TILE - 1) / TILE + (count + TILE - 1) / TILE
-               : (length + count + TILE - 1) / TILE;
+// a / b of numbers that are not negative: in 32 bits where they fit, several times as fast.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
 }
 
+// Key tiles of an item: the cache's, and the nodes' (in tiles of their own when APART), up to the
+// last row's node where the nodes are a chain.
 template <int TILE, bool APART>
-__device__ __forceinline__ int64_t part_size(const Args& a, const Deal& deal, int lane,
-                                             int32_t* status) {
-  int64_t total = 0;
-  for (int b = lane; b < (int)a.batch; b += 32) {
-    int64_t length;
-    int count;
-    sequence_extent(a, b, length, count, status);
-    total += key_tiles<TILE, APART>(length, count);
-  }
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-  const int64_t spare = deal.slots - a.batch + 1;
-  const int64_t size = (total + spare - 1) / spare;
-  return size > deal.least ? size : deal.least;
+__device__ __forceinline__ int item_tiles(const Args& a, const Deal& deal, int length, int count,
+                                          int r) {
+  const int row0 = r * deal.item_rows;
+  if (row0 >= count * deal.group) return 0;
+  int last = count;
+  if (a.parents == nullptr)
+    last = min(count, (row0 + deal.item_rows + deal.group - 1) / deal.group);
+  return APART ? (length + TILE - 1) / TILE + (last + TILE - 1) / TILE
+               : (length + last + TILE - 1) / TILE;
 }
 
-// The part of slot `slot` (a warp together; every lane gets it). Extents that were out of range
-// raise `status`.
+// The axis: tiles of one key head's items (`span`), the CTAs that share it, and a CTA's place.
 template <int TILE, bool APART>
-__device__ __forceinline__ Part part_of(const Args& a, const Deal& deal, int slot, int32_t* status) {
-  const int lane = threadIdx.x & 31;
-  const int64_t size = part_size<TILE, APART>(a, deal, lane, status);
-  Part part;
-  int before = 0;
-  for (int b0 = 0; b0 < (int)a.batch; b0 += 32) {
-    int64_t length = 0, tiles = 0;
-    int count = 0;
-    if (b0 + lane < (int)a.batch) {
-      sequence_extent(a, b0 + lane, length, count, nullptr);
-      tiles = key_tiles<TILE, APART>(length, count);
+struct Walk {
+  int64_t span;
+  int left, offset, ctas, cta, kvh, item;
+
+  // A warp together. Extents that are out of range raise `status`.
+  __device__ __forceinline__ void measure(const Args& a, const Deal& deal, int32_t* status) {
+    const int lane = threadIdx.x & 31, items = (int)a.batch * deal.items;
+    span = 0;
+    for (int i = lane; i < items; i += 32) {
+      int length, count;
+      sequence_extent(a, i / deal.items, length, count, status);
+      span += item_tiles<TILE, APART>(a, deal, length, count, i % deal.items);
     }
-    const int mine = (int)((tiles + size - 1) / size);
-    int run = mine;
 #pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, run, w);
-      if (lane >= w) run += up;
-    }
-    const int first = before + run - mine;
-    const unsigned hit = __ballot_sync(0xffffffffu, slot >= first && slot < first + mine);
-    if (hit != 0) {
-      const int l = __ffs(hit) - 1;
-      part.b = b0 + l;
-      part.length = __shfl_sync(0xffffffffu, length, l);
-      part.count = __shfl_sync(0xffffffffu, count, l);
-      tiles = __shfl_sync(0xffffffffu, tiles, l);
-      part.parts = __shfl_sync(0xffffffffu, mine, l);
-      part.index = slot - __shfl_sync(0xffffffffu, first, l);
-      part.first = part.index * tiles / part.parts;
-      part.tiles = (part.index + 1) * tiles / part.parts - part.first;
-      return part;
-    }
-    before += __shfl_sync(0xffffffffu, run, 31);
+    for (int w = 16; w > 0; w >>= 1) span += __shfl_xor_sync(0xffffffffu, span, w);
+    const int64_t most = quotient(span * a.kv_heads, deal.least);
+    ctas = most < 1 ? 1 : most < deal.grid ? (int)most : deal.grid;
   }
-  return part;
+  __device__ __forceinline__ int64_t start_of(const Args& a, int c) const {
+    return quotient(c * (span * a.kv_heads), ctas);
+  }
+  // The CTA whose share holds tile w of the axis.
+  __device__ __forceinline__ int cta_of(const Args& a, int64_t w) const {
+    return (int)quotient((w + 1) * ctas - 1, span * a.kv_heads);
+  }
+  // The first of the results that CTA c leaves of an item (one a stream): a CTA has at most one
+  // segment that continues an item and one that starts an item without ending it, and c + the
+  // item's number on the axis tells all segments apart.
+  __device__ __forceinline__ static int64_t result_of(const Args& a, const Deal& deal, int c,
+                                                      int kvh, int item, bool starts) {
+    if (deal.streams == 1) return 2 * (int64_t)c + (starts ? 1 : 0);
+    return 2 * (c + (int64_t)kvh * a.batch * deal.items + item);
+  }
+  // To the start of CTA c's share (a warp together).
+  __device__ __forceinline__ void enter(const Args& a, const Deal& deal, int c) {
+    const int lane = threadIdx.x & 31, items = (int)a.batch * deal.items;
+    cta = c;
+    left = 0;
+    kvh = item = 0;
+    offset = 0;
+    if (c >= ctas || span == 0) return;
+    const int64_t start = start_of(a, c);
+    left = (int)(start_of(a, c + 1) - start);
+    kvh = (int)quotient(start, span);
+    int64_t rest = start - kvh * span;
+    for (int i0 = 0; i0 < items; i0 += 32) {
+      int64_t tiles = 0;
+      if (i0 + lane < items) {
+        int length, count;
+        sequence_extent(a, (i0 + lane) / deal.items, length, count, nullptr);
+        tiles = item_tiles<TILE, APART>(a, deal, length, count, (i0 + lane) % deal.items);
+      }
+      int64_t run = tiles;
+#pragma unroll
+      for (int w = 1; w < 32; w <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, run, w);
+        if (lane >= w) run += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, rest < run);
+      if (hit != 0) {
+        const int l = __ffs(hit) - 1;
+        item = i0 + l;
+        offset = (int)(rest - __shfl_sync(0xffffffffu, run - tiles, l));
+        return;
+      }
+      rest -= __shfl_sync(0xffffffffu, run, 31);
+    }
+  }
+  // The next segment of the share; false behind its end.
+  __device__ __forceinline__ bool next(const Args& a, const Deal& deal, Segment& s) {
+    while (left > 0) {
+      s.b = item / deal.items;
+      const int r = item - s.b * deal.items;
+      sequence_extent(a, s.b, s.length, s.count, nullptr);
+      const int tiles = item_tiles<TILE, APART>(a, deal, s.length, s.count, r);
+      if (offset < tiles) {
+        s.kvh = kvh;
+        s.row0 = r * deal.item_rows;
+        s.first = offset;
+        s.tiles = min(tiles - offset, left);
+        s.whole = s.tiles == tiles && deal.streams == 1;
+        s.result = result_of(a, deal, cta, kvh, item, offset == 0);
+        left -= s.tiles;
+        offset += s.tiles;
+        return true;
+      }
+      offset = 0;
+      if (++item == (int)a.batch * deal.items) {
+        item = 0;
+        ++kvh;
+      }
+    }
+    return false;
+  }
+};
+
+// The nodes whose first row lies in an item are appended by the segment that starts the item, by
+// `threads` threads of which this is the `thread`-th.
+template <class T>
+__device__ __forceinline__ void append(const Args& a, const Deal& deal, const Segment& s,
+                                       int thread, int threads) {
+  if (s.first != 0) return;
+  const int from = (s.row0 + deal.group - 1) / deal.group;
+  const int to = min(s.count, (s.row0 + deal.item_rows + deal.group - 1) / deal.group);
+  const T* k_new = static_cast<const T*>(a.k_new) + s.b * a.k_new_strides[0] +
+                   s.kvh * a.k_new_strides[2];
+  const T* v_new = static_cast<const T*>(a.v_new) + s.b * a.v_new_strides[0] +
+                   s.kvh * a.v_new_strides[2];
+  T* keys = static_cast<T*>(a.keys) + s.b * a.keys_strides[0] + s.kvh * a.keys_strides[1];
+  T* values = static_cast<T*>(a.values) + s.b * a.values_strides[0] + s.kvh * a.values_strides[1];
+  const int pieces = (int)a.head_dim / 8;
+  for (int i = thread; i < (to - from) * pieces; i += threads) {
+    const int64_t n = from + i / pieces, j = s.length + n;
+    const int x = i % pieces * 8;
+    *reinterpret_cast<uint4*>(keys + j * a.keys_strides[2] + x) =
+        *reinterpret_cast<const uint4*>(k_new + n * a.k_new_strides[1] + x);
+    *reinterpret_cast<uint4*>(values + j * a.values_strides[2] + x) =
+        *reinterpret_cast<const uint4*>(v_new + n * a.v_new_strides[1] + x);
+  }
 }
 
-// The slots of sequence b's parts: the first, and how many (a warp together).
-template <int TILE, bool APART>
-__device__ __forceinline__ int2 parts_of(const Args& a, const Deal& deal, int b) {
-  const int lane = threadIdx.x & 31;
-  const int64_t size = part_size<TILE, APART>(a, deal, lane, nullptr);
-  int before = 0, mine = 0;
-  for (int i = lane; i <= b; i += 32) {
-    int64_t length;
-    int count;
-    sequence_extent(a, i, length, count, nullptr);
-    const int parts = (int)((key_tiles<TILE, APART>(length, count) + size - 1) / size);
-    if (i < b) before += parts;
-    else mine = parts;
-  }
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, w);
-    mine += __shfl_xor_sync(0xffffffffu, mine, w);
-  }
-  return make_int2(before, mine);
-}
-
-// The workspace: unnormalised outputs [slots * streams][kv_heads][rows][D] f32 (rows = nodes x
-// query heads a key head), then maximum (in powers of two) and sum [..][..][rows][2].
+// The workspace: unnormalised outputs [results][item_rows][D] f32, then maximum (in powers of two)
+// and sum [results][item_rows][2].
 struct Results {
   float* out;
   float2* top;
-  int64_t rows;
-  int kv_heads;
-  __host__ __device__ __forceinline__ Results(void* workspace, const Args& a, const Deal& deal,
-                                              int dim) {
-    rows = a.nodes * (a.heads / a.kv_heads);
-    kv_heads = (int)a.kv_heads;
-    out = static_cast<float*>(workspace);
-    top = reinterpret_cast<float2*>(out + (int64_t)deal.slots * deal.streams * kv_heads * rows *
-                                              dim);
+  int item_rows;
+  __host__ __device__ __forceinline__ static int64_t count(const Args& a, const Deal& deal) {
+    return 2 * (deal.grid + (deal.streams == 1 ? 0 : a.kv_heads * a.batch * deal.items));
   }
-  __host__ __device__ __forceinline__ int64_t at(int64_t slot, int kvh, int64_t row) const {
-    return (slot * kv_heads + kvh) * rows + row;
+  __device__ __forceinline__ Results(const Args& a, const Deal& deal, int dim)
+      : item_rows(deal.item_rows) {
+    out = static_cast<float*>(a.workspace);
+    top = reinterpret_cast<float2*>(out + count(a, deal) * item_rows * dim);
+  }
+  __device__ __forceinline__ int64_t at(int64_t result, int64_t row) const {
+    return result * item_rows + row;
   }
   static int64_t bytes(const Args& a, const Deal& deal, int dim) {
-    return (int64_t)deal.slots * deal.streams * a.nodes * a.heads * (dim + 2) * 4;
+    return count(a, deal) * deal.item_rows * (dim + 2) * 4;
   }
 };
 

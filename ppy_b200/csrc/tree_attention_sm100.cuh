@@ -1,8 +1,8 @@
 // The tree attention's tensor-core kernel, for key heads with many query rows (nodes x the
 // query heads that share the key head): tcgen05 products with TMEM accumulators, fed by TMA.
 //
-// A CTA takes a part of one sequence's key tiles (128 keys each: the cache's, then the nodes' own)
-// and walks it with two streams, each a query tile of 128 rows with its own softmax warpgroup and
+// A CTA an SM walks its share of the work (Walk): segments of key tiles (128 keys each: the cache's,
+// then the nodes' own) of one sequence and key head, with two streams, each a query tile of 128 rows with its own softmax warpgroup and
 // MMA issuer, so that one stream's products run while the other's softmax does:
 //   rows > 128   the streams hold two row tiles and share every key tile (read once for 256 rows)
 //   rows <= 128  the streams hold the same rows and take the key tiles in turn, two results
@@ -24,10 +24,11 @@
 // shared memory before the product: rows behind the sequence are zeroed, and so are single
 // values of nodes that are not finite, which the last step adds to the rows that see them.
 //
-//   warps 0-7  softmax (warpgroup t = stream t; warp w reads TMEM lanes 32 (w % 4) ...)
+//   warps 0-7  softmax (warpgroup t = stream t; warp w reads TMEM lanes 32 (w % 4) ...), and the
+//              append of a segment's nodes to the cache
 //   warp 8     one thread: TMA loads of Q, K and V (a ring of K and V tiles in turn)
 //   warps 9,10 one thread each: the MMAs of stream 0 and 1; warp 9 owns the TMEM
-//   warp 11    appends the nodes to the cache, a share of them each CTA
+//   warp 11    idle: it completes the third warpgroup
 //
 // Every mbarrier wait is bounded: on giving up the CTA raises the status, every role leaves its
 // loop, copies and MMAs in flight are drained and the TMEM is freed.
@@ -79,6 +80,7 @@ struct WideShape {
   static constexpr int kBoxes = D / 64;
   static constexpr int kTileBytes = kBoxes * kBox;  // a K, V or Q tile
   static constexpr int kSlots = D == 64 ? 10 : 5;   // K and V tiles in the ring
+  static constexpr int kTrees = D == 64 ? 8 : 4;    // more than the segments in the ring
   static constexpr bool kOver = D == 128;           // P lies over S
   static constexpr uint32_t kOCol = 256;
   static constexpr uint32_t kPCol = kOver ? 0 : 384;
@@ -89,11 +91,14 @@ template <int D>
 struct WideShared {
   alignas(1024) uint8_t q[2][WideShape<D>::kTileBytes];
   alignas(1024) uint8_t ring[WideShape<D>::kSlots][WideShape<D>::kTileBytes];
-  alignas(8) uint64_t q_full, full[WideShape<D>::kSlots], empty[WideShape<D>::kSlots];
-  alignas(8) uint64_t s_full[2], s_free[2], p_full[2], o_done[2], drain[2];
+  alignas(8) uint64_t q_full, q_empty, full[WideShape<D>::kSlots], empty[WideShape<D>::kSlots];
+  alignas(8) uint64_t s_full[2], s_free[2], p_full[2], o_done[2], turn[2], drain[2];
   uint32_t tmem_base;
   int abort;
-  int spoiled[2];  // stream t met a value that is not finite among its node tiles
+  // a value among a segment's node tiles is not finite: the segment's mark, in turns of eight (the
+  // ring holds five tiles, so no stream is eight segments ahead of the other)
+  int spoiled[8];
+  uint8_t parents[WideShape<D>::kTrees][256];  // of the last segments with node tiles
 };
 
 __device__ __forceinline__ void support_registers() {
@@ -111,10 +116,8 @@ struct WideMaps {
 
 struct WideRows {
   int tile_nodes;  // nodes of a row tile (tile_nodes x group <= 128, or <= 64 when half)
-  int pairs;       // CTAs along the rows
-  bool share;      // two row tiles a CTA, sharing the key tiles; else two streams over the keys
+  bool share;      // two row tiles an item, sharing the key tiles; else two streams over the keys
   bool half;       // not share, at most 64 rows: stream 1's rows in lanes 64-127
-  int group;
 };
 
 template <class Layout>
@@ -166,10 +169,19 @@ constexpr uint32_t idesc_o() {  // B (the values) MN-major
          ((uint32_t)(kRowsTile >> 4) << 24);
 }
 
+// Two 16-bit values, zero in the place of one that is not finite (its exponent bits all ones).
+template <class T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t kExponent = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  if ((w & kExponent) == kExponent) w &= 0xffff0000u;
+  if (((w >> 16) & kExponent) == kExponent) w &= 0x0000ffffu;
+  return w;
+}
+
 // Which keys of a tile a row sees, a bit each.
 struct Sight {
   uint64_t lo, hi;
-  __device__ __forceinline__ static Sight first(int64_t n) {  // keys 0 .. n - 1
+  __device__ __forceinline__ static Sight first(int n) {  // keys 0 .. n - 1
     Sight s;
     s.lo = n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
     n -= 64;
@@ -185,21 +197,16 @@ struct Sight {
   }
 };
 
-// What node `node` sees of the node tile that starts at node n0.
-__device__ __forceinline__ Sight node_sight(const int32_t* parents, int node, int n0, int count,
-                                            int32_t* status) {
+// What node `node` sees of the node tile that starts at node n0 (parents null: of a chain).
+__device__ __forceinline__ Sight node_sight(const uint8_t* parents, int node, int n0, int count) {
   if (parents == nullptr) return Sight::first(min(node + 1, count) - n0);
   Sight s = Sight::first(0);
   for (int i = node;;) {
     if (i >= n0 && i < n0 + kKeysTile) s.add(i - n0);
     const int p = parents[i];
-    if (p < 0 || p >= i) {  // a root; an index that is no earlier node raises
-      if (p != -1) raise(status);
-      break;
-    }
+    if (p == 255) return s;  // a root
     i = p;
   }
-  return s;
 }
 
 template <class T, int D>
@@ -211,47 +218,24 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
   WideShared<D>& s = *reinterpret_cast<WideShared<D>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  const Part part = part_of<kKeysTile, true>(
-      a, deal, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0 ? a.status : nullptr);
-  const int kvh = blockIdx.y / wide.pairs, pair = blockIdx.y % wide.pairs;
-  const int group = wide.group, d = (int)a.head_dim, b = part.b;
-  // row tiles: stream t starts at node node0[t]
-  const int node0 = wide.share ? pair * 2 * wide.tile_nodes : 0;
-  if (b < 0 || node0 >= part.count) return;  // the whole CTA
-  const bool both = !wide.share || node0 + wide.tile_nodes < part.count;
-  const int64_t cache_tiles = (part.length + kKeysTile - 1) / kKeysTile;
-  int64_t tiles = part.tiles;
-  if (a.parents == nullptr && wide.share) {
-    // a chain: node tiles behind the last row's node are hidden from every row
-    const int last = min(part.count, node0 + 2 * wide.tile_nodes);
-    const int64_t end = cache_tiles + (last + kKeysTile - 1) / kKeysTile;
-    tiles = min(tiles, end - part.first);
-    tiles = tiles < 0 ? 0 : tiles;
-  }
-  // stream t walks tiles t_first(t), + t_step, ...: t_count(t) of them
-  const int step = wide.share ? 1 : 2;
-  auto tile_count = [&](int t) -> int64_t {
-    if (wide.share) return t == 0 || both ? tiles : 0;
-    return (tiles - t + 1) / 2;
-  };
-  auto tile_index = [&](int t, int64_t k) { return wide.share ? k : 2 * k + t; };
 
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 2);
     for (int i = 0; i < Shape::kSlots; ++i) {
       mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], wide.share && both ? 2 : 1);
+      mbar_init(&s.empty[i], wide.share ? 2 : 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s.s_full[t], 1);
       mbar_init(&s.s_free[t], 4);
       mbar_init(&s.p_full[t], 4);
       mbar_init(&s.o_done[t], 1);
+      mbar_init(&s.turn[t], 4);
       mbar_init(&s.drain[t], 1);
-      s.spoiled[t] = 0;
     }
     s.abort = 0;
+    for (int i = 0; i < 8; ++i) s.spoiled[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
@@ -264,61 +248,93 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
+  // the set-up above overlaps the previous kernel; its results are needed from here on
+  pdl_wait();
+  Walk<kKeysTile, true> walk;
+  walk.measure(a, deal, blockIdx.x == 0 ? a.status : nullptr);
+  walk.enter(a, deal, blockIdx.x);
+  const int group = deal.group, d = (int)a.head_dim;
+  // Stream t of a segment walks its tiles t, t + 2, ..., or all of them when the streams share
+  // them. Rows of the second row tile may be missing (`both` false): its stream is idle then.
+  auto both_of = [&](const Segment& seg) {
+    return !wide.share || seg.row0 + wide.tile_nodes * group < seg.count * group;
+  };
+  auto count_of = [&](const Segment& seg, int t) -> int {
+    if (wide.share) return t == 0 || both_of(seg) ? seg.tiles : 0;
+    return (seg.tiles - t + 1) / 2;
+  };
+  auto index_of = [&](int t, int k) { return wide.share ? k : 2 * k + t; };
+  auto cache_tiles_of = [&](const Segment& seg) {
+    return (seg.length + kKeysTile - 1) / kKeysTile;
+  };
+  Segment seg;
 
   if (warp == 8) {
     support_registers();
-    if (lane == 0 && tiles > 0) {
-      // ---- loader: Q once, then K and V of every tile; tile i's K is ring entry 2 i, its V 2 i + 1
+    if (lane == 0) {
+      // ---- loader: a segment's Q, then K and V of its tiles; K of the CTA's i-th tile is entry
+      // 2 i of the ring, its V entry 2 i + 1
       const uint32_t q_bytes = (uint32_t)(Shape::kBoxes * wide.tile_nodes * group * 128);
-      mbar_expect_tx(&s.q_full, both ? 2 * q_bytes : q_bytes);
-      for (int t = 0; t < (both ? 2 : 1); ++t)
-        for (int x = 0; x < Shape::kBoxes; ++x)
-          tma_load_4d(s.q[t] + x * kBox + (wide.half && t == 1 ? kBox / 2 : 0), &maps.q,
-                      &s.q_full, x * 64, kvh * group,
-                      node0 + (wide.share ? t * wide.tile_nodes : 0), b);
-      int64_t c = 0;
+      int c = 0, segments = 0;
       bool ok = true;
-      for (int64_t i = 0; i < tiles && ok; ++i) {
-        const int64_t tile = part.first + i;
-        const bool own = tile >= cache_tiles;
-        const int32_t at = (int32_t)((own ? tile - cache_tiles : tile) * kKeysTile);
-        for (int v = 0; v < 2; ++v, ++c) {
-          const int slot = (int)(c % Shape::kSlots);
-          if (!wide_wait(s, &s.empty[slot], (uint32_t)(((c / Shape::kSlots) & 1) ^ 1),
-                         a.status)) {
-            ok = false;
-            break;
-          }
-          const CUtensorMap* map = own ? (v == 0 ? &maps.k_new : &maps.v_new)
-                                       : (v == 0 ? &maps.keys : &maps.values);
-          mbar_expect_tx(&s.full[slot], Shape::kTileBytes);
+      for (; ok && walk.next(a, deal, seg); ++segments) {
+        if (!wide_wait(s, &s.q_empty, (uint32_t)((segments & 1) ^ 1), a.status)) break;
+        const int streams = both_of(seg) ? 2 : 1;
+        const int node0 = seg.row0 / group;
+        mbar_expect_tx(&s.q_full, streams * q_bytes);
+        for (int t = 0; t < streams; ++t)
           for (int x = 0; x < Shape::kBoxes; ++x)
-            tma_load_4d(s.ring[slot] + x * kBox, map, &s.full[slot], x * 64, at, kvh, b);
+            tma_load_4d(s.q[t] + x * kBox + (wide.half && t == 1 ? kBox / 2 : 0), &maps.q,
+                        &s.q_full, x * 64, seg.kvh * group,
+                        node0 + (wide.share ? t * wide.tile_nodes : 0), seg.b);
+        const int cache_tiles = cache_tiles_of(seg);
+        for (int i = 0; i < seg.tiles && ok; ++i) {
+          const int tile = seg.first + i;
+          const bool own = tile >= cache_tiles;
+          const int at = (own ? tile - cache_tiles : tile) * kKeysTile;
+          for (int v = 0; v < 2; ++v, ++c) {
+            const int slot = (int)(c % Shape::kSlots);
+            if (!wide_wait(s, &s.empty[slot], (uint32_t)(((c / Shape::kSlots) & 1) ^ 1),
+                           a.status)) {
+              ok = false;
+              break;
+            }
+            const CUtensorMap* map = own ? (v == 0 ? &maps.k_new : &maps.v_new)
+                                         : (v == 0 ? &maps.keys : &maps.values);
+            mbar_expect_tx(&s.full[slot], Shape::kTileBytes);
+            for (int x = 0; x < Shape::kBoxes; ++x)
+              tma_load_4d(s.ring[slot] + x * kBox, map, &s.full[slot], x * 64, at, seg.kvh, seg.b);
+          }
         }
       }
       // the copies issued here land before the CTA may leave
-      for (int64_t j = c > Shape::kSlots ? c - Shape::kSlots : 0; j < c; ++j)
+      for (int j = c > Shape::kSlots ? c - Shape::kSlots : 0; j < c; ++j)
         mbar_drain_wait(&s.full[j % Shape::kSlots], (uint32_t)((j / Shape::kSlots) & 1));
-      mbar_drain_wait(&s.q_full, 0);
+      if (segments > 0) mbar_drain_wait(&s.q_full, (uint32_t)((segments - 1) & 1));
     }
   } else if (warp == 9 || warp == 10) {
     support_registers();
-    const int t = warp - 9;
-    const int64_t mine = tile_count(t);
-    if (lane == 0 && mine > 0) {
-      // ---- MMA issuer of stream t. Each commit to `empty` frees a ring entry of this stream's.
+    if (lane == 0) {
+      // ---- MMA issuer of stream t. tcgen05.commit tracks the products of the committing thread:
+      // a commit to `empty` frees a ring entry of this stream's; for an entry (and a Q) that it has
+      // no product of, where the other stream has, it arrives once the load is there, so that
+      // the arrival falls in the phase it belongs to.
+      const int t = warp - 9;
       const uint32_t s_col = tmem + (uint32_t)(t * kKeysTile);
       const uint32_t o_col = tmem + Shape::kOCol + (uint32_t)(t * D);
       const uint32_t p_col = tmem + Shape::kPCol + (uint32_t)(t * Shape::kPStep);
-      auto full = [&](int64_t c) {
+      int base = 0, n = 0, segments = 0;  // tiles before this segment's; this stream's so far
+      bool ok = true;
+      auto full = [&](int c) {
         return wide_wait(s, &s.full[c % Shape::kSlots], (uint32_t)((c / Shape::kSlots) & 1),
                          a.status);
       };
-      auto scores = [&](int64_t k) -> bool {  // S = Q K^T of this stream's tile k
-        const int64_t c = 2 * tile_index(t, k);
+      // S = Q K^T of this stream's tile k of the segment, its (n + k)-th in all
+      auto scores = [&](int k) -> bool {
+        const int c = 2 * (base + index_of(t, k));
         if (!full(c)) return false;
-        if (!Shape::kOver && k > 0 &&
-            !wide_wait(s, &s.s_free[t], (uint32_t)((k - 1) & 1), a.status))
+        if (!Shape::kOver && n + k > 0 &&
+            !wide_wait(s, &s.s_free[t], (uint32_t)((n + k - 1) & 1), a.status))
           return false;
         tc_fence_after();
         const uint8_t* key = s.ring[c % Shape::kSlots];
@@ -333,9 +349,11 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         commit(&s.empty[c % Shape::kSlots]);
         return true;
       };
-      auto product = [&](int64_t k) -> bool {  // O += P V of tile k
-        const int64_t c = 2 * tile_index(t, k) + 1;
-        if (!full(c) || !wide_wait(s, &s.p_full[t], (uint32_t)(k & 1), a.status)) return false;
+      // O += P V of tile k
+      auto product = [&](int k) -> bool {
+        const int c = 2 * (base + index_of(t, k)) + 1;
+        if (!full(c) || !wide_wait(s, &s.p_full[t], (uint32_t)((n + k) & 1), a.status))
+          return false;
         tc_fence_after();
         const uint64_t value = smem_desc_mn(s.ring[c % Shape::kSlots]);
 #pragma unroll
@@ -346,281 +364,310 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         commit(&s.empty[c % Shape::kSlots]);
         return true;
       };
-      if (wide_wait(s, &s.q_full, 0, a.status)) {
-        bool ok = scores(0);
-        for (int64_t k = 0; k < mine && ok; ++k) {
-          if (!Shape::kOver && k + 1 < mine) ok = scores(k + 1);
-          ok = ok && product(k);
-          if (Shape::kOver && k + 1 < mine) ok = ok && scores(k + 1);
+      for (; ok && walk.next(a, deal, seg); ++segments) {
+        const int mine = count_of(seg, t);
+        if (!wide_wait(s, &s.q_full, (uint32_t)(segments & 1), a.status)) break;
+        if (mine == 0) {
+          mbar_arrive(&s.q_empty);
+          for (int c = 2 * base; wide.share && ok && c < 2 * (base + seg.tiles); ++c) {
+            ok = full(c);
+            if (ok) mbar_arrive(&s.empty[c % Shape::kSlots]);
+          }
+        } else {
+          ok = scores(0);
+          for (int k = 0; k < mine && ok; ++k) {
+            if (k + 1 == mine) commit(&s.q_empty);
+            if (!Shape::kOver && k + 1 < mine) ok = scores(k + 1);
+            ok = ok && product(k);
+            if (Shape::kOver && k + 1 < mine) ok = ok && scores(k + 1);
+          }
         }
+        base += seg.tiles;
+        n += mine;
       }
       commit(&s.drain[t]);
       mbar_drain_wait(&s.drain[t], 0);
     }
   } else if (warp == 11) {
-    support_registers();
-    // ---- append: CTA (part, pair) of this key head takes every n-th node
-    const int n = part.parts * wide.pairs;
-    const T* k_new = static_cast<const T*>(a.k_new) + b * a.k_new_strides[0] +
-                     kvh * a.k_new_strides[2];
-    const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
-                     kvh * a.v_new_strides[2];
-    T* keys = static_cast<T*>(a.keys) + b * a.keys_strides[0] + kvh * a.keys_strides[1];
-    T* values = static_cast<T*>(a.values) + b * a.values_strides[0] + kvh * a.values_strides[1];
-    // pairs without rows have left: the others are dealt with by the pairs that stay
-    const int tile2 = 2 * wide.tile_nodes;
-    const int live = wide.share ? part.parts * ((part.count + tile2 - 1) / tile2) : n;
-    for (int i = part.index + part.parts * pair; i < part.count; i += live) {
-      const int64_t j = part.length + i;
-      for (int piece = lane; piece < d / 4; piece += 32) {
-        const bool is_key = piece < d / 8;
-        const int x = (is_key ? piece : piece - d / 8) * 8;
-        if (is_key)
-          *reinterpret_cast<uint4*>(keys + j * a.keys_strides[2] + x) =
-              *reinterpret_cast<const uint4*>(k_new + i * a.k_new_strides[1] + x);
-        else
-          *reinterpret_cast<uint4*>(values + j * a.values_strides[2] + x) =
-              *reinterpret_cast<const uint4*>(v_new + i * a.v_new_strides[1] + x);
-      }
-    }
+    support_registers();  // completes the third warpgroup
   } else {
     softmax_registers();
     // ---- softmax: warpgroup t, thread = row (a TMEM lane) and, when cleaning, a key
     const int t = warp >> 2;
     const int lane_row = (warp & 3) * 32 + lane;
     const int row = lane_row - (wide.half && t == 1 ? 64 : 0);  // of the row tile
-    const int node = node0 + (wide.share ? t * wide.tile_nodes : 0) + row / group;
-    const bool real = row >= 0 && row < wide.tile_nodes * group && node < part.count &&
-                      (t == 0 || both);
-    const bool busy = __any_sync(0xffffffffu, real) != 0;  // the warp has rows
-    const int64_t mine = tile_count(t);
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + (uint32_t)(t * kKeysTile);
     const uint32_t o_addr = tmem + lane_addr + Shape::kOCol + (uint32_t)(t * D);
     const uint32_t p_addr = tmem + lane_addr + Shape::kPCol + (uint32_t)(t * Shape::kPStep);
     const float scale_log2 = (float)a.scale * mma16::kLog2e;
     const uint64_t scale2 = f2(scale_log2, scale_log2);
-    const int32_t* parents = a.parents == nullptr ? nullptr
-                                                  : a.parents + (int64_t)b * a.parents_stride;
-    const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
-                     kvh * a.v_new_strides[2];
-    float m = -INFINITY, l = 0.f;  // m in raw score units
+    const Results results(a, deal, D);
+    int base = 0, n = 0;  // as the MMA issuer's
+    int mark = 1;             // this segment's, in `spoiled`
+    int turn = 0;         // tiles of shared segments so far
     bool ok = true;
-    for (int64_t k = 0; k < mine; ++k) {
-      if (!wide_warp_wait(s, &s.s_full[t], (uint32_t)(k & 1), a.status)) {
-        ok = false;
-        break;
+    while (ok && walk.next(a, deal, seg)) {
+      append<T>(a, deal, seg, threadIdx.x, 256);
+      const int mine = count_of(seg, t);
+      const bool turns = wide.share && both_of(seg);
+      const int cache_tiles = cache_tiles_of(seg);
+      const int tile_row = (wide.share ? t * wide.tile_nodes * group : 0) + row;  // of the item
+      const int node = (seg.row0 + tile_row) / group;
+      const bool real = row >= 0 && row < wide.tile_nodes * group && node < seg.count;
+      const bool busy = __any_sync(0xffffffffu, real) != 0;  // the warp has rows
+      const uint8_t* parents = nullptr;
+      if (a.parents != nullptr && seg.first + seg.tiles > cache_tiles) {
+        // a tree of up to 256 nodes: each parent a byte, 255 for a root, as any that is no earlier
+        // node is taken; every warp writes the same bytes
+        uint8_t* to = s.parents[mark % Shape::kTrees];
+        const int32_t* from = a.parents + (int64_t)seg.b * a.parents_stride;
+        for (int i = lane; i < seg.count; i += 32) {
+          const int p = from[i];
+          if (p < -1 || p >= i) raise(a.status);
+          to[i] = p >= 0 && p < i ? (uint8_t)p : (uint8_t)255;
+        }
+        __syncwarp();
+        parents = to;
       }
-      tc_fence_after();
-      const int64_t tile = part.first + tile_index(t, k);
-      const bool own = tile >= cache_tiles;
-      const int64_t left = own ? 0 : part.length - tile * kKeysTile;
-      const bool ragged = own || left < kKeysTile;
-      if (busy) {
-        float sv[kKeysTile];
-#pragma unroll
-        for (int c = 0; c < kKeysTile / 32; ++c)
-          tmem_ld32_nowait(s_addr + (uint32_t)(c * 32), sv + c * 32);
-        tmem_wait_ld();
-        if (!Shape::kOver) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s.s_free[t]);
-        }
-        if (ragged) {
-          const Sight sees =
-              !own ? Sight::first(left)
-                   : real ? node_sight(parents, node, (int)(tile - cache_tiles) * kKeysTile,
-                                       part.count, a.status)
-                          : Sight::first(0);
-#pragma unroll
-          for (int c = 0; c < kKeysTile; ++c)
-            if ((((c < 64 ? sees.lo : sees.hi) >> (c & 63)) & 1ull) == 0) sv[c] = -INFINITY;
-        }
-        float mx[4] = {m, m, m, m};
-#pragma unroll
-        for (int c = 0; c < kKeysTile; c += 8) {
-          mx[0] = max3(mx[0], sv[c + 0], sv[c + 1]);
-          mx[1] = max3(mx[1], sv[c + 2], sv[c + 3]);
-          mx[2] = max3(mx[2], sv[c + 4], sv[c + 5]);
-          mx[3] = max3(mx[3], sv[c + 6], sv[c + 7]);
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // the maximum moves by more than kMoveLog2, or stays; a row that has seen nothing yet
-        // stays at -inf, its weights 2^-inf = 0
-        const bool move = top != -INFINITY && !((top - m) * scale_log2 <= kMoveLog2);
-        float alpha = 1.f;
-        if (move) {
-          alpha = m == -INFINITY ? 0.f : exp2_sfu((m - top) * scale_log2);
-          m = top;
-          l *= alpha;
-        }
-        const float shift = m == -INFINITY ? 0.f : -m * scale_log2;
-        const uint64_t shift2 = f2(shift, shift);
-        if (!Shape::kOver && k > 0) {
-          // the product before this tile's reads P, which the stores below replace
-          if (!wide_warp_wait(s, &s.o_done[t], (uint32_t)((k - 1) & 1), a.status)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-        }
-        uint64_t sum2[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int quarter = 0; quarter < 4; ++quarter) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int c = quarter * 32; c < quarter * 32 + 32; c += 2) {
-            float lo, hi;
-            unf2(fma2(f2(sv[c], sv[c + 1]), scale2, shift2), lo, hi);
-            const float e0 = exp2_sfu(lo), e1 = exp2_sfu(hi);
-            sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], f2(e0, e1));
-            pk[(c >> 1) & 15] = Kind<T>::pack(e0, e1);
-          }
-          tmem_st16(p_addr + (uint32_t)(quarter * 16), pk);
-        }
-        float s0, s1, s2, s3;
-        unf2(add2(sum2[0], sum2[1]), s0, s1);
-        unf2(add2(sum2[2], sum2[3]), s2, s3);
-        l += (s0 + s1) + (s2 + s3);
-        if (k > 0 && __any_sync(0xffffffffu, move)) {
-          // scale O of the rows whose maximum moved. Every product before this tile's is
-          // complete: S of this tile was issued behind the last (D = 128), or its barrier was
-          // waited for above.
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tmem_ld32_nowait(o_addr + (uint32_t)(c * 32), o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= alpha;
-            tmem_st32(o_addr + (uint32_t)(c * 32), o);
-          }
-        }
-        tmem_wait_st();
-      } else {
-        // no rows in this warp: it only keeps the barriers' counts (its P rows are never read
-        // by a row that leaves the CTA), in step with the others: two arrivals of one warp in a
-        // phase of p_full would stand for another's
-        if (!Shape::kOver) {
-          if (lane == 0) mbar_arrive(&s.s_free[t]);
-          if (k > 0 && !wide_warp_wait(s, &s.o_done[t], (uint32_t)((k - 1) & 1), a.status)) {
-            ok = false;
-            break;
-          }
-        }
-      }
-      if (ragged) {
-        // clean the tile's values: thread = key
-        const int64_t c = 2 * tile_index(t, k) + 1;
-        const int slot = (int)(c % Shape::kSlots);
-        if (!wide_warp_wait(s, &s.full[slot], (uint32_t)((c / Shape::kSlots) & 1), a.status)) {
+      const T* v_new = static_cast<const T*>(a.v_new) + seg.b * a.v_new_strides[0] +
+                       seg.kvh * a.v_new_strides[2];
+      float m = -INFINITY, l = 0.f;  // m in raw score units
+      for (int k = 0; k < mine; ++k) {
+        const uint32_t phase = (uint32_t)((n + k) & 1);
+        if (!wide_warp_wait(s, &s.s_full[t], phase, a.status)) {
           ok = false;
           break;
         }
-        const int64_t n = own ? (tile - cache_tiles) * kKeysTile + lane_row : 0;
-        uint8_t* line = s.ring[slot] + lane_row * 128;
-        if (own ? n >= part.count : lane_row >= left) {
+        tc_fence_after();
+        const int tile = seg.first + index_of(t, k);
+        const bool own = tile >= cache_tiles;
+        const int left = own ? 0 : seg.length - tile * kKeysTile;
+        const bool ragged = own || left < kKeysTile;
+        if (busy) {
+          float sv[kKeysTile];
 #pragma unroll
-          for (int x = 0; x < Shape::kBoxes; ++x)
+          for (int c = 0; c < kKeysTile / 32; ++c)
+            tmem_ld32_nowait(s_addr + (uint32_t)(c * 32), sv + c * 32);
+          tmem_wait_ld();
+          if (!Shape::kOver) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.s_free[t]);
+          }
+          if (ragged) {
+            const Sight sees =
+                !own ? Sight::first(left)
+                     : real ? node_sight(parents, node, (tile - cache_tiles) * kKeysTile,
+                                         seg.count)
+                            : Sight::first(0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4*>(line + x * kBox + e * 16) = make_uint4(0, 0, 0, 0);
-        } else if (own) {
-          const T* from = v_new + n * a.v_new_strides[1];
-          for (int e = 0; e < d / 8; ++e) {
-            const uint4 w = *reinterpret_cast<const uint4*>(from + e * 8);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-            uint32_t clean[4];
-            bool bad = false;
+            for (int c = 0; c < kKeysTile; ++c)
+              if ((((c < 64 ? sees.lo : sees.hi) >> (c & 63)) & 1ull) == 0) sv[c] = -INFINITY;
+            __syncwarp();  // the walks differ; tensor memory is accessed by whole warps
+          }
+          float mx[4] = {m, m, m, m};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 v = Kind<T>::unpack(words[i]);
-              const bool x = isfinite(v.x), y = isfinite(v.y);
-              bad = bad || !x || !y;
-              clean[i] = (x ? words[i] & 0xffffu : 0u) | (y ? words[i] & 0xffff0000u : 0u);
+          for (int c = 0; c < kKeysTile; c += 8) {
+            mx[0] = max3(mx[0], sv[c + 0], sv[c + 1]);
+            mx[1] = max3(mx[1], sv[c + 2], sv[c + 3]);
+            mx[2] = max3(mx[2], sv[c + 4], sv[c + 5]);
+            mx[3] = max3(mx[3], sv[c + 6], sv[c + 7]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // the maximum moves by more than kMoveLog2, or stays; a row that has seen nothing yet
+          // stays at -inf, its weights 2^-inf = 0
+          const bool move = top != -INFINITY && !((top - m) * scale_log2 <= kMoveLog2);
+          float alpha = 1.f;
+          if (move) {
+            alpha = m == -INFINITY ? 0.f : exp2_sfu((m - top) * scale_log2);
+            m = top;
+            l *= alpha;
+          }
+          __syncwarp();
+          const float shift = m == -INFINITY ? 0.f : -m * scale_log2;
+          const uint64_t shift2 = f2(shift, shift);
+          if (!Shape::kOver && k > 0) {
+            // the product before this tile's reads P, which the stores below replace
+            if (!wide_warp_wait(s, &s.o_done[t], phase ^ 1, a.status)) {
+              ok = false;
+              break;
             }
-            if (bad) {
-              *reinterpret_cast<uint4*>(line + (e >> 3) * kBox +
-                                        (((e & 7) ^ (lane_row & 7)) << 4)) =
-                  make_uint4(clean[0], clean[1], clean[2], clean[3]);
-              *(volatile int*)&s.spoiled[t] = 1;
+            tc_fence_after();
+          }
+          // Streams that share their tiles take turns at the exponentials: both at once would each
+          // take twice as long and leave the tensor core idle for as long.
+          if (turns && (t == 1 || turn > 0) &&
+              !wide_warp_wait(s, &s.turn[t], (uint32_t)((turn - (t == 0 ? 1 : 0)) & 1),
+                              a.status)) {
+            ok = false;
+            break;
+          }
+          uint64_t sum2[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int quarter = 0; quarter < 4; ++quarter) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = quarter * 32; c < quarter * 32 + 32; c += 2) {
+              float lo, hi;
+              unf2(fma2(f2(sv[c], sv[c + 1]), scale2, shift2), lo, hi);
+              const float e0 = exp2_sfu(lo), e1 = exp2_sfu(hi);
+              sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], f2(e0, e1));
+              pk[(c >> 1) & 15] = Kind<T>::pack(e0, e1);
+            }
+            tmem_st16(p_addr + (uint32_t)(quarter * 16), pk);
+          }
+          if (turns) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.turn[t ^ 1]);
+          }
+          float s0, s1, s2, s3;
+          unf2(add2(sum2[0], sum2[1]), s0, s1);
+          unf2(add2(sum2[2], sum2[3]), s2, s3);
+          l += (s0 + s1) + (s2 + s3);
+          if (k > 0 && __any_sync(0xffffffffu, move)) {
+            // scale O of the rows whose maximum moved. Every product before this tile's is
+            // complete: S of this tile was issued behind the last (D = 128), or its barrier was
+            // waited for above.
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32_nowait(o_addr + (uint32_t)(c * 32), o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= alpha;
+              tmem_st32(o_addr + (uint32_t)(c * 32), o);
             }
           }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.p_full[t]);
-    }
-    // the row's result, once the stream's last product has completed
-    if (ok && mine > 0) {
-      ok = wide_warp_wait(s, &s.o_done[t], (uint32_t)((mine - 1) & 1), a.status);
-      tc_fence_after();
-    }
-    if (ok && busy && (t == 0 || both)) {
-      const int64_t slot = (int64_t)blockIdx.x * deal.streams + (deal.streams == 2 ? t : 0);
-      const Results results(a.workspace, a, deal, D);
-      const int64_t at = results.at(slot, kvh, (int64_t)node * group + row % group);
-      const int head = kvh * group + row % group;
-      const bool whole = deal.streams == 1 && part.parts == 1;
-      const float inv = 1.f / l;
-      T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
-               (int64_t)head * a.out_strides[2];
-      const bool spoiled = mine > 0 && *(volatile int*)&s.spoiled[t] != 0;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        if (mine > 0) {
-          tmem_ld32_nowait(o_addr + (uint32_t)(c * 32), o);
-          tmem_wait_ld();
+          tmem_wait_st();
         } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          // no rows in this warp: it only keeps the barriers' counts (its P rows are never read
+          // by a row that leaves the CTA), in step with the others: two arrivals of one warp in
+          // a phase of p_full would stand for another's
+          if (!Shape::kOver) {
+            if (lane == 0) mbar_arrive(&s.s_free[t]);
+            if (k > 0 && !wide_warp_wait(s, &s.o_done[t], phase ^ 1, a.status)) {
+              ok = false;
+              break;
+            }
+          }
+          if (turns) {
+            if ((t == 1 || turn > 0) &&
+                !wide_warp_wait(s, &s.turn[t], (uint32_t)((turn - (t == 0 ? 1 : 0)) & 1),
+                                a.status)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_arrive(&s.turn[t ^ 1]);
+          }
         }
-        if (spoiled && real) {
-          // add what the cleaning took out, to the rows that see it
-          for (int64_t k = 0; k < mine; ++k) {
-            const int64_t tile = part.first + tile_index(t, k) - cache_tiles;
-            if (tile < 0) continue;
-            const int n0 = (int)tile * kKeysTile;
-            const Sight sees = node_sight(parents, node, n0, part.count, nullptr);
-            for (int key = 0; key < kKeysTile && n0 + key < part.count; ++key) {
-              if (!sees.has(key)) continue;
+        turn += turns ? 1 : 0;
+        if (ragged) {
+          // clean the tile's values: thread = key
+          const int c = 2 * (base + index_of(t, k)) + 1;
+          const int slot = (int)(c % Shape::kSlots);
+          if (!wide_warp_wait(s, &s.full[slot], (uint32_t)((c / Shape::kSlots) & 1), a.status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* line = s.ring[slot] + lane_row * 128;
+          const int real_keys =
+              own ? seg.count - (tile - cache_tiles) * kKeysTile : left;
+          // piece by piece in the order that lies in different banks for neighbouring keys
+#pragma unroll 1
+          for (int x = 0; x < Shape::kBoxes; ++x)
+#pragma unroll 2
+            for (int e = 0; e < 8; ++e) {
+              uint4* piece = reinterpret_cast<uint4*>(line + x * kBox + ((e ^ (lane & 7)) << 4));
+              if (lane_row >= real_keys) {
+                *piece = make_uint4(0, 0, 0, 0);
+              } else if (own) {
+                const uint4 w = *piece;
+                const uint4 clean = make_uint4(finite_only<T>(w.x), finite_only<T>(w.y),
+                                               finite_only<T>(w.z), finite_only<T>(w.w));
+                if (clean.x != w.x || clean.y != w.y || clean.z != w.z || clean.w != w.w) {
+                  *(volatile int*)&s.spoiled[mark & 7] = mark;  // before the value goes
+                  *piece = clean;
+                }
+              }
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[t]);
+      }
+      // the row's result, once the stream's last product has completed
+      if (ok && mine > 0) {
+        ok = wide_warp_wait(s, &s.o_done[t], (uint32_t)((n + mine - 1) & 1), a.status);
+        tc_fence_after();
+      }
+      if (ok && busy) {
+        const bool spoiled = mine > 0 && *(volatile int*)&s.spoiled[mark & 7] == mark;
+        const int64_t at = results.at(seg.result + (deal.streams == 2 ? t : 0), tile_row);
+        const int head = seg.kvh * group + tile_row % group;
+        const float inv = 1.f / l;
+        T* out = static_cast<T*>(a.out) + seg.b * a.out_strides[0] + node * a.out_strides[1] +
+                 (int64_t)head * a.out_strides[2];
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          __syncwarp();  // rows differ in what they store; a tensor memory load is the whole warp's
+          if (mine > 0) {
+            tmem_ld32_nowait(o_addr + (uint32_t)(c * 32), o);
+            tmem_wait_ld();
+          } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                if (c * 32 + e >= d) continue;
-                const float v = (float)v_new[(n0 + key) * a.v_new_strides[1] + c * 32 + e];
-                if (!isfinite(v)) o[e] += v;
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (spoiled && real) {
+            // add what the cleaning took out, to the rows that see it
+            for (int k = 0; k < mine; ++k) {
+              const int tile = seg.first + index_of(t, k) - cache_tiles;
+              if (tile < 0) continue;
+              const int n0 = tile * kKeysTile;
+              const Sight sees = node_sight(parents, node, n0, seg.count);
+              for (int key = 0; key < kKeysTile && n0 + key < seg.count; ++key) {
+                if (!sees.has(key)) continue;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  if (c * 32 + e >= d) continue;
+                  const float v = (float)v_new[(n0 + key) * a.v_new_strides[1] + c * 32 + e];
+                  if (!isfinite(v)) o[e] += v;
+                }
               }
             }
           }
-        }
-        if (real && whole) {
+          if (real && seg.whole) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            if (c * 32 + e < d)
-              *reinterpret_cast<uint4*>(out + c * 32 + e) = make_uint4(
-                  Kind<T>::pack(o[e] * inv, o[e + 1] * inv),
-                  Kind<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
-                  Kind<T>::pack(o[e + 4] * inv, o[e + 5] * inv),
-                  Kind<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
+            for (int e = 0; e < 32; e += 8)
+              if (c * 32 + e < d)
+                *reinterpret_cast<uint4*>(out + c * 32 + e) = make_uint4(
+                    Kind<T>::pack(o[e] * inv, o[e + 1] * inv),
+                    Kind<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
+                    Kind<T>::pack(o[e + 4] * inv, o[e + 5] * inv),
+                    Kind<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
+          } else if (real) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(results.out + at * D + c * 32 + e) =
+                  make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        const float m_log2 = m == -INFINITY ? m : m * scale_log2;
+        if (real && seg.whole) {
+          if (a.lse != nullptr)
+            a.lse[((int64_t)seg.b * a.heads + head) * a.nodes + node] =
+                (m_log2 + log2f(l)) * mma16::kLn2;
         } else if (real) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(results.out + at * D + c * 32 + e) =
-                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          results.top[at] = make_float2(m_log2, l);
         }
       }
-      const float m_log2 = m == -INFINITY ? m : m * scale_log2;
-      if (real && whole) {
-        if (a.lse != nullptr)
-          a.lse[((int64_t)b * a.heads + head) * a.nodes + node] =
-              (m_log2 + log2f(l)) * mma16::kLn2;
-      } else if (real) {
-        results.top[at] = make_float2(m_log2, l);
-      }
+      __syncwarp();
+      tc_fence_before();  // O has been read before the next segment's first product
+      base += seg.tiles;
+      n += mine;
+      ++mark;
     }
   }
   tc_fence_before();
@@ -661,12 +708,11 @@ inline bool wide_map(CUtensorMap* map, const void* base, bool bf16, int64_t colu
 // How the rows lie in tiles; tile_nodes 0 when a key head's group does not fit a tile.
 inline WideRows wide_rows(const Args& a) {
   WideRows w;
-  w.group = (int)(a.heads / a.kv_heads);
-  w.half = a.nodes <= 64 / w.group;
-  w.tile_nodes = w.half ? 64 / w.group : kRowsTile / w.group;
+  const int group = (int)(a.heads / a.kv_heads);
+  w.half = a.nodes <= 64 / group;
+  w.tile_nodes = w.half ? 64 / group : kRowsTile / group;
   w.share = w.tile_nodes > 0 && a.nodes > w.tile_nodes;
   if (w.tile_nodes > a.nodes) w.tile_nodes = (int)a.nodes;
-  w.pairs = w.share ? (int)((a.nodes + 2 * w.tile_nodes - 1) / (2 * w.tile_nodes)) : 1;
   return w;
 }
 
@@ -676,7 +722,7 @@ inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& 
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const int64_t d = a.head_dim, kv = a.kv_heads;
   WideMaps maps;
-  if (!wide_map(&maps.q, a.q, bf16, d, a.heads, a.q_strides[2], w.group, a.nodes,
+  if (!wide_map(&maps.q, a.q, bf16, d, a.heads, a.q_strides[2], deal.group, a.nodes,
                 a.q_strides[1], w.tile_nodes, a.batch, a.q_strides[0]) ||
       !wide_map(&maps.keys, a.keys, bf16, d, a.capacity, a.keys_strides[2], kKeysTile, kv,
                 a.keys_strides[1], 1, a.batch, a.keys_strides[0]) ||
@@ -703,8 +749,8 @@ inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& 
       &ready);
   if (e != cudaSuccess) return e;
   if (ready != 1) return cudaErrorInvalidKernelImage;
-  return launch_pdl(kernel, dim3((unsigned)deal.slots, (unsigned)(a.kv_heads * w.pairs)),
-                    dim3(kWideThreads), smem, stream, maps, a, deal, w);
+  return launch_pdl(kernel, dim3((unsigned)deal.grid), dim3(kWideThreads), smem, stream, maps, a,
+                    deal, w);
 }
 
 }  // namespace tree
