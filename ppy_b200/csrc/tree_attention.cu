@@ -40,6 +40,7 @@ constexpr int kTile = 64;       // keys a tile
 constexpr int kStages = 3;      // tiles in flight
 constexpr int kRows = 16;       // rows a CTA
 constexpr int kWarps = 4;       // along a tile's keys
+constexpr int kJoinRows = 16;   // rows of an item that a CTA joins
 constexpr int kTreeWords = PPYB200_TREE_NODES / 32;
 
 // Shared memory rows of D elements: 16-byte pieces XORed with the row's low bits, so that the
@@ -132,6 +133,9 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
   }
 
   ppyb200::tree::append<T>(a, deal, seg, tid, kThreads);
+
+  if (seg.starts && tid == 0)
+    Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
 
   // query fragments: the 16 rows, zero beyond the rows and the head size
   const int ra = row0 + gid, rb = ra + 8;
@@ -369,66 +373,54 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
   }
 }
 
-// One warp a row: joins the unnormalised results of an item's segments in their order.
-template <class T, int D, int TILE, bool APART>
+// Joins the unnormalised results of an item's segments in their order: CTA (item, rows) takes
+// sixteen rows, a warp a row at a time.
+template <class T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a,
                                                    const Deal deal) {
   ppyb200::pdl_wait();
-  const int group = deal.group, rows = (int)a.nodes * group, kv_heads = (int)a.kv_heads;
-  const int index = (int)(blockIdx.x * 4 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
-  if (index >= (int)a.batch * kv_heads * rows) return;
-  const int row = index % rows, kvh = index / rows % kv_heads, b = index / rows / kv_heads;
-  const int node = row / group, head = kvh * group + row % group;
+  const int number = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int items = (int)a.batch * deal.items, kvh = number / items, item = number - kvh * items;
+  const int b = item / deal.items, row0 = (item - b * deal.items) * deal.item_rows;
+  const Results results(a, deal, D);
+  const int2 ctas = results.ctas[number];  // meaningless where the item has no rows
   int length, count;
   sequence_extent(a, b, length, count, nullptr);
-  if (node >= count) return;
-  // the item's place on the axis, and the CTAs whose shares hold it
-  Walk<TILE, APART> walk;
-  walk.measure(a, deal, nullptr);
-  const int item = b * deal.items + row / deal.item_rows;
-  int64_t start = 0;
-  for (int i = lane; i < item; i += 32) {
-    int other, nodes;
-    sequence_extent(a, i / deal.items, other, nodes, nullptr);
-    start += ppyb200::tree::item_tiles<TILE, APART>(a, deal, other, nodes, i % deal.items);
-  }
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) start += __shfl_xor_sync(0xffffffffu, start, w);
-  start += kvh * walk.span;
-  const int tiles =
-      ppyb200::tree::item_tiles<TILE, APART>(a, deal, length, count, item % deal.items);
-  const int c0 = walk.cta_of(a, start), c1 = walk.cta_of(a, start + tiles - 1);
-  if (deal.streams == 1 && c0 == c1) return;  // whole: written by its CTA
-  const Results results(a, deal, D);
+  if (deal.streams == 1 && ctas.x == ctas.y) return;  // whole: written by its CTA
+  const int parts = (ctas.y - ctas.x + 1) * deal.streams;
   // the first segment starts the item, the others continue it
-  auto place = [&](int i) {
-    const int c = c0 + i / deal.streams;
-    return results.at(walk.result_of(a, deal, c, kvh, item, c == c0) + i % deal.streams,
-                      row % deal.item_rows);
+  auto place = [&](int i, int r) {
+    const int c = ctas.x + i / deal.streams;
+    return results.at(Walk<kTile, false>::result_of(deal, c, number, c == ctas.x) +
+                          i % deal.streams, r);
   };
-  const int parts = (c1 - c0 + 1) * deal.streams;
-  float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, results.top[place(i)].x);
+  const int end = min(deal.item_rows, (int)(blockIdx.y + 1) * kJoinRows);
+  for (int r = blockIdx.y * kJoinRows + warp; r < end; r += 4) {
+    const int node = (row0 + r) / deal.group;
+    if (node >= count) return;
+    float m = -INFINITY, l = 0.f, sum[D / 32];
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, results.top[place(i, r)].x);
 #pragma unroll
-  for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-  const float u = m == -INFINITY ? 0.f : m;
-  float l = 0.f, sum[D / 32];
+    for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+    const float u = m == -INFINITY ? 0.f : m;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
+    for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const int64_t at = place(i);
-    const float2 top = results.top[at];
-    const float f = exp2_sfu(top.x - u);
-    l += f * top.y;
+    for (int i = 0; i < parts; ++i) {
+      const int64_t at = place(i, r);
+      const float2 top = results.top[at];
+      const float f = exp2_sfu(top.x - u);
+      l += f * top.y;
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k) {
-      const float2 v = *reinterpret_cast<const float2*>(results.out + at * D + k * 64 + lane * 2);
-      sum[2 * k] += f * v.x;
-      sum[2 * k + 1] += f * v.y;
+      for (int k = 0; k < D / 64; ++k) {
+        const float2 v =
+            *reinterpret_cast<const float2*>(results.out + at * D + k * 64 + lane * 2);
+        sum[2 * k] += f * v.x;
+        sum[2 * k + 1] += f * v.y;
+      }
     }
+    write_row<T, D>(a, b, node, kvh * deal.group + (row0 + r) % deal.group, lane, m, l, sum);
   }
-  write_row<T, D>(a, b, node, head, lane, m, l, sum);
 }
 
 // ---------------------------------------------------------------- host
@@ -490,11 +482,11 @@ Plan plan_for(const Args& a, bool wide, int sm_count) {
   return p;
 }
 
-template <class T, int D, int TILE, bool APART>
+template <class T, int D>
 cudaError_t join(const Args& a, const Plan& p, cudaStream_t stream) {
-  const int64_t rows = a.batch * a.heads * a.nodes;
-  return ppyb200::launch_pdl(join_kernel<T, D, TILE, APART>, dim3((unsigned)((rows + 3) / 4)),
-                             dim3(128), 0, stream, a, p.deal);
+  const dim3 grid((unsigned)(a.kv_heads * a.batch * p.deal.items),
+                  (unsigned)((p.deal.item_rows + kJoinRows - 1) / kJoinRows));
+  return ppyb200::launch_pdl(join_kernel<T, D>, grid, dim3(128), 0, stream, a, p.deal);
 }
 
 template <class T, int D>
@@ -514,14 +506,9 @@ cudaError_t launch_narrow(const Args& a, const Plan& p, cudaStream_t stream) {
 
 template <class T, int D>
 cudaError_t launch_dim(const Args& a, const Plan& p, cudaStream_t stream) {
-  cudaError_t e;
-  if (p.wide) {
-    e = ppyb200::tree::launch_wide<T, D>(a, p.deal, p.rows, stream);
-    return e == cudaSuccess && p.join ? join<T, D, ppyb200::tree::kKeysTile, true>(a, p, stream)
-                                      : e;
-  }
-  e = launch_narrow<T, D>(a, p, stream);
-  return e == cudaSuccess && p.join ? join<T, D, kTile, false>(a, p, stream) : e;
+  const cudaError_t e = p.wide ? ppyb200::tree::launch_wide<T, D>(a, p.deal, p.rows, stream)
+                               : launch_narrow<T, D>(a, p, stream);
+  return e == cudaSuccess && p.join ? join<T, D>(a, p, stream) : e;
 }
 
 template <class T>

@@ -50,7 +50,9 @@ struct Segment {
   int row0;              // the item's first row
   int length, count;     // the sequence's extent
   int first, tiles;      // the key tiles to walk
-  bool whole;            // all of the item's
+  bool starts, whole;    // from the item's first tile; all of them, by one stream
+  int number;            // the item's on the axis
+  int last_cta;          // of those that share the item (where this segment starts it)
   int64_t result;        // the first in the workspace, unless whole
 };
 
@@ -77,7 +79,7 @@ __device__ __forceinline__ int item_tiles(const Args& a, const Deal& deal, int l
 // The axis: tiles of one key head's items (`span`), the CTAs that share it, and a CTA's place.
 template <int TILE, bool APART>
 struct Walk {
-  int64_t span;
+  int64_t span, place;  // `place`: of the next tile, on the axis
   int left, offset, ctas, cta, kvh, item;
 
   // A warp together. Extents that are out of range raise `status`.
@@ -104,10 +106,9 @@ struct Walk {
   // The first of the results that CTA c leaves of an item (one a stream): a CTA has at most one
   // segment that continues an item and one that starts an item without ending it, and c + the
   // item's number on the axis tells all segments apart.
-  __device__ __forceinline__ static int64_t result_of(const Args& a, const Deal& deal, int c,
-                                                      int kvh, int item, bool starts) {
-    if (deal.streams == 1) return 2 * (int64_t)c + (starts ? 1 : 0);
-    return 2 * (c + (int64_t)kvh * a.batch * deal.items + item);
+  __device__ __forceinline__ static int64_t result_of(const Deal& deal, int c, int number,
+                                                      bool starts) {
+    return deal.streams == 1 ? 2 * (int64_t)c + (starts ? 1 : 0) : 2 * ((int64_t)c + number);
   }
   // To the start of CTA c's share (a warp together).
   __device__ __forceinline__ void enter(const Args& a, const Deal& deal, int c) {
@@ -118,6 +119,7 @@ struct Walk {
     offset = 0;
     if (c >= ctas || span == 0) return;
     const int64_t start = start_of(a, c);
+    place = start;
     left = (int)(start_of(a, c + 1) - start);
     kvh = (int)quotient(start, span);
     int64_t rest = start - kvh * span;
@@ -156,8 +158,12 @@ struct Walk {
         s.row0 = r * deal.item_rows;
         s.first = offset;
         s.tiles = min(tiles - offset, left);
+        s.starts = offset == 0;
         s.whole = s.tiles == tiles && deal.streams == 1;
-        s.result = result_of(a, deal, cta, kvh, item, offset == 0);
+        s.number = kvh * (int)a.batch * deal.items + item;
+        s.result = result_of(deal, cta, s.number, s.starts);
+        s.last_cta = s.tiles == tiles ? cta : cta_of(a, place + tiles - 1);
+        place += s.tiles;
         left -= s.tiles;
         offset += s.tiles;
         return true;
@@ -173,11 +179,11 @@ struct Walk {
 };
 
 // The nodes whose first row lies in an item are appended by the segment that starts the item, by
-// `threads` threads of which this is the `thread`-th.
+// `threads` threads of which this is the `thread`-th, four pieces in flight each.
 template <class T>
 __device__ __forceinline__ void append(const Args& a, const Deal& deal, const Segment& s,
                                        int thread, int threads) {
-  if (s.first != 0) return;
+  if (!s.starts) return;
   const int from = (s.row0 + deal.group - 1) / deal.group;
   const int to = min(s.count, (s.row0 + deal.item_rows + deal.group - 1) / deal.group);
   const T* k_new = static_cast<const T*>(a.k_new) + s.b * a.k_new_strides[0] +
@@ -186,22 +192,36 @@ __device__ __forceinline__ void append(const Args& a, const Deal& deal, const Se
                    s.kvh * a.v_new_strides[2];
   T* keys = static_cast<T*>(a.keys) + s.b * a.keys_strides[0] + s.kvh * a.keys_strides[1];
   T* values = static_cast<T*>(a.values) + s.b * a.values_strides[0] + s.kvh * a.values_strides[1];
-  const int pieces = (int)a.head_dim / 8;
-  for (int i = thread; i < (to - from) * pieces; i += threads) {
-    const int64_t n = from + i / pieces, j = s.length + n;
-    const int x = i % pieces * 8;
-    *reinterpret_cast<uint4*>(keys + j * a.keys_strides[2] + x) =
-        *reinterpret_cast<const uint4*>(k_new + n * a.k_new_strides[1] + x);
-    *reinterpret_cast<uint4*>(values + j * a.values_strides[2] + x) =
-        *reinterpret_cast<const uint4*>(v_new + n * a.v_new_strides[1] + x);
+  const int pieces = (int)a.head_dim / 8, total = (to - from) * pieces * 2;
+  for (int i0 = thread; i0 < total; i0 += 4 * threads) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {  // keys and values in turn
+      const int i = i0 + u * threads;
+      const int64_t n = from + (i >> 1) / pieces;
+      const int x = (i >> 1) % pieces * 8;
+      if (i < total)
+        v[u] = *reinterpret_cast<const uint4*>((i & 1) == 0 ? k_new + n * a.k_new_strides[1] + x
+                                                            : v_new + n * a.v_new_strides[1] + x);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * threads;
+      const int64_t n = from + (i >> 1) / pieces, j = s.length + n;
+      const int x = (i >> 1) % pieces * 8;
+      if (i < total)
+        *reinterpret_cast<uint4*>((i & 1) == 0 ? keys + j * a.keys_strides[2] + x
+                                               : values + j * a.values_strides[2] + x) = v[u];
+    }
   }
 }
 
 // The workspace: unnormalised outputs [results][item_rows][D] f32, then maximum (in powers of two)
-// and sum [results][item_rows][2].
+// and sum [results][item_rows][2], then the first and last CTA of each item on the axis.
 struct Results {
   float* out;
   float2* top;
+  int2* ctas;
   int item_rows;
   __host__ __device__ __forceinline__ static int64_t count(const Args& a, const Deal& deal) {
     return 2 * (deal.grid + (deal.streams == 1 ? 0 : a.kv_heads * a.batch * deal.items));
@@ -210,12 +230,14 @@ struct Results {
       : item_rows(deal.item_rows) {
     out = static_cast<float*>(a.workspace);
     top = reinterpret_cast<float2*>(out + count(a, deal) * item_rows * dim);
+    ctas = reinterpret_cast<int2*>(top + count(a, deal) * item_rows);
   }
   __device__ __forceinline__ int64_t at(int64_t result, int64_t row) const {
     return result * item_rows + row;
   }
   static int64_t bytes(const Args& a, const Deal& deal, int dim) {
-    return count(a, deal) * deal.item_rows * (dim + 2) * 4;
+    return count(a, deal) * deal.item_rows * (dim + 2) * 4 +
+           a.kv_heads * a.batch * deal.items * 8;
   }
 };
 

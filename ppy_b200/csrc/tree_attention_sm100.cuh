@@ -24,11 +24,10 @@
 // shared memory before the product: rows behind the sequence are zeroed, and so are single
 // values of nodes that are not finite, which the last step adds to the rows that see them.
 //
-//   warps 0-7  softmax (warpgroup t = stream t; warp w reads TMEM lanes 32 (w % 4) ...), and the
-//              append of a segment's nodes to the cache
-//   warp 8     one thread: TMA loads of Q, K and V (a ring of K and V tiles in turn)
+//   warps 0-7  softmax (warpgroup t = stream t; warp w reads TMEM lanes 32 (w % 4) ...)
+//   warp 8     TMA loads of Q, K and V (a ring of K and V tiles in turn), by one thread
 //   warps 9,10 one thread each: the MMAs of stream 0 and 1; warp 9 owns the TMEM
-//   warp 11    idle: it completes the third warpgroup
+//   warp 11    appends a segment's nodes to the cache
 //
 // Every mbarrier wait is bounded: on giving up the CTA raises the status, every role leaves its
 // loop, copies and MMAs in flight are drained and the TMEM is freed.
@@ -107,6 +106,25 @@ __device__ __forceinline__ void support_registers() {
 __device__ __forceinline__ void softmax_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
 }
+
+// The ring's entries. Streams that share their tiles take every entry in one order. Streams that do
+// not have slots of their own (the first kSlots - kSlots / 2, and the rest): loads complete in
+// any order, and a stream that came round to a slot of the other's could take the completion
+// before last for its own, the barrier's phases being told apart by parity only.
+template <int D>
+struct Entry {
+  int slot;
+  uint32_t parity;
+  static constexpr int kAll = WideShape<D>::kSlots, kRest = kAll / 2, kFirst = kAll - kRest;
+  __device__ __forceinline__ static int slots(bool share, int t) {
+    return share ? kAll : t == 0 ? kFirst : kRest;
+  }
+  __device__ __forceinline__ Entry(bool share, int t, int e) {
+    const int round = share ? e / kAll : t == 0 ? e / kFirst : e / kRest;
+    slot = e - round * slots(share, t) + (share || t == 0 ? 0 : kFirst);
+    parity = (uint32_t)(round & 1);
+  }
+};
 
 // The launch's tensor maps: [columns][slots or nodes][key heads][batch], and for q [columns]
 // [heads][nodes][batch].
@@ -271,45 +289,84 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
 
   if (warp == 8) {
     support_registers();
-    if (lane == 0) {
-      // ---- loader: a segment's Q, then K and V of its tiles; K of the CTA's i-th tile is entry
-      // 2 i of the ring, its V entry 2 i + 1
-      const uint32_t q_bytes = (uint32_t)(Shape::kBoxes * wide.tile_nodes * group * 128);
-      int c = 0, segments = 0;
-      bool ok = true;
-      for (; ok && walk.next(a, deal, seg); ++segments) {
-        if (!wide_wait(s, &s.q_empty, (uint32_t)((segments & 1) ^ 1), a.status)) break;
-        const int streams = both_of(seg) ? 2 : 1;
-        const int node0 = seg.row0 / group;
-        mbar_expect_tx(&s.q_full, streams * q_bytes);
-        for (int t = 0; t < streams; ++t)
-          for (int x = 0; x < Shape::kBoxes; ++x)
-            tma_load_4d(s.q[t] + x * kBox + (wide.half && t == 1 ? kBox / 2 : 0), &maps.q,
-                        &s.q_full, x * 64, seg.kvh * group,
-                        node0 + (wide.share ? t * wide.tile_nodes : 0), seg.b);
-        const int cache_tiles = cache_tiles_of(seg);
-        for (int i = 0; i < seg.tiles && ok; ++i) {
-          const int tile = seg.first + i;
-          const bool own = tile >= cache_tiles;
-          const int at = (own ? tile - cache_tiles : tile) * kKeysTile;
-          for (int v = 0; v < 2; ++v, ++c) {
-            const int slot = (int)(c % Shape::kSlots);
-            if (!wide_wait(s, &s.empty[slot], (uint32_t)(((c / Shape::kSlots) & 1) ^ 1),
-                           a.status)) {
-              ok = false;
-              break;
-            }
-            const CUtensorMap* map = own ? (v == 0 ? &maps.k_new : &maps.v_new)
-                                         : (v == 0 ? &maps.keys : &maps.values);
-            mbar_expect_tx(&s.full[slot], Shape::kTileBytes);
+    // ---- loader: lane 0 loads a segment's Q, then K and V of its tiles (K of the CTA's i-th tile
+    // is entry 2 i of the ring, its V entry 2 i + 1); the warp together leaves a tree's parents in
+    // shared memory before the first node tile
+    const uint32_t q_bytes = (uint32_t)(Shape::kBoxes * wide.tile_nodes * group * 128);
+    int loaded[2] = {0, 0}, segments = 0;  // entries of each stream (of both, when they share)
+    bool ok = true;
+    for (; ok && walk.next(a, deal, seg); ++segments) {
+      const int cache_tiles = cache_tiles_of(seg);
+      const bool tree = a.parents != nullptr && seg.first + seg.tiles > cache_tiles;
+      int parent[8];
+      if (tree) {
+        const int32_t* from = a.parents + (int64_t)seg.b * a.parents_stride;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          parent[i] = i * 32 + lane < seg.count ? from[i * 32 + lane] : -1;
+      }
+      if (lane == 0) {
+        ok = wide_wait(s, &s.q_empty, (uint32_t)((segments & 1) ^ 1), a.status);
+        if (ok) {
+          const int streams = both_of(seg) ? 2 : 1;
+          const int node0 = seg.row0 / group;
+          mbar_expect_tx(&s.q_full, streams * q_bytes);
+          for (int t = 0; t < streams; ++t)
             for (int x = 0; x < Shape::kBoxes; ++x)
-              tma_load_4d(s.ring[slot] + x * kBox, map, &s.full[slot], x * 64, at, seg.kvh, seg.b);
-          }
+              tma_load_4d(s.q[t] + x * kBox + (wide.half && t == 1 ? kBox / 2 : 0), &maps.q,
+                          &s.q_full, x * 64, seg.kvh * group,
+                          node0 + (wide.share ? t * wide.tile_nodes : 0), seg.b);
         }
       }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (!ok) break;
+      for (int part = 0; part < 2; ++part) {  // the cache's tiles, then the nodes'
+        const bool own = part == 1;
+        const int from = own ? max(seg.first, cache_tiles) : seg.first;
+        const int to = own ? seg.first + seg.tiles : min(seg.first + seg.tiles, cache_tiles);
+        if (own && tree) {
+          // up to 256 nodes: each parent a byte, 255 for a root, as any that is no earlier node
+          // is taken
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int node = i * 32 + lane, p = parent[i];
+            if (p < -1 || (p >= node && node < seg.count)) raise(a.status);
+            s.parents[segments % Shape::kTrees][node] =
+                p >= 0 && p < node ? (uint8_t)p : (uint8_t)255;
+          }
+          __syncwarp();
+        }
+        if (lane == 0) {
+          for (int tile = from; tile < to && ok; ++tile) {
+            const int at = (own ? tile - cache_tiles : tile) * kKeysTile;
+            const int t = wide.share ? 0 : (tile - seg.first) & 1;
+            for (int v = 0; v < 2; ++v) {
+              const Entry<D> entry(wide.share, t, t == 0 ? loaded[0] : loaded[1]);
+              if (!wide_wait(s, &s.empty[entry.slot], entry.parity ^ 1, a.status)) {
+                ok = false;
+                break;
+              }
+              const CUtensorMap* map = own ? (v == 0 ? &maps.k_new : &maps.v_new)
+                                           : (v == 0 ? &maps.keys : &maps.values);
+              mbar_expect_tx(&s.full[entry.slot], Shape::kTileBytes);
+              for (int x = 0; x < Shape::kBoxes; ++x)
+                tma_load_4d(s.ring[entry.slot] + x * kBox, map, &s.full[entry.slot], x * 64, at,
+                            seg.kvh, seg.b);
+              if (t == 0) ++loaded[0];
+              else ++loaded[1];
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      }
+    }
+    if (lane == 0) {
       // the copies issued here land before the CTA may leave
-      for (int j = c > Shape::kSlots ? c - Shape::kSlots : 0; j < c; ++j)
-        mbar_drain_wait(&s.full[j % Shape::kSlots], (uint32_t)((j / Shape::kSlots) & 1));
+      for (int t = 0; t < 2; ++t)
+        for (int e = max(0, loaded[t] - Entry<D>::slots(wide.share, t)); e < loaded[t]; ++e) {
+          const Entry<D> entry(wide.share, t, e);
+          mbar_drain_wait(&s.full[entry.slot], entry.parity);
+        }
       if (segments > 0) mbar_drain_wait(&s.q_full, (uint32_t)((segments - 1) & 1));
     }
   } else if (warp == 9 || warp == 10) {
@@ -323,21 +380,23 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       const uint32_t s_col = tmem + (uint32_t)(t * kKeysTile);
       const uint32_t o_col = tmem + Shape::kOCol + (uint32_t)(t * D);
       const uint32_t p_col = tmem + Shape::kPCol + (uint32_t)(t * Shape::kPStep);
-      int base = 0, n = 0, segments = 0;  // tiles before this segment's; this stream's so far
+      int base = 0, n = 0, segments = 0;  // tiles so far: of both streams, and of this one
       bool ok = true;
-      auto full = [&](int c) {
-        return wide_wait(s, &s.full[c % Shape::kSlots], (uint32_t)((c / Shape::kSlots) & 1),
-                         a.status);
+      auto full = [&](const Entry<D>& entry) {
+        return wide_wait(s, &s.full[entry.slot], entry.parity, a.status);
+      };
+      auto entry_of = [&](int k, int v) {  // K (v = 0) or V of this stream's tile k
+        return Entry<D>(wide.share, t, 2 * ((wide.share ? base : n) + k) + v);
       };
       // S = Q K^T of this stream's tile k of the segment, its (n + k)-th in all
       auto scores = [&](int k) -> bool {
-        const int c = 2 * (base + index_of(t, k));
-        if (!full(c)) return false;
+        const Entry<D> entry = entry_of(k, 0);
+        if (!full(entry)) return false;
         if (!Shape::kOver && n + k > 0 &&
             !wide_wait(s, &s.s_free[t], (uint32_t)((n + k - 1) & 1), a.status))
           return false;
         tc_fence_after();
-        const uint8_t* key = s.ring[c % Shape::kSlots];
+        const uint8_t* key = s.ring[entry.slot];
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const int box = kk >> 2, off = (kk & 3) * 2;
@@ -346,22 +405,22 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
               kk > 0 ? 1u : 0u);
         }
         commit(&s.s_full[t]);
-        commit(&s.empty[c % Shape::kSlots]);
+        commit(&s.empty[entry.slot]);
         return true;
       };
       // O += P V of tile k
       auto product = [&](int k) -> bool {
-        const int c = 2 * (base + index_of(t, k)) + 1;
-        if (!full(c) || !wide_wait(s, &s.p_full[t], (uint32_t)((n + k) & 1), a.status))
+        const Entry<D> entry = entry_of(k, 1);
+        if (!full(entry) || !wide_wait(s, &s.p_full[t], (uint32_t)((n + k) & 1), a.status))
           return false;
         tc_fence_after();
-        const uint64_t value = smem_desc_mn(s.ring[c % Shape::kSlots]);
+        const uint64_t value = smem_desc_mn(s.ring[entry.slot]);
 #pragma unroll
         for (int kk = 0; kk < kKeysTile / 16; ++kk)  // 16 keys: two groups of 1024 bytes
           mma_ts(o_col, p_col + (uint32_t)(kk * 8), value + (uint64_t)(kk * (2048 >> 4)),
                  idesc_o<T, D>(), k > 0 || kk > 0 ? 1u : 0u);
         commit(&s.o_done[t]);
-        commit(&s.empty[c % Shape::kSlots]);
+        commit(&s.empty[entry.slot]);
         return true;
       };
       for (; ok && walk.next(a, deal, seg); ++segments) {
@@ -369,9 +428,10 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         if (!wide_wait(s, &s.q_full, (uint32_t)(segments & 1), a.status)) break;
         if (mine == 0) {
           mbar_arrive(&s.q_empty);
-          for (int c = 2 * base; wide.share && ok && c < 2 * (base + seg.tiles); ++c) {
-            ok = full(c);
-            if (ok) mbar_arrive(&s.empty[c % Shape::kSlots]);
+          for (int i = 0; wide.share && ok && i < 2 * seg.tiles; ++i) {
+            const Entry<D> entry = entry_of(i >> 1, i & 1);
+            ok = full(entry);
+            if (ok) mbar_arrive(&s.empty[entry.slot]);
           }
         } else {
           ok = scores(0);
@@ -389,7 +449,13 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       mbar_drain_wait(&s.drain[t], 0);
     }
   } else if (warp == 11) {
-    support_registers();  // completes the third warpgroup
+    support_registers();
+    // ---- append, and where the join finds an item's results
+    while (walk.next(a, deal, seg)) {
+      if (seg.starts && lane == 0)
+        Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
+      append<T>(a, deal, seg, lane, 32);
+    }
   } else {
     softmax_registers();
     // ---- softmax: warpgroup t, thread = row (a TMEM lane) and, when cleaning, a key
@@ -408,7 +474,6 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     int turn = 0;         // tiles of shared segments so far
     bool ok = true;
     while (ok && walk.next(a, deal, seg)) {
-      append<T>(a, deal, seg, threadIdx.x, 256);
       const int mine = count_of(seg, t);
       const bool turns = wide.share && both_of(seg);
       const int cache_tiles = cache_tiles_of(seg);
@@ -416,20 +481,9 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       const int node = (seg.row0 + tile_row) / group;
       const bool real = row >= 0 && row < wide.tile_nodes * group && node < seg.count;
       const bool busy = __any_sync(0xffffffffu, real) != 0;  // the warp has rows
-      const uint8_t* parents = nullptr;
-      if (a.parents != nullptr && seg.first + seg.tiles > cache_tiles) {
-        // a tree of up to 256 nodes: each parent a byte, 255 for a root, as any that is no earlier
-        // node is taken; every warp writes the same bytes
-        uint8_t* to = s.parents[mark % Shape::kTrees];
-        const int32_t* from = a.parents + (int64_t)seg.b * a.parents_stride;
-        for (int i = lane; i < seg.count; i += 32) {
-          const int p = from[i];
-          if (p < -1 || p >= i) raise(a.status);
-          to[i] = p >= 0 && p < i ? (uint8_t)p : (uint8_t)255;
-        }
-        __syncwarp();
-        parents = to;
-      }
+      // the loader's, there before the first node tile's keys
+      const uint8_t* parents =
+          a.parents == nullptr ? nullptr : s.parents[(mark - 1) % Shape::kTrees];
       const T* v_new = static_cast<const T*>(a.v_new) + seg.b * a.v_new_strides[0] +
                        seg.kvh * a.v_new_strides[2];
       float m = -INFINITY, l = 0.f;  // m in raw score units
@@ -564,13 +618,12 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         turn += turns ? 1 : 0;
         if (ragged) {
           // clean the tile's values: thread = key
-          const int c = 2 * (base + index_of(t, k)) + 1;
-          const int slot = (int)(c % Shape::kSlots);
-          if (!wide_warp_wait(s, &s.full[slot], (uint32_t)((c / Shape::kSlots) & 1), a.status)) {
+          const Entry<D> entry(wide.share, t, 2 * ((wide.share ? base : n) + k) + 1);
+          if (!wide_warp_wait(s, &s.full[entry.slot], entry.parity, a.status)) {
             ok = false;
             break;
           }
-          uint8_t* line = s.ring[slot] + lane_row * 128;
+          uint8_t* line = s.ring[entry.slot] + lane_row * 128;
           const int real_keys =
               own ? seg.count - (tile - cache_tiles) * kKeysTile : left;
           // piece by piece in the order that lies in different banks for neighbouring keys
