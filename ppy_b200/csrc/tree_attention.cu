@@ -40,7 +40,7 @@ constexpr int kTile = 64;       // keys a tile
 constexpr int kStages = 3;      // tiles in flight
 constexpr int kRows = 16;       // rows a CTA
 constexpr int kWarps = 4;       // along a tile's keys
-constexpr int kJoinRows = 16;   // rows of an item that a CTA joins
+constexpr int kJoinRows = 4;    // rows of an item that a CTA joins, a warp each
 constexpr int kTreeWords = PPYB200_TREE_NODES / 32;
 
 // Shared memory rows of D elements: 16-byte pieces XORed with the row's low bits, so that the
@@ -373,54 +373,71 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
   }
 }
 
-// Joins the unnormalised results of an item's segments in their order: CTA (item, rows) takes
-// sixteen rows, a warp a row at a time.
+// Joins the unnormalised results of an item's segments in their order, a warp a row. What it costs
+// is the latency of its loads one after another, so the outputs of the first eight results are
+// under way before the maxima are known.
 template <class T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a,
-                                                   const Deal deal) {
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ Args a,
+                                                              const Deal deal) {
   ppyb200::pdl_wait();
-  const int number = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int number = blockIdx.x, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
   const int items = (int)a.batch * deal.items, kvh = number / items, item = number - kvh * items;
-  const int b = item / deal.items, row0 = (item - b * deal.items) * deal.item_rows;
+  const int b = item / deal.items, row = (item - b * deal.items) * deal.item_rows + r;
+  const int node = row / deal.group;
   const Results results(a, deal, D);
   const int2 ctas = results.ctas[number];  // meaningless where the item has no rows
   int length, count;
   sequence_extent(a, b, length, count, nullptr);
+  if (r >= deal.item_rows || node >= count) return;
   if (deal.streams == 1 && ctas.x == ctas.y) return;  // whole: written by its CTA
   const int parts = (ctas.y - ctas.x + 1) * deal.streams;
   // the first segment starts the item, the others continue it
-  auto place = [&](int i, int r) {
+  auto place = [&](int i) {
     const int c = ctas.x + i / deal.streams;
     return results.at(Walk<kTile, false>::result_of(deal, c, number, c == ctas.x) +
                           i % deal.streams, r);
   };
-  const int end = min(deal.item_rows, (int)(blockIdx.y + 1) * kJoinRows);
-  for (int r = blockIdx.y * kJoinRows + warp; r < end; r += 4) {
-    const int node = (row0 + r) / deal.group;
-    if (node >= count) return;
-    float m = -INFINITY, l = 0.f, sum[D / 32];
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, results.top[place(i, r)].x);
+  constexpr int kBatch = 8;
+  float m = -INFINITY, l = 0.f, sum[D / 32];
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-    const float u = m == -INFINITY ? 0.f : m;
+  for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += kBatch) {
+    const int n = min(kBatch, parts - i0);
+    float2 v[kBatch][D / 64];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const int64_t at = place(i, r);
-      const float2 top = results.top[at];
-      const float f = exp2_sfu(top.x - u);
-      l += f * top.y;
+    for (int i = 0; i < kBatch; ++i)
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        const float2 v =
-            *reinterpret_cast<const float2*>(results.out + at * D + k * 64 + lane * 2);
-        sum[2 * k] += f * v.x;
-        sum[2 * k + 1] += f * v.y;
+      for (int k = 0; k < D / 64; ++k)
+        if (i < n)
+          v[i][k] = *reinterpret_cast<const float2*>(results.out + place(i0 + i) * D + k * 64 +
+                                                     lane * 2);
+    const float2 top = lane < n ? results.top[place(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    float most = fmaxf(m, top.x);
+#pragma unroll
+    for (int w = 4; w > 0; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+    most = __shfl_sync(0xffffffffu, most, 0);
+    const float u = most == -INFINITY ? 0.f : most, f = exp2_sfu(m - u);
+    const float mine = exp2_sfu(top.x - u);
+    m = most;
+    l *= f;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) sum[k] *= f;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float g = __shfl_sync(0xffffffffu, mine, i);
+      const float z = __shfl_sync(0xffffffffu, top.y, i);
+      if (i < n) {
+        l += g * z;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+          sum[2 * k] += g * v[i][k].x;
+          sum[2 * k + 1] += g * v[i][k].y;
+        }
       }
     }
-    write_row<T, D>(a, b, node, kvh * deal.group + (row0 + r) % deal.group, lane, m, l, sum);
   }
+  write_row<T, D>(a, b, node, kvh * deal.group + row % deal.group, lane, m, l, sum);
 }
 
 // ---------------------------------------------------------------- host
@@ -446,8 +463,21 @@ bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int64_t n2
     if (n[i] > 1 && (strides[i] <= 0 || strides[i] >= (1ll << 39))) return false;
   return true;
 }
+// Which kernel is the faster, by the bytes of a full cache (the lengths are on the device). The
+// narrow kernel starts and ends an item in about 2 us where the wide one takes 8 to 10, and
+// reads the cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.4. Measured,
+// wide against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 21.6 / 11.6,
+// 64 of 500 to 1000 (197 MB) 98.7 / 54.5; 4 rows, 8 heads of 128, 64 of 1000 to 2000 (525 MB)
+// 101 / 105, 16 of 2500 to 16001 (1.1 GB) 112 / 134; 64 rows, 12 heads of 64, 2 sequences (6.5 MB)
+// 27.9 / 25.6, 4 (13 MB) 31.3 / 32.0, 64 (209 MB) 183 / 247.
+bool narrow_faster(const Args& a) {
+  const int64_t rows = a.nodes * (a.heads / a.kv_heads), item = a.capacity * a.head_dim * 4;
+  const int64_t cache = a.batch * a.kv_heads * item;
+  if (rows <= kRows) return item < (1 << 20) || cache < (256 << 20);
+  return rows <= 4 * kRows && cache * ((rows + kRows - 1) / kRows) < (40 << 20);
+}
 bool wide_takes(const Args& a) {
-  return wide_fits(a) && a.scale > 0 && strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
+  return wide_fits(a) && !narrow_faster(a) && a.scale > 0 && strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
          strides_fit(a.k_new_strides, a.batch, a.nodes, a.kv_heads) &&
          strides_fit(a.v_new_strides, a.batch, a.nodes, a.kv_heads) &&
          strides_fit(a.keys_strides, a.batch, a.kv_heads, a.capacity) &&
@@ -462,7 +492,7 @@ Plan plan_for(const Args& a, bool wide, int sm_count) {
   p.deal.least = 2;
   if (wide) {
     p.rows = ppyb200::tree::wide_rows(a);
-    p.deal.streams = p.rows.share ? 1 : 2;
+    p.deal.streams = p.rows.share ? 1 : 2 * p.rows.copies;
     p.deal.item_rows = (int)(p.rows.tile_nodes * group * (p.rows.share ? 2 : 1));
     p.deal.grid = sm_count;
   } else {
@@ -477,7 +507,7 @@ Plan plan_for(const Args& a, bool wide, int sm_count) {
                        ((a.capacity + tile - 1) / tile + (wide ? (a.nodes + tile - 1) / tile : 0));
   const int64_t most = work / p.deal.least;
   if (p.deal.grid > most) p.deal.grid = most < 1 ? 1 : (int)most;
-  p.join = p.deal.streams == 2 || p.deal.grid > 1;
+  p.join = p.deal.streams > 1 || p.deal.grid > 1;
   p.workspace = p.join ? Results::bytes(a, p.deal, padded_dim(a.head_dim)) : 0;
   return p;
 }
@@ -486,7 +516,7 @@ template <class T, int D>
 cudaError_t join(const Args& a, const Plan& p, cudaStream_t stream) {
   const dim3 grid((unsigned)(a.kv_heads * a.batch * p.deal.items),
                   (unsigned)((p.deal.item_rows + kJoinRows - 1) / kJoinRows));
-  return ppyb200::launch_pdl(join_kernel<T, D>, grid, dim3(128), 0, stream, a, p.deal);
+  return ppyb200::launch_pdl(join_kernel<T, D>, grid, dim3(32 * kJoinRows), 0, stream, a, p.deal);
 }
 
 template <class T, int D>
@@ -506,8 +536,11 @@ cudaError_t launch_narrow(const Args& a, const Plan& p, cudaStream_t stream) {
 
 template <class T, int D>
 cudaError_t launch_dim(const Args& a, const Plan& p, cudaStream_t stream) {
-  const cudaError_t e = p.wide ? ppyb200::tree::launch_wide<T, D>(a, p.deal, p.rows, stream)
-                               : launch_narrow<T, D>(a, p, stream);
+  using ppyb200::tree::launch_wide;
+  const cudaError_t e = !p.wide ? launch_narrow<T, D>(a, p, stream)
+                        : p.rows.copies == 4 ? launch_wide<T, D, 4>(a, p.deal, p.rows, stream)
+                        : p.rows.copies == 2 ? launch_wide<T, D, 2>(a, p.deal, p.rows, stream)
+                                             : launch_wide<T, D, 1>(a, p.deal, p.rows, stream);
   return e == cudaSuccess && p.join ? join<T, D>(a, p, stream) : e;
 }
 

@@ -34,15 +34,15 @@ __device__ __forceinline__ void sequence_extent(const Args& a, int b, int& lengt
 // axis of tiles, and CTA c of G takes the tiles [c W / G, (c + 1) W / G) of it: equal shares
 // whatever the lengths are, walked as segments of one item each. At most the first and the last
 // segment of a CTA are less than an item; those leave their unnormalised results in the workspace
-// for the join, a whole item is written out by its CTA. Where a CTA's two streams split an
-// item's keys, every segment leaves two results.
+// for the join, a whole item is written out by its CTA. Where a CTA's streams split an
+// item's keys, every segment leaves several results.
 struct Deal {
   int grid;       // CTAs at most; fewer when each would have less than `least` tiles
   int least;
   int items;      // items a sequence and key head
   int item_rows;
   int group;      // query heads a key head
-  int streams;    // 2 where a CTA's two streams split an item's keys, else 1
+  int streams;    // results a segment leaves: several where streams or copies split its keys
 };
 
 struct Segment {
@@ -108,7 +108,8 @@ struct Walk {
   // item's number on the axis tells all segments apart.
   __device__ __forceinline__ static int64_t result_of(const Deal& deal, int c, int number,
                                                       bool starts) {
-    return deal.streams == 1 ? 2 * (int64_t)c + (starts ? 1 : 0) : 2 * ((int64_t)c + number);
+    return deal.streams == 1 ? 2 * (int64_t)c + (starts ? 1 : 0)
+                             : deal.streams * ((int64_t)c + number);
   }
   // To the start of CTA c's share (a warp together).
   __device__ __forceinline__ void enter(const Args& a, const Deal& deal, int c) {
@@ -224,7 +225,8 @@ struct Results {
   int2* ctas;
   int item_rows;
   __host__ __device__ __forceinline__ static int64_t count(const Args& a, const Deal& deal) {
-    return 2 * (deal.grid + (deal.streams == 1 ? 0 : a.kv_heads * a.batch * deal.items));
+    return deal.streams == 1 ? 2 * (int64_t)deal.grid
+                             : deal.streams * (deal.grid + a.kv_heads * a.batch * deal.items);
   }
   __device__ __forceinline__ Results(const Args& a, const Deal& deal, int dim)
       : item_rows(deal.item_rows) {

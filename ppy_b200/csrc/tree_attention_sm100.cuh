@@ -5,9 +5,11 @@
 // then the nodes' own) of one sequence and key head, with two streams, each a query tile of 128 rows with its own softmax warpgroup and
 // MMA issuer, so that one stream's products run while the other's softmax does:
 //   rows > 128   the streams hold two row tiles and share every key tile (read once for 256 rows)
-//   rows <= 128  the streams hold the same rows and take the key tiles in turn, two results
-//   rows <= 64   as before, the second stream's rows in lanes 64-127: the four warps with rows sit
-//                on four SM sub-partitions instead of two
+//   rows <= 128  the streams hold the same rows and take the key tiles in turn
+//   rows <= 64   the same, and a query tile holds its rows twice (four times up to 32 rows): each
+//                copy weighs a half (a quarter) of a tile's keys, with zeros for the others, so
+//                that all eight softmax warps have rows and each less to do
+// Streams that split an item's keys, and copies, leave results of their own for the join.
 // Per key tile and stream:
 //   S = Q K^T   M = 128, N = 128, both operands K-major with the 128-byte swizzle; the query rows
 //               of a tile come as one box [nodes][heads of the group][64 columns]
@@ -133,9 +135,9 @@ struct WideMaps {
 };
 
 struct WideRows {
-  int tile_nodes;  // nodes of a row tile (tile_nodes x group <= 128, or <= 64 when half)
+  int tile_nodes;  // nodes of a row tile (tile_nodes x group <= 128 / copies)
   bool share;      // two row tiles an item, sharing the key tiles; else two streams over the keys
-  bool half;       // not share, at most 64 rows: stream 1's rows in lanes 64-127
+  int copies;      // of the rows in a query tile (1 when shared)
 };
 
 template <class Layout>
@@ -227,11 +229,12 @@ __device__ __forceinline__ Sight node_sight(const uint8_t* parents, int node, in
   }
 }
 
-template <class T, int D>
+template <class T, int D, int COPIES>
 __global__ void __launch_bounds__(kWideThreads, 1)
 wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args a,
             const Deal deal, const WideRows wide) {
   using Shape = WideShape<D>;
+  constexpr int kSpan = 128 / COPIES;  // rows of a copy, and keys of a tile that it weighs
   extern __shared__ uint8_t smem_raw[];
   WideShared<D>& s = *reinterpret_cast<WideShared<D>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -292,7 +295,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     // ---- loader: lane 0 loads a segment's Q, then K and V of its tiles (K of the CTA's i-th tile
     // is entry 2 i of the ring, its V entry 2 i + 1); the warp together leaves a tree's parents in
     // shared memory before the first node tile
-    const uint32_t q_bytes = (uint32_t)(Shape::kBoxes * wide.tile_nodes * group * 128);
+    const uint32_t q_bytes = (uint32_t)(COPIES * Shape::kBoxes * wide.tile_nodes * group * 128);
     int loaded[2] = {0, 0}, segments = 0;  // entries of each stream (of both, when they share)
     bool ok = true;
     for (; ok && walk.next(a, deal, seg); ++segments) {
@@ -312,10 +315,10 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           const int node0 = seg.row0 / group;
           mbar_expect_tx(&s.q_full, streams * q_bytes);
           for (int t = 0; t < streams; ++t)
-            for (int x = 0; x < Shape::kBoxes; ++x)
-              tma_load_4d(s.q[t] + x * kBox + (wide.half && t == 1 ? kBox / 2 : 0), &maps.q,
-                          &s.q_full, x * 64, seg.kvh * group,
-                          node0 + (wide.share ? t * wide.tile_nodes : 0), seg.b);
+            for (int x = 0; x < Shape::kBoxes * COPIES; ++x)
+              tma_load_4d(s.q[t] + x * (kBox / COPIES), &maps.q, &s.q_full, x / COPIES * 64,
+                          seg.kvh * group, node0 + (wide.share ? t * wide.tile_nodes : 0),
+                          seg.b);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -461,7 +464,8 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     // ---- softmax: warpgroup t, thread = row (a TMEM lane) and, when cleaning, a key
     const int t = warp >> 2;
     const int lane_row = (warp & 3) * 32 + lane;
-    const int row = lane_row - (wide.half && t == 1 ? 64 : 0);  // of the row tile
+    const int row = lane_row % kSpan;                   // of the row tile
+    const int key0 = (warp & 3) * 32 / kSpan * kSpan;  // first of the tile's keys that it weighs
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + (uint32_t)(t * kKeysTile);
     const uint32_t o_addr = tmem + lane_addr + Shape::kOCol + (uint32_t)(t * D);
@@ -469,6 +473,13 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     const float scale_log2 = (float)a.scale * mma16::kLog2e;
     const uint64_t scale2 = f2(scale_log2, scale_log2);
     const Results results(a, deal, D);
+    if (COPIES > 1 && !Shape::kOver) {
+      // the weights of the keys that other copies weigh: zero throughout
+      const uint32_t zeros[16] = {};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_st16(p_addr + (uint32_t)(q * 16), zeros);
+      tmem_wait_st();
+    }
     int base = 0, n = 0;  // as the MMA issuer's
     int mark = 1;             // this segment's, in `spoiled`
     int turn = 0;         // tiles of shared segments so far
@@ -479,7 +490,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       const int cache_tiles = cache_tiles_of(seg);
       const int tile_row = (wide.share ? t * wide.tile_nodes * group : 0) + row;  // of the item
       const int node = (seg.row0 + tile_row) / group;
-      const bool real = row >= 0 && row < wide.tile_nodes * group && node < seg.count;
+      const bool real = row < wide.tile_nodes * group && node < seg.count;
       const bool busy = __any_sync(0xffffffffu, real) != 0;  // the warp has rows
       // the loader's, there before the first node tile's keys
       const uint8_t* parents =
@@ -499,10 +510,10 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         const int left = own ? 0 : seg.length - tile * kKeysTile;
         const bool ragged = own || left < kKeysTile;
         if (busy) {
-          float sv[kKeysTile];
+          float sv[kSpan];
 #pragma unroll
-          for (int c = 0; c < kKeysTile / 32; ++c)
-            tmem_ld32_nowait(s_addr + (uint32_t)(c * 32), sv + c * 32);
+          for (int c = 0; c < kSpan / 32; ++c)
+            tmem_ld32_nowait(s_addr + (uint32_t)(key0 + c * 32), sv + c * 32);
           tmem_wait_ld();
           if (!Shape::kOver) {
             tc_fence_before();
@@ -515,14 +526,15 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
                      : real ? node_sight(parents, node, (tile - cache_tiles) * kKeysTile,
                                          seg.count)
                             : Sight::first(0);
+            const uint64_t low = key0 < 64 ? sees.lo >> key0 : sees.hi >> (key0 - 64);
 #pragma unroll
-            for (int c = 0; c < kKeysTile; ++c)
-              if ((((c < 64 ? sees.lo : sees.hi) >> (c & 63)) & 1ull) == 0) sv[c] = -INFINITY;
+            for (int c = 0; c < kSpan; ++c)
+              if ((((c < 64 ? low : sees.hi) >> (c & 63)) & 1ull) == 0) sv[c] = -INFINITY;
             __syncwarp();  // the walks differ; tensor memory is accessed by whole warps
           }
           float mx[4] = {m, m, m, m};
 #pragma unroll
-          for (int c = 0; c < kKeysTile; c += 8) {
+          for (int c = 0; c < kSpan; c += 8) {
             mx[0] = max3(mx[0], sv[c + 0], sv[c + 1]);
             mx[1] = max3(mx[1], sv[c + 2], sv[c + 3]);
             mx[2] = max3(mx[2], sv[c + 4], sv[c + 5]);
@@ -559,7 +571,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           }
           uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int quarter = 0; quarter < 4; ++quarter) {
+          for (int quarter = 0; quarter < kSpan / 32; ++quarter) {
             uint32_t pk[16];
 #pragma unroll
             for (int c = quarter * 32; c < quarter * 32 + 32; c += 2) {
@@ -569,7 +581,14 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
               sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], f2(e0, e1));
               pk[(c >> 1) & 15] = Kind<T>::pack(e0, e1);
             }
-            tmem_st16(p_addr + (uint32_t)(quarter * 16), pk);
+            tmem_st16(p_addr + (uint32_t)(key0 / 2 + quarter * 16), pk);
+          }
+          if (COPIES > 1 && Shape::kOver) {
+            // P lies over S: zeros over the scores that other copies weigh
+            const uint32_t zeros[16] = {};
+#pragma unroll
+            for (int quarter = kSpan / 32; quarter < 4; ++quarter)
+              tmem_st16(p_addr + (uint32_t)((key0 / 2 + quarter * 16) % 64), zeros);
           }
           if (turns) {
             __syncwarp();
@@ -657,7 +676,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       }
       if (ok && busy) {
         const bool spoiled = mine > 0 && *(volatile int*)&s.spoiled[mark & 7] == mark;
-        const int64_t at = results.at(seg.result + (deal.streams == 2 ? t : 0), tile_row);
+        const int64_t at = results.at(seg.result + (wide.share ? 0 : t * COPIES + key0 / kSpan), tile_row);
         const int head = seg.kvh * group + tile_row % group;
         const float inv = 1.f / l;
         T* out = static_cast<T*>(a.out) + seg.b * a.out_strides[0] + node * a.out_strides[1] +
@@ -680,7 +699,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
               if (tile < 0) continue;
               const int n0 = tile * kKeysTile;
               const Sight sees = node_sight(parents, node, n0, seg.count);
-              for (int key = 0; key < kKeysTile && n0 + key < seg.count; ++key) {
+              for (int key = key0; key < key0 + kSpan && n0 + key < seg.count; ++key) {
                 if (!sees.has(key)) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
@@ -762,14 +781,14 @@ inline bool wide_map(CUtensorMap* map, const void* base, bool bf16, int64_t colu
 inline WideRows wide_rows(const Args& a) {
   WideRows w;
   const int group = (int)(a.heads / a.kv_heads);
-  w.half = a.nodes <= 64 / group;
-  w.tile_nodes = w.half ? 64 / group : kRowsTile / group;
+  w.copies = a.nodes <= 32 / group ? 4 : a.nodes <= 64 / group ? 2 : 1;
+  w.tile_nodes = kRowsTile / w.copies / group;
   w.share = w.tile_nodes > 0 && a.nodes > w.tile_nodes;
   if (w.tile_nodes > a.nodes) w.tile_nodes = (int)a.nodes;
   return w;
 }
 
-template <class T, int D>
+template <class T, int D, int COPIES>
 inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& w,
                                cudaStream_t stream) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -788,7 +807,7 @@ inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& 
     return cudaErrorInvalidValue;
   static DeviceOnce once;
   constexpr int smem = (int)sizeof(WideShared<D>) + 1024;
-  auto kernel = wide_kernel<T, D>;
+  auto kernel = wide_kernel<T, D, COPIES>;
   int ready = 0;
   const cudaError_t e = once.get(
       [&](int* value) {
