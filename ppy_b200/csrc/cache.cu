@@ -18,6 +18,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <cooperative_groups.h>
+
 #include "../../include/ppyb200.h"
 #include "mma16.cuh"
 #include "ppyb200_device.cuh"
@@ -242,7 +244,9 @@ cudaError_t launch_accept(const ppyb200_accept_args& a, cudaStream_t stream) {
 
 // ---------------------------------------------------------------- evict
 
-constexpr int kSelectThreads = 512;
+constexpr int kSelectThreads = 256;
+constexpr int kBins = 2048;           // of a digit of a rank
+constexpr int kCachedRanks = 16384;   // ranks a CTA keeps in shared memory
 constexpr int kMoveRows = 32;  // rows a CTA moves
 
 // An entry's rank as an unsigned number: protected entries above every weight, weights in
@@ -254,49 +258,83 @@ __device__ __forceinline__ uint32_t entry_key(float w, int32_t position, int64_t
   return (bits >> 31) != 0 ? ~bits : bits | 0x80000000u;
 }
 
-// Exclusive prefix sums over the block of two counts a thread (packed 16 + 16 bits; a chunk
-// holds fewer than 65536 entries), and their totals.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t* totals,
-                                                 uint32_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t run = mine;
+// Adds one to each lane's bin; lanes that share the first lane's bin (entries that never gathered
+// any weight fall into one) add once for all.
+__device__ __forceinline__ void count_bins(uint32_t* bins, uint32_t bin, bool valid) {
+  const uint32_t first = __shfl_sync(0xffffffffu, bin, 0);
+  const unsigned same = __ballot_sync(0xffffffffu, valid && bin == first);
+  if (valid && bin == first) {
+    if ((threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&bins[first], __popc(same));
+  } else if (valid) {
+    atomicAdd(&bins[bin], 1u);
+  }
+}
+
+// Exclusive prefix sums of 32 kPer numbers in shared memory, by one warp; returns their sum.
+template <int kPer>
+__device__ __forceinline__ uint32_t warp_prefix(uint32_t* numbers) {
+  const int lane = threadIdx.x & 31;
+  uint32_t mine[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    mine[i] = numbers[lane * kPer + i];
+    sum += mine[i];
+  }
+  uint32_t run = sum;
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
     const uint32_t up = __shfl_up_sync(0xffffffffu, run, w);
     if (lane >= w) run += up;
   }
-  __syncthreads();  // the last call's totals have been read
-  if (lane == 31) totals[warp] = run;
-  __syncthreads();
-  uint32_t before = 0;
-  total = 0;
+  uint32_t before = run - sum;
 #pragma unroll
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    const uint32_t t = totals[w];
-    if (w < warp) before += t;
-    total += t;
+  for (int i = 0; i < kPer; ++i) {
+    numbers[lane * kPer + i] = before;
+    before += mine[i];
   }
-  return before + run - mine;
+  return __shfl_sync(0xffffffffu, run, 31);
 }
 
-// One CTA a key head: finds the budget-th rank with four 8-bit histograms, then walks the
-// entries in slot order, writes the tables of those that stay and lists holes and sources.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const ppyb200_evict_args a,
-                                                                     const int64_t most) {
-  __shared__ uint32_t bins[256];
-  __shared__ uint32_t totals[kSelectThreads / 32];
-  __shared__ uint32_t picked, rest;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kWalkRows = 8;  // rows of kSelectThreads entries that the walk takes at once
+constexpr int kWalkParts = kWalkRows * kSelectWarps;
+
+struct SelectShared {
+  alignas(16) uint32_t bins[2][kBins];  // of a digit, read by the whole cluster
+  uint32_t sums[kSelectWarps];
+  uint32_t equal[kWalkParts], holes[kWalkParts], sources[kWalkParts];  // by row and warp
+  uint32_t all[3];     // of the rows together
+  uint32_t counts[4];  // entries above / equal to the threshold, before / behind the budget
+  uint32_t slice;      // entries in this CTA's slice of the bins
+  uint32_t picked, rest;
+};
+
+// A cluster a key head; each CTA takes a stretch of its entries and keeps their ranks in shared
+// memory where they fit (`cached` of them). The budget-th rank is found digit by digit (11, 11
+// and 10 bits): every CTA counts its own entries, adds up a slice of the bins over the cluster from
+// the others' shared memory, and reads the slice that holds the digit. Then each walks its entries in slot order, writes the tables of those that stay in
+// front of the budget, and lists holes and sources; the lists filled, the holes' tables follow.
+// Loops stay rolled: a kernel of some microseconds waits for each line of its code once.
+__global__ void __launch_bounds__(kSelectThreads, 4) evict_select_kernel(const ppyb200_evict_args a,
+                                                                     const int64_t most,
+                                                                     const int cached) {
+  namespace cg = cooperative_groups;
+  extern __shared__ uint32_t keys[];
+  __shared__ SelectShared s;
   ppyb200::pdl_wait();
-  const int tid = threadIdx.x;
-  const int64_t head = blockIdx.x;
-  const int h = (int)(head % a.kv_heads), b = (int)(head / a.kv_heads % a.batch);
-  const int layer = (int)(head / a.kv_heads / a.batch);
-  int64_t length = a.lengths[b];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int head = (int)blockIdx.x / ranks, kv_heads = (int)a.kv_heads, batch = (int)a.batch;
+  const int row = head / kv_heads, h = head - row * kv_heads;
+  const int layer = row / batch, b = row - layer * batch;
+  int length = a.lengths[b];
   if (length < 0 || length > a.capacity) {
     if (layer == 0 && h == 0 && tid == 0) raise(a.status);
-    length = length < 0 ? 0 : a.capacity;
+    length = length < 0 ? 0 : (int)a.capacity;
   }
-  const int64_t budget = a.budget, protect_from = (int64_t)a.seen[b] - a.recent;
+  const int budget = (int)a.budget;
+  const int64_t protect_from = (int64_t)a.seen[b] - a.recent;
   const int64_t at = layer * a.weights_strides[0] + b * a.weights_strides[1] +
                      h * a.weights_strides[2];
   const int64_t out_at = layer * a.out_strides[0] + b * a.out_strides[1] + h * a.out_strides[2];
@@ -304,13 +342,18 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const ppyb
   const int32_t* positions = a.positions + at;
   float* weights_out = a.weights_out + out_at;
   int32_t* positions_out = a.positions_out + out_at;
-  int32_t* kept = a.kept + head * budget;
+  int32_t* kept = a.kept + (int64_t)head * budget;
   int32_t* moves = static_cast<int32_t*>(a.workspace);  // counts, then holes and sources
   int32_t* holes = moves + a.layers * a.batch * a.kv_heads + head * 2 * most;
   int32_t* sources = holes + most;
+  const int step = kSelectThreads * ranks, first_thread = rank * kSelectThreads + tid;
+  auto sync_all = [&] {
+    if (ranks == 1) __syncthreads();
+    else cluster.sync();
+  };
 
   if (length <= budget) {  // nothing to evict
-    for (int64_t j = tid; j < budget; j += kSelectThreads) {
+    for (int64_t j = first_thread; j < budget; j += step) {
       kept[j] = j < length ? (int32_t)j : -1;
       if (j < length) {
         const float w = weights[j];
@@ -319,102 +362,271 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const ppyb
         positions_out[j] = p;
       }
     }
-    if (tid == 0) moves[head] = 0;
-    return;
+    if (rank == 0 && tid == 0) moves[head] = 0;
+    return;  // the whole cluster
   }
 
-  // the budget-th largest key, eight bits at a time from the top
+  const int stretch = (length + ranks - 1) / ranks;
+  const int begin = min(rank * stretch, length), end = min(begin + stretch, length);
+  const int in_cache = min(end - begin, cached);
+  auto key_of = [&](int j) {
+    return j - begin < in_cache ? keys[j - begin]
+                                : entry_key(weights[j], positions[j], protect_from);
+  };
+  if (tid < 4) s.counts[tid] = 0;
+
   uint32_t prefix = 0;
-  int64_t need = budget;  // entries to take among those that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) bins[i] = 0;
+  uint32_t need = (uint32_t)budget;  // entries to take among those that share the prefix
+#pragma unroll 1
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+    const int bins = digit == 2 ? kBins / 2 : kBins;
+    const uint32_t known = ~0u << (digit == 1 ? 21 : 10);
+    // The third digit has the first's memory: every CTA had read it before the second's barrier.
+    uint32_t* mine = s.bins[digit & 1];
+#pragma unroll 1
+    for (int i = tid; i < kBins / 4; i += kSelectThreads)
+      reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int64_t j = tid; j < length; j += kSelectThreads) {
-      const uint32_t key = entry_key(weights[j], positions[j], protect_from);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&bins[(key >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (tid < 32) {  // lane l: bins 255 - 8 l down to 248 - 8 l
-      uint32_t mine = 0;
+    if (digit == 0) {
+#pragma unroll 1
+      for (int j0 = begin; j0 < end; j0 += 8 * kSelectThreads) {
+        float w[8];
+        int32_t p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += bins[255 - 8 * tid - i];
-      uint32_t run = mine;
+        for (int u = 0; u < 8; ++u) {  // all loads first
+          const int j = j0 + u * kSelectThreads + tid;
+          w[u] = j < end ? weights[j] : 0.f;
+          p[u] = j < end ? positions[j] : 0;
+        }
 #pragma unroll
-      for (int w = 1; w < 32; w <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, run, w);
-        if (tid >= w) run += up;
-      }
-      uint32_t above = run - mine;
-      if ((int64_t)above < need && need <= (int64_t)run) {
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t c = bins[255 - 8 * tid - i];
-          if ((int64_t)(above + c) >= need) {
-            picked = (uint32_t)(255 - 8 * tid - i);
-            rest = (uint32_t)(need - above);
-            break;
-          }
-          above += c;
+        for (int u = 0; u < 8; ++u) {
+          const int j = j0 + u * kSelectThreads + tid;
+          const uint32_t key = entry_key(w[u], p[u], protect_from);
+          if (j < end && j - begin < in_cache) keys[j - begin] = key;
+          count_bins(mine, key >> 21, j < end);
         }
       }
+    } else {
+#pragma unroll 2
+      for (int j0 = begin; j0 < end; j0 += kSelectThreads) {
+        const int j = j0 + tid;
+        const uint32_t key = j < end ? key_of(j) : 0u;
+        const bool counts = j < end && ((key ^ prefix) & known) == 0;
+        if (__any_sync(0xffffffffu, counts))
+          count_bins(mine, (key >> shift) & (uint32_t)(bins - 1), counts);
+      }
+    }
+    sync_all();
+    const int slice = bins / ranks;
+    if (ranks > 1) {
+      uint32_t sum = 0;
+#pragma unroll 1
+      for (int i = rank * slice + tid; i < (rank + 1) * slice; i += kSelectThreads) {
+        uint32_t c = 0;
+#pragma unroll 1
+        for (int q = 0; q < ranks; ++q) c += cluster.map_shared_rank(mine, q)[i];
+        mine[i] = c;  // no other CTA reads this slice of this CTA's before the next barrier
+        sum += c;
+      }
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      if (lane == 0) s.sums[warp] = sum;
+      __syncthreads();
+      if (tid == 0) {
+        uint32_t all = 0;
+        for (int w = 0; w < kSelectWarps; ++w) all += s.sums[w];
+        s.slice = all;
+      }
+      cluster.sync();
+    }
+    // the slice that holds the need-th entry from the top, then its bins from the top
+    uint32_t above = 0;
+    int owner = ranks - 1;
+#pragma unroll 1
+    for (; ranks > 1 && owner > 0; --owner) {
+      const uint32_t all = *cluster.map_shared_rank(&s.slice, owner);
+      if (above + all >= need) break;
+      above += all;
+    }
+    const uint32_t* from = cluster.map_shared_rank(mine, owner) + owner * slice;
+    const int each = (slice + kSelectThreads - 1) / kSelectThreads;
+    const int top = slice - 1 - tid * each;  // this thread's highest bin of the slice
+    uint32_t sum = 0;
+#pragma unroll 1
+    for (int i = 0; i < each; ++i) sum += top - i >= 0 ? from[top - i] : 0u;
+    uint32_t run = sum;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, run, w);
+      if (lane >= w) run += up;
+    }
+    if (lane == 31) s.sums[warp] = run;
+    __syncthreads();
+    above += run - sum;
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) above += w < warp ? s.sums[w] : 0u;
+    if (above < need && need <= above + sum) {  // one thread
+#pragma unroll 1
+      for (int i = 0; i < each; ++i) {
+        const uint32_t c = from[top - i];
+        if (need <= above + c) {
+          s.picked = (uint32_t)(owner * slice + top - i);
+          s.rest = need - above;
+          break;
+        }
+        above += c;
+      }
     }
     __syncthreads();
-    prefix |= picked << shift;
-    need = rest;
-    __syncthreads();
+    prefix |= s.picked << shift;
+    need = s.rest;
   }
-  const uint32_t threshold = prefix;  // take every larger key and the first `need` equal ones
+  const uint32_t threshold = prefix;  // take every larger rank and the first `need` equal ones
 
-  constexpr int kItems = 4;
-  int64_t equal_before = 0, hole_count = 0, source_count = 0;
-  for (int64_t j0 = 0; j0 < length; j0 += kSelectThreads * kItems) {
-    const int64_t first = j0 + tid * kItems;
-    uint32_t key[kItems];
-    uint32_t equal = 0;
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int64_t j = first + i;
-      key[i] = j < length ? entry_key(weights[j], positions[j], protect_from) : 0u;
-      if (j < length && key[i] == threshold) ++equal;
+  {  // entries of this stretch above and equal to the threshold, before and behind the budget
+    uint32_t more[4] = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int j = begin + tid; j < end; j += kSelectThreads) {
+      const uint32_t key = key_of(j);
+      const bool above = key > threshold, same = key == threshold;
+      more[0] += above && j < budget ? 1 : 0;
+      more[1] += above && j >= budget ? 1 : 0;
+      more[2] += same && j < budget ? 1 : 0;
+      more[3] += same && j >= budget ? 1 : 0;
     }
-    uint32_t total;
-    int64_t order = equal_before + block_prefix(equal, totals, total);
-    equal_before += total;
-    bool keep[kItems];
-    uint32_t moving = 0;  // holes low, sources high
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int64_t j = first + i;
-      keep[i] = j < length && key[i] > threshold;
-      if (j < length && key[i] == threshold) keep[i] = order++ < need;
-      if (j < budget && !keep[i]) moving += 1;
-      if (j >= budget && keep[i]) moving += 1u << 16;
-    }
-    const uint32_t rank = block_prefix(moving, totals, total);
-    int64_t hole = hole_count + (rank & 0xffffu), source = source_count + (rank >> 16);
-    hole_count += total & 0xffffu;
-    source_count += total >> 16;
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int64_t j = first + i;
-      if (j < budget) {
-        if (keep[i]) {
-          kept[j] = (int32_t)j;
-          const float w = weights[j];
-          const int32_t p = positions[j];
-          weights_out[j] = w;
-          positions_out[j] = p;
-        } else {
-          holes[hole++] = (int32_t)j;
-        }
-      } else if (keep[i]) {
-        sources[source++] = (int32_t)j;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t sum = __reduce_add_sync(0xffffffffu, more[i]);
+      if (lane == 0 && sum != 0) atomicAdd(&s.counts[i], sum);
     }
   }
-  if (tid == 0) moves[head] = (int32_t)hole_count;
-  __syncthreads();  // the lists are complete
-  for (int64_t r = tid; r < hole_count; r += kSelectThreads) {
+  sync_all();
+  // holes and sources of the earlier CTAs' stretches, and all of them; equal entries are taken in
+  // slot order, so early stretches and early entries first
+  uint32_t hole_count = 0, source_count = 0, all_holes = 0, equal_before = 0;
+  uint32_t left = need, own_left = 0, own_equal = 0;
+#pragma unroll 1
+  for (int q = 0; q < ranks; ++q) {
+    const uint32_t* other = cluster.map_shared_rank(s.counts, q);
+    const uint32_t equal = other[2] + other[3];
+    const uint32_t taken = min(left, equal), early = min(taken, other[2]);
+    const int from = min(q * stretch, length), to = min(from + stretch, length);
+    const uint32_t gone = (uint32_t)(min(to, max(from, budget)) - from) - other[0] - early;
+    if (q < rank) {
+      hole_count += gone;
+      source_count += other[1] + taken - early;
+      equal_before += equal;
+    }
+    if (q == rank) {
+      own_left = taken;
+      own_equal = equal;
+    }
+    all_holes += gone;
+    left -= taken;
+  }
+  // in most stretches all equal entries stay or all go, and their order does not matter
+  const bool ordered = own_left != 0 && own_left != own_equal;
+
+  // Rows of kSelectThreads entries, eight at once: a warp's votes give an entry's place within
+  // its row and warp, the prefix sums over rows and warps the rest.
+  const unsigned below = (1u << lane) - 1u;
+#pragma unroll 1
+  for (int j0 = begin; j0 < end; j0 += kWalkRows * kSelectThreads) {
+    uint32_t key[kWalkRows];
+    float w[kWalkRows];
+    int32_t p[kWalkRows];
+    const bool front = j0 < budget, back = min(j0 + kWalkRows * kSelectThreads, end) > budget;
+#pragma unroll
+    for (int i = 0; i < kWalkRows; ++i) {
+      const int j = j0 + i * kSelectThreads + tid;
+      key[i] = j < end ? key_of(j) : 0u;
+      if (front && j < end && j < budget) {  // under way while the places are found
+        w[i] = weights[j];
+        p[i] = positions[j];
+      }
+    }
+    uint32_t keep = 0;  // a bit a row
+    if (ordered) {
+#pragma unroll
+      for (int i = 0; i < kWalkRows; ++i) {
+        const bool same = j0 + i * kSelectThreads + tid < end && key[i] == threshold;
+        const unsigned votes = __ballot_sync(0xffffffffu, same);
+        if (lane == 0) s.equal[i * kSelectWarps + warp] = __popc(votes);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const uint32_t all = warp_prefix<kWalkParts / 32>(s.equal);
+        if (lane == 0) s.all[0] = all;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kWalkRows; ++i) {
+        const int j = j0 + i * kSelectThreads + tid;
+        const bool same = j < end && key[i] == threshold;
+        const unsigned votes = __ballot_sync(0xffffffffu, same);
+        const uint32_t order =
+            equal_before + s.equal[i * kSelectWarps + warp] + __popc(votes & below);
+        if (j < end && (key[i] > threshold || (same && order < need))) keep |= 1u << i;
+      }
+      equal_before += s.all[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWalkRows; ++i)
+        if (j0 + i * kSelectThreads + tid < end &&
+            (key[i] > threshold || (key[i] == threshold && own_left != 0)))
+          keep |= 1u << i;
+    }
+#pragma unroll
+    for (int i = 0; i < kWalkRows; ++i) {
+      const int j = j0 + i * kSelectThreads + tid;
+      const bool stays = ((keep >> i) & 1u) != 0;
+      if (front) {
+        const unsigned gone = __ballot_sync(0xffffffffu, j < end && j < budget && !stays);
+        if (lane == 0) s.holes[i * kSelectWarps + warp] = __popc(gone);
+      }
+      if (back) {
+        const unsigned late = __ballot_sync(0xffffffffu, j >= budget && stays);
+        if (lane == 0) s.sources[i * kSelectWarps + warp] = __popc(late);
+      }
+    }
+    __syncthreads();
+    if (warp == 0 && front) {
+      const uint32_t all = warp_prefix<kWalkParts / 32>(s.holes);
+      if (lane == 0) s.all[1] = all;
+    }
+    if (warp == 1 && back) {
+      const uint32_t all = warp_prefix<kWalkParts / 32>(s.sources);
+      if (lane == 0) s.all[2] = all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWalkRows; ++i) {
+      const int j = j0 + i * kSelectThreads + tid;
+      const bool stays = ((keep >> i) & 1u) != 0;
+      if (front) {
+        const unsigned gone = __ballot_sync(0xffffffffu, j < end && j < budget && !stays);
+        if (j < end && j < budget) {
+          if (stays) {
+            kept[j] = j;
+            weights_out[j] = w[i];
+            positions_out[j] = p[i];
+          } else {
+            holes[hole_count + s.holes[i * kSelectWarps + warp] + __popc(gone & below)] = j;
+          }
+        }
+      }
+      if (back) {
+        const unsigned late = __ballot_sync(0xffffffffu, j >= budget && stays);
+        if (j >= budget && stays)
+          sources[source_count + s.sources[i * kSelectWarps + warp] + __popc(late & below)] = j;
+      }
+    }
+    if (front) hole_count += s.all[1];
+    if (back) source_count += s.all[2];
+  }
+  if (rank == 0 && tid == 0) moves[head] = (int32_t)all_holes;
+  sync_all();  // the lists are complete, and no CTA reads another's shared memory any more
+  for (uint32_t r = first_thread; r < all_holes; r += step) {
     const int32_t to = holes[r], from = sources[r];
     kept[to] = from;
     weights_out[to] = weights[from];
@@ -463,6 +675,41 @@ bool rows16(const void* p, const int64_t* strides, int count) {
 int64_t most_moves(const ppyb200_evict_args& a) {
   const int64_t behind = a.capacity - a.budget;
   return behind <= 0 ? 0 : behind < a.budget ? behind : a.budget;
+}
+
+// Clusters of the select kernel: two CTAs more for each head (up to eight) while the SMs have room
+// for four of each and a stretch stays above 2048 entries. 64 heads of 40001-65000 entries: one CTA
+// a head 286 us, eight 31 us; 576 heads of 700-1000: 11 us with one.
+cudaError_t launch_select(const ppyb200_evict_args& a, int64_t heads, int64_t most, int sm_count,
+                          cudaStream_t stream) {
+  static ppyb200::DeviceOnce once;
+  int ready = 0;
+  cudaError_t e = once.get([](int* value) {
+    *value = 1;
+    return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kCachedRanks * 4);
+  }, &ready);
+  if (e != cudaSuccess) return e;
+  int ranks = 1;
+  while (ranks < 8 && heads * ranks * 2 <= 4 * (int64_t)sm_count &&
+         a.capacity >= (int64_t)ranks * 2 * 2048)
+    ranks *= 2;
+  const int64_t stretch = (a.capacity + ranks - 1) / ranks;
+  const int cached = (int)(stretch < kCachedRanks ? stretch : kCachedRanks);
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(heads * ranks));
+  config.blockDim = dim3(kSelectThreads);
+  config.dynamicSmemBytes = (size_t)cached * 4;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = (unsigned)ranks;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = ppyb200_pdl() ? 2 : 1;
+  return cudaLaunchKernelEx(&config, evict_select_kernel, a, most, cached);
 }
 
 const char* refusal(const ppyb200_evict_args& a) {
@@ -532,8 +779,7 @@ int32_t ppyb200_evict(const ppyb200_evict_args* args) {
     return refuse("ppyb200_evict",
                   "a 16-byte aligned workspace of ppyb200_evict_workspace bytes required");
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(ppyb200_stream());
-  cudaError_t e = ppyb200::launch_pdl(evict_select_kernel, dim3((unsigned)heads),
-                                      dim3(kSelectThreads), 0, stream, a, most);
+  cudaError_t e = launch_select(a, heads, most, ppyb200_sm_count(), stream);
   if (e == cudaSuccess && most > 0)
     e = ppyb200::launch_pdl(evict_move_kernel,
                             dim3((unsigned)((most + kMoveRows - 1) / kMoveRows), (unsigned)heads),

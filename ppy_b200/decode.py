@@ -52,20 +52,23 @@ def _need(ok: bool, what: str) -> None:
         raise B200Error(what)
 
 
-def _element_rows(name: str, t, shape, dtype, device) -> None:
-    """A tensor of `shape` and `dtype` on `device` with unit stride along its last axis."""
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or (
-            t.stride(-1) != 1 and shape[-1] > 1):
-        raise B200Error(f"{name}: {dtype} {list(shape)} on {device}, unit stride along the last "
+def _element_rows(name: str, t, shape, dtype, device: int):
+    """The strides of a tensor of `shape` and `dtype` on CUDA device `device` with unit stride along
+    its last axis."""
+    strides = t.stride()
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (
+            strides[-1] != 1 and shape[-1] > 1):
+        raise B200Error(f"{name}: {dtype} {list(shape)} on cuda:{device}, unit stride along the last "
                         f"axis (not {t.dtype} {list(t.shape)} on {t.device}, strides "
-                        f"{list(t.stride())})")
+                        f"{list(strides)})")
+    return strides
 
 
-def _whole(name: str, t, shape, dtype, device) -> None:
-    """A contiguous tensor of `shape` and `dtype` on `device`."""
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or (
+def _whole(name: str, t, shape, dtype, device: int) -> None:
+    """A contiguous tensor of `shape` and `dtype` on CUDA device `device`."""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (
             not t.is_contiguous()):
-        raise B200Error(f"{name}: contiguous {dtype} {list(shape)} on {device} (not {t.dtype} "
+        raise B200Error(f"{name}: contiguous {dtype} {list(shape)} on cuda:{device} (not {t.dtype} "
                         f"{list(t.shape)} on {t.device}, strides {list(t.stride())})")
 
 
@@ -101,58 +104,63 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
     parents. `status` (int32 [1], optional) is raised to 2 when a length, count or parent is out of
     range: the call then keeps to the buffers, and takes such a parent for -1."""
     torch = _torch()
-    kind, device = _kinds().get(q.dtype), q.device
-    _need(kind is not None and q.is_cuda and q.dim() == 4 and keys.dim() == 4,
-          "q: bf16 or f16 [batch, nodes, heads, head_dim], keys [batch, kv_heads, capacity, "
-          "head_dim], on a CUDA device")
-    batch, nodes, heads, d = q.shape
-    kv_heads, capacity = keys.shape[1], keys.shape[2]
-    _element_rows("q", q, (batch, nodes, heads, d), q.dtype, device)
-    _element_rows("k_new", k_new, (batch, nodes, kv_heads, d), q.dtype, device)
-    _element_rows("v_new", v_new, (batch, nodes, kv_heads, d), q.dtype, device)
-    _element_rows("keys", keys, (batch, kv_heads, capacity, d), q.dtype, device)
-    _element_rows("values", values, (batch, kv_heads, capacity, d), q.dtype, device)
+    dtype, device = q.dtype, q.get_device()
+    kind = _kinds().get(dtype)
+    if kind is None or device < 0 or q.dim() != 4 or keys.dim() != 4:
+        raise B200Error("q: bf16 or f16 [batch, nodes, heads, head_dim], keys [batch, kv_heads, "
+                        "capacity, head_dim], on a CUDA device")
+    batch, nodes, heads, d = shape = q.shape
+    cache = keys.shape
+    kv_heads, capacity = cache[1], cache[2]
+    new, entries = (batch, nodes, kv_heads, d), (batch, kv_heads, capacity, d)
+    q_strides = _element_rows("q", q, shape, dtype, device)
+    k_strides = _element_rows("k_new", k_new, new, dtype, device)
+    v_strides = _element_rows("v_new", v_new, new, dtype, device)
+    keys_strides = _element_rows("keys", keys, entries, dtype, device)
+    values_strides = _element_rows("values", values, entries, dtype, device)
     _whole("lengths", lengths, (batch,), torch.int32, device)
-    parents_stride = 0
+    parents_stride = parents_at = counts_at = status_at = workspace_at = 0
     if parents is not None:
         shared = parents.dim() == 1
         _whole("parents", parents, (nodes,) if shared else (batch, nodes), torch.int32, device)
-        parents_stride = 0 if shared else nodes
+        parents_stride, parents_at = 0 if shared else nodes, parents.data_ptr()
     if counts is not None:
         _whole("counts", counts, (batch,), torch.int32, device)
+        counts_at = counts.data_ptr()
     if status is not None:
         _whole("status", status, (1,), torch.int32, device)
-    with runtime.launches_beside_torch(device.index) as launch:
-        make = torch.empty if counts is None else torch.zeros
+        status_at = status.data_ptr()
+    with runtime.launches_beside_torch(device) as launch:
         made = []
-        if out is None:
-            out = make((batch, nodes, heads, d), dtype=q.dtype, device=device)
-            made.append(out)
-        else:
-            _element_rows("out", out, (batch, nodes, heads, d), q.dtype, device)
-        if lse is None:
-            lse = make((batch, heads, nodes), dtype=torch.float32, device=device)
-            made.append(lse)
-        else:
-            _whole("lse", lse, (batch, heads, nodes), torch.float32, device)
-        if launch.side is not None and made:  # zeros were written on torch's stream
-            launch.side.wait_stream(torch.cuda.current_stream())
-        size = _attention_workspace(device.index, kind, batch, nodes, heads, kv_heads, d,
-                                    capacity)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        if out is None or lse is None:
+            make = torch.empty if counts is None else torch.zeros
+            if out is None:
+                out = make(shape, dtype=dtype, device=q.device)
+                made.append(out)
+            if lse is None:
+                lse = make((batch, heads, nodes), dtype=torch.float32, device=q.device)
+                made.append(lse)
+            if launch.side is not None:  # zeros were written on torch's stream
+                launch.side.wait_stream(torch.cuda.current_stream())
+        out_strides = _element_rows("out", out, shape, dtype, device)
+        _whole("lse", lse, (batch, heads, nodes), torch.float32, device)
+        size = _attention_workspace(device, kind, batch, nodes, heads, kv_heads, d, capacity)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            made.append(workspace)
+            workspace_at = workspace.data_ptr()
         args = _ATTENTION.pack(
             q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), keys.data_ptr(), values.data_ptr(),
-            lengths.data_ptr(), _address(parents), _address(counts), out.data_ptr(),
-            lse.data_ptr(), _address(status), _address(workspace), size, kind, batch, nodes,
-            heads, kv_heads, d, capacity, *q.stride()[:3], *k_new.stride()[:3],
-            *v_new.stride()[:3], *keys.stride()[:3], *values.stride()[:3], *out.stride()[:3],
-            parents_stride, 1.0 / math.sqrt(d) if scale is None else scale)
+            lengths.data_ptr(), parents_at, counts_at, out.data_ptr(), lse.data_ptr(), status_at,
+            workspace_at, size, kind, batch, nodes, heads, kv_heads, d, capacity,
+            *q_strides[:3], *k_strides[:3], *v_strides[:3], *keys_strides[:3],
+            *values_strides[:3], *out_strides[:3], parents_stride,
+            1.0 / math.sqrt(d) if scale is None else scale)
         if runtime.library().ppyb200_tree_attention(args) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
         if launch.side is not None:
-            for t in (*made, workspace):
-                if t is not None:
-                    t.record_stream(launch.side)
+            for t in made:
+                t.record_stream(launch.side)
     return out, lse
 
 
@@ -174,16 +182,16 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
     caller's to advance. `status` as in tree_attention: raised when the path is not in order (it is
     cut there) or a length or count is out of range."""
     torch = _torch()
-    kind, device = _kinds().get(keys.dtype), keys.device
-    _need(kind is not None and keys.is_cuda and keys.dim() == 5 and q.dim() == 5,
+    kind, device = _kinds().get(keys.dtype), keys.get_device()
+    _need(kind is not None and device >= 0 and keys.dim() == 5 and q.dim() == 5,
           "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim], q [layers, batch, "
           "nodes, heads, head_dim], on a CUDA device")
     layers, batch, kv_heads, capacity, d = keys.shape
     nodes, heads = q.shape[2], q.shape[3]
     steps = path.shape[-1]
-    _element_rows("q", q, (layers, batch, nodes, heads, d), keys.dtype, device)
-    _element_rows("keys", keys, tuple(keys.shape), keys.dtype, device)
-    _element_rows("values", values, tuple(keys.shape), keys.dtype, device)
+    q_strides = _element_rows("q", q, (layers, batch, nodes, heads, d), keys.dtype, device)
+    keys_strides = _element_rows("keys", keys, keys.shape, keys.dtype, device)
+    values_strides = _element_rows("values", values, keys.shape, keys.dtype, device)
     if weights is not None:
         _whole("lse", lse, (layers, batch, heads, nodes), torch.float32, device)
     for name, t in (("lengths", lengths), ("seen", seen), ("accepted", accepted)):
@@ -199,12 +207,12 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
             strides = t.stride()[:3]
     if status is not None:
         _whole("status", status, (1,), torch.int32, device)
-    with runtime.launches_beside_torch(device.index):
+    with runtime.launches_beside_torch(device):
         args = _ACCEPT.pack(
             q.data_ptr(), lse.data_ptr(), keys.data_ptr(), values.data_ptr(), _address(weights),
             _address(positions), lengths.data_ptr(), seen.data_ptr(), path.data_ptr(),
             accepted.data_ptr(), _address(status), kind, layers, batch, nodes, steps, heads,
-            kv_heads, d, capacity, *q.stride()[:4], *keys.stride()[:4], *values.stride()[:4],
+            kv_heads, d, capacity, *q_strides[:4], *keys_strides[:4], *values_strides[:4],
             *strides, 1.0 / math.sqrt(d) if scale is None else scale)
         if runtime.library().ppyb200_accept(args) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
@@ -231,15 +239,15 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
     [layers, batch, kv_heads, at least budget], the tables themselves by default. Sequences of up to `budget` entries
     keep them all. lengths are the caller's to set to min(lengths, budget)."""
     torch = _torch()
-    device = keys.device
-    _need(keys.dtype in _kinds() and keys.is_cuda and keys.dim() == 5,
+    device = keys.get_device()
+    _need(keys.dtype in _kinds() and device >= 0 and keys.dim() == 5,
           "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim] on a CUDA device")
     layers, batch, kv_heads, capacity, d = keys.shape
     budget, recent = int(budget), int(recent)
     _need(0 < budget <= capacity and recent >= 0,
           "a budget of 1 up to the capacity, and recent not negative")
-    _element_rows("keys", keys, tuple(keys.shape), keys.dtype, device)
-    _element_rows("values", values, tuple(keys.shape), keys.dtype, device)
+    keys_strides = _element_rows("keys", keys, keys.shape, keys.dtype, device)
+    values_strides = _element_rows("values", values, keys.shape, keys.dtype, device)
     _element_rows("weights", weights, (layers, batch, kv_heads, capacity), torch.float32, device)
     _element_rows("positions", positions, (layers, batch, kv_heads, capacity), torch.int32,
                   device)
@@ -258,10 +266,11 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
         _whole(name, t, (batch,), torch.int32, device)
     if status is not None:
         _whole("status", status, (1,), torch.int32, device)
-    with runtime.launches_beside_torch(device.index) as launch:
-        kept = torch.empty((layers, batch, kv_heads, budget), dtype=torch.int32, device=device)
+    with runtime.launches_beside_torch(device) as launch:
+        kept = torch.empty((layers, batch, kv_heads, budget), dtype=torch.int32,
+                           device=keys.device)
         size = _evict_workspace(layers, batch, kv_heads, d, capacity, budget)
-        workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
+        workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=keys.device)
         if launch.side is not None:
             kept.record_stream(launch.side)
             workspace.record_stream(launch.side)
@@ -270,7 +279,7 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
             weights_out.data_ptr(), positions_out.data_ptr(), kept.data_ptr(),
             lengths.data_ptr(), seen.data_ptr(), _address(status), workspace.data_ptr(),
             workspace.numel(), layers, batch, kv_heads, d, capacity, budget, recent,
-            *keys.stride()[:4], *values.stride()[:4], *weights.stride()[:3],
+            *keys_strides[:4], *values_strides[:4], *weights.stride()[:3],
             *weights_out.stride()[:3])
         if runtime.library().ppyb200_evict(args) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())

@@ -242,10 +242,10 @@ class GPT2:
         if parents is not None:
             shared = parents.dim() == 1
             decode._whole("parents", parents, (nodes,) if shared else (batch, nodes),
-                          torch.int32, ids.device)
+                          torch.int32, ids.get_device())
             stride = 0 if shared else nodes
         if counts is not None:
-            decode._whole("counts", counts, (batch,), torch.int32, ids.device)
+            decode._whole("counts", counts, (batch,), torch.int32, ids.get_device())
         s = cache.buffers.get((batch, nodes))
         if s is None:
             d = ids.device

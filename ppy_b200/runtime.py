@@ -53,6 +53,8 @@ _library: ctypes.CDLL | None = None
 def library() -> ctypes.CDLL:
     """libppyb200.so, loaded once with its symbols global (the modules resolve them)."""
     global _library
+    if _library is not None:
+        return _library
     with _lock:
         if _library is not None:
             return _library
@@ -123,35 +125,37 @@ class launches_beside_torch:
     call's, so the tensors are the caller's to use as if the call had run on it; `side` is the
     thread's stream then, for tensors made inside (record_stream), else None."""
 
-    __slots__ = ("_guard", "_stream", "side")
+    __slots__ = ("_guard", "_index", "side")
 
     def __init__(self, index: int) -> None:
         import torch
 
         lib = library()
         bound = lib.ppyb200_current_device()
-        self._guard = None
+        self._guard = self.side = None
+        self._index = index
         if bound != index and bound >= 0:
             raise B200Error(f"tensors on cuda:{index}, but this thread's device is {bound} "
                             "(runtime.init)")
-        if torch.cuda.current_device() != index:
+        if torch._C._cuda_getDevice() != index:
             self._guard = torch.cuda.device(index)
             self._guard.__enter__()
         if bound < 0:
             init(index)
-        self._stream, self.side = torch.cuda.current_stream(index), None
         handle = lib.ppyb200_stream() or 0
-        if handle != (self._stream.cuda_stream or _LEGACY_STREAM):
+        if handle != (torch._C._cuda_getCurrentRawStream(index) or _LEGACY_STREAM):
             self.side = (torch.cuda.default_stream(index) if handle == _LEGACY_STREAM
                          else torch.cuda.ExternalStream(handle, index))
-            self.side.wait_stream(self._stream)
+            self.side.wait_stream(torch.cuda.current_stream(index))
 
     def __enter__(self) -> "launches_beside_torch":
         return self
 
     def __exit__(self, *exc) -> None:
         if self.side is not None:
-            self._stream.wait_stream(self.side)
+            import torch
+
+            torch.cuda.current_stream(self._index).wait_stream(self.side)
         if self._guard is not None:
             self._guard.__exit__(*exc)
 

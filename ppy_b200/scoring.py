@@ -34,14 +34,16 @@ def _kinds() -> dict:
     return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _rows(logits) -> tuple[int, int]:
-    """(rows, distance between rows) of [..., vocab] logits with evenly spaced rows."""
-    shape, strides = logits.shape, logits.stride()
+def _rows(shape, strides) -> tuple[int, int]:
+    """(rows, distance between rows) of [..., vocab] logits with evenly spaced rows; the distance is
+    -1 where they are not."""
+    if len(shape) == 2 and shape[0] > 1:
+        return shape[0], strides[0]
     rows, pitch = 1, 0
     for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size != 1:
             if rows > 1 and stride != pitch * rows:
-                return logits.numel() // shape[-1], -1
+                return rows * size, -1
             pitch = stride if rows == 1 else pitch
         rows *= size
     return rows, pitch if rows > 1 else shape[-1]
@@ -57,34 +59,37 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     or +inf, or with nothing above -inf, has NaN log probabilities and entropy."""
     import torch
 
-    kind = _kinds().get(logits.dtype)
-    if kind is None or not logits.is_cuda or logits.dim() < 1 or logits.shape[-1] < 1:
+    kind, device = _kinds().get(logits.dtype), logits.get_device()
+    shape = logits.shape
+    if kind is None or device < 0 or len(shape) < 1 or shape[-1] < 1:
         raise B200Error("logits: f32, bf16 or f16 [..., vocab] on a CUDA device")
-    leading, vocab, device = tuple(logits.shape[:-1]), logits.shape[-1], logits.device
-    rows, pitch = _rows(logits)
-    if pitch < vocab or (logits.stride(-1) != 1 and vocab > 1):
+    leading, vocab, strides = shape[:-1], shape[-1], logits.stride()
+    rows, pitch = _rows(shape, strides)
+    if pitch < vocab or (strides[-1] != 1 and vocab > 1):
         raise B200Error("logits: unit stride along the vocabulary, rows evenly spaced and at least "
                         "vocab elements apart")
-    several = tokens.dim() == len(leading) + 1
-    if (tokens.dtype != torch.int64 or tokens.device != device or not tokens.is_contiguous()
-            or tuple(tokens.shape[:len(leading)]) != leading
-            or not (several or tokens.dim() == len(leading))):
+    asked = tokens.shape
+    several = len(asked) == len(shape)
+    if (tokens.dtype is not torch.int64 or tokens.get_device() != device
+            or not tokens.is_contiguous() or asked[:len(leading)] != leading
+            or not (several or len(asked) == len(leading))):
         raise B200Error(f"tokens: contiguous int64 {list(leading)} or {list(leading)} + [given], "
-                        f"on {device}")
+                        f"on {logits.device}")
     if not 0 <= top <= min(TOP_LIMIT, vocab):
         raise B200Error(f"top: 0 up to {TOP_LIMIT} and the vocabulary")
-    given = tokens.shape[-1] if several else 1
-    with runtime.launches_beside_torch(device.index) as launch:
+    with runtime.launches_beside_torch(device) as launch:
+        place, f32 = logits.device, torch.float32
         result = TokenLogprobs(
-            torch.empty(tokens.shape, dtype=torch.float32, device=device),
-            torch.empty(leading, dtype=torch.float32, device=device),
-            torch.empty((*leading, top), dtype=torch.float32, device=device),
-            torch.empty((*leading, top), dtype=torch.int64, device=device))
+            torch.empty(asked, dtype=f32, device=place),
+            torch.empty(leading, dtype=f32, device=place),
+            torch.empty((*leading, top), dtype=f32, device=place),
+            torch.empty((*leading, top), dtype=torch.int64, device=place))
         if launch.side is not None:
             for t in result:
                 t.record_stream(launch.side)
         if runtime.library().ppyb200_token_logprobs(
-                logits.data_ptr(), kind, rows, vocab, pitch, tokens.data_ptr(), given, top,
-                *(t.data_ptr() for t in result)) != runtime.STATUS_OK:
+                logits.data_ptr(), kind, rows, vocab, pitch, tokens.data_ptr(),
+                asked[-1] if several else 1, top, result[0].data_ptr(), result[1].data_ptr(),
+                result[2].data_ptr(), result[3].data_ptr()) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
     return result

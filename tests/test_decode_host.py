@@ -136,16 +136,19 @@ def test_operators_refuse_host_tensors_and_wrong_types():
 
 def test_argument_checks_name_the_tensor():
     x = torch.zeros(2, 3, 8, dtype=torch.bfloat16)
-    decode._element_rows("x", x.transpose(0, 1), (3, 2, 8), torch.bfloat16, x.device)
+    on = x.get_device()  # -1: host memory
+    assert decode._element_rows("x", x.transpose(0, 1), (3, 2, 8), torch.bfloat16, on) == (8, 24, 1)
     for bad in (x.transpose(1, 2), x.float(), x[:1]):
         with pytest.raises(runtime.B200Error, match="x:"):
-            decode._element_rows("x", bad, (2, 3, 8), torch.bfloat16, x.device)
+            decode._element_rows("x", bad, (2, 3, 8), torch.bfloat16, on)
+    with pytest.raises(runtime.B200Error, match="x:"):
+        decode._element_rows("x", x, (2, 3, 8), torch.bfloat16, 0)
     with pytest.raises(runtime.B200Error, match="n:"):
-        decode._whole("n", torch.zeros(4, dtype=torch.int32)[::2], (2,), torch.int32, x.device)
+        decode._whole("n", torch.zeros(4, dtype=torch.int32)[::2], (2,), torch.int32, on)
 
 
 def test_logits_rows_layout():
-    rows = scoring._rows
+    rows = lambda t: scoring._rows(t.shape, t.stride())  # noqa: E731
     assert rows(torch.empty(4, 10)) == (4, 10)
     assert rows(torch.empty(2, 3, 16)[:, :, :10]) == (6, 16)
     assert rows(torch.empty(2, 3, 16)[:, 1]) == (2, 48)
