@@ -5,18 +5,21 @@
 //   H = - sum p log p = log Z - (sum (x - m) e^{x - m}) / Z
 //
 // m, Z and the sum T of (x - m) e^{x - m} run along the row with each other: when the maximum
-// grows by D, Z becomes e^{-D} Z and T becomes e^{-D} (T - D Z). Everything is kept in powers of
-// two (y = (x - m) log2 e), one exponential an element.
+// grows by D, Z becomes e^{-D} Z and T becomes e^{-D} (T - D Z). One exponential an element, the
+// other arithmetic on pairs.
 //
-// The alternatives need no second pass over the row. A CTA's threads form 64 slots; the k-th
-// largest of the slots' maxima is a lower bound for the k-th largest logit, and only slots whose
-// maximum reaches it (about k of them) hold candidates: their elements, just read, come from L2
-// again. The few candidates are ranked by counting.
+// The alternatives need no second pass over the row. The k-th largest of 64 slots' maxima (of four
+// threads each) is a lower bound for the k-th largest logit, and only threads whose own maximum
+// reaches it (about k of 256) hold candidates: their elements, just read, come from L2 again. The
+// few candidates are ranked by counting. Few rows are split over a cluster of CTAs each, whose
+// first joins the sums and the alternatives of the parts.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <cooperative_groups.h>
 
 #include "../../include/ppyb200.h"
 #include "mma16.cuh"
@@ -28,9 +31,11 @@ using ppyb200::mma16::exp2_sfu;
 using ppyb200::mma16::kLn2;
 using ppyb200::mma16::kLog2e;
 
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kSlots = PPYB200_TOP_LIMIT;
 constexpr int kCandidates = 1024;
-constexpr float kLeast = -200.f;  // 2^kLeast = 0 in f32: stands for -inf where 0 times it is 0
+constexpr int kMostRanks = 8;    // CTAs of a cluster
+constexpr float kLeast = -200.f;  // e^kLeast = 0 in f32: stands for -inf where 0 times it is 0
 
 // A logit as an unsigned number in its order: NaN above all, the two zeros alike.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -43,24 +48,11 @@ __device__ __forceinline__ float disordered(uint32_t key) {
   return __uint_as_float((key >> 31) != 0 ? key & 0x7fffffffu : ~key);
 }
 
+// Sixteen bytes of logits as pairs of f32.
 template <class T>
-struct Vector;
-template <>
-struct Vector<float> {
-  static constexpr int kCount = 4;
-  __device__ __forceinline__ static void load(const float* p, float (&v)[4]) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(p));
-    v[0] = x.x;
-    v[1] = x.y;
-    v[2] = x.z;
-    v[3] = x.w;
-  }
-};
-template <class T>
-struct Vector16 {
-  static constexpr int kCount = 8;
-  __device__ __forceinline__ static void load(const T* p, float (&v)[8]) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+struct Vector {
+  static constexpr int kCount = 8, kPairs = 4;
+  __device__ __forceinline__ static void unpack(const uint4& x, float (&v)[8]) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -71,18 +63,32 @@ struct Vector16 {
   }
 };
 template <>
-struct Vector<__nv_bfloat16> : Vector16<__nv_bfloat16> {};
-template <>
-struct Vector<__half> : Vector16<__half> {};
+struct Vector<float> {
+  static constexpr int kCount = 4, kPairs = 2;
+  __device__ __forceinline__ static void unpack(const uint4& x, float (&v)[4]) {
+    v[0] = __uint_as_float(x.x);
+    v[1] = __uint_as_float(x.y);
+    v[2] = __uint_as_float(x.z);
+    v[3] = __uint_as_float(x.w);
+  }
+};
 
-struct Sums {  // of a part of a row: maximum, Z and T in powers of two
-  float m = -INFINITY, z = 0.f, t = 0.f;
+using ppyb200::add2;
+using ppyb200::f2;
+using ppyb200::fma2;
+using ppyb200::mul2;
+using ppyb200::unf2;
+
+// Maximum, Z and T of a part of a row; Z and T as two sums each until they are joined.
+struct Sums {
+  float m = -INFINITY;
+  uint64_t z = 0, t = 0;
 
   __device__ __forceinline__ void raise_to(float top) {
-    const float drop = m == -INFINITY ? 0.f : fmaxf((m - top) * kLog2e, kLeast);
-    const float f = exp2_sfu(drop);
-    t = m == -INFINITY ? 0.f : f * (t + drop * z);
-    z = m == -INFINITY ? 0.f : f * z;
+    const float drop = fmaxf(m - top, kLeast);
+    const float f = exp2_sfu(drop * kLog2e);
+    t = mul2(f2(f, f), fma2(f2(drop, drop), z, t));
+    z = mul2(f2(f, f), z);
     m = top;
   }
   template <int N>
@@ -93,243 +99,315 @@ struct Sums {  // of a part of a row: maximum, Z and T in powers of two
     if (top > m) raise_to(top);
     const float u = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; i += 2) {
       // the difference first: exact near the maximum, however large the logits are
-      const float y = (v[i] - u) * kLog2e, e = exp2_sfu(y);
-      z += e;
-      t = fmaf(fmaxf(y, kLeast), e, t);
+      const uint64_t d = add2(f2(v[i], N == 1 ? -INFINITY : v[(i + 1) % N]), f2(-u, -u));
+      float y0, y1, d0, d1;
+      unf2(mul2(d, f2(kLog2e, kLog2e)), y0, y1);
+      unf2(d, d0, d1);
+      const uint64_t e = f2(exp2_sfu(y0), exp2_sfu(y1));
+      z = add2(z, e);
+      t = fma2(f2(fmaxf(d0, kLeast), fmaxf(d1, kLeast)), e, t);
     }
   }
-  __device__ __forceinline__ void join(const Sums& o) {
-    Sums a = *this, b = o;
-    const float top = fmaxf(a.m, b.m);
-    if (top > a.m) a.raise_to(top);
-    if (top > b.m) b.raise_to(top);
-    m = top;
-    z = a.z + b.z;
-    t = a.t + b.t;
+  __device__ __forceinline__ void join(float om, uint64_t oz, uint64_t ot) {
+    Sums o;
+    o.m = om;
+    o.z = oz;
+    o.t = ot;
+    const float top = fmaxf(m, om);
+    if (top > m) raise_to(top);
+    if (top > om) o.raise_to(top);
+    z = add2(z, o.z);
+    t = add2(t, o.t);
+  }
+  __device__ __forceinline__ float total_z() const {
+    float a, b;
+    unf2(z, a, b);
+    return a + b;
+  }
+  __device__ __forceinline__ float total_t() const {
+    float a, b;
+    unf2(t, a, b);
+    return a + b;
   }
 };
 
-// The elements of a row as a thread walks them: single ones up to the first 16-byte boundary,
-// vectors, single ones to the end. Slot s is threads [s w, s w + w) with w = THREADS / kSlots.
+// The elements of a part of a row as its threads walk them: single ones up to the first 16-byte
+// boundary, vectors, single ones to the end.
 template <class T>
 struct Row {
   const T* x;
-  int head, vectors, tail, vocab;
+  int head, vectors, tail, count;
   static constexpr int kCount = Vector<T>::kCount;
-  __device__ __forceinline__ Row(const T* row, int64_t count) : x(row), vocab((int)count) {
+  __device__ __forceinline__ Row(const T* row, int n) : x(row), count(n) {
     const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15u) / (int)sizeof(T);
-    head = off == 0 ? 0 : kCount - off;
-    head = head < vocab ? head : vocab;
-    vectors = (vocab - head) / kCount;
-    tail = vocab - head - vectors * kCount;
+    head = min(off == 0 ? 0 : kCount - off, count);
+    vectors = (count - head) / kCount;
+    tail = count - head - vectors * kCount;
   }
-  __device__ __forceinline__ const T* vector(int i) const { return x + head + i * kCount; }
-  __device__ __forceinline__ int tail_at() const { return vocab - tail; }
+  __device__ __forceinline__ uint4 raw(int i) const {
+    return __ldg(reinterpret_cast<const uint4*>(x + head + i * kCount));
+  }
+  __device__ __forceinline__ int tail_at() const { return count - tail; }
+  __device__ __forceinline__ bool has(int thread) const {
+    return thread < head || thread < vectors || thread < tail;
+  }
 };
 
-template <class T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-token_logprobs_kernel(const T* __restrict__ logits, int64_t vocab, int64_t pitch,
-                      const int64_t* __restrict__ tokens, int given, int top,
-                      float* __restrict__ logprobs, float* __restrict__ entropy,
-                      float* __restrict__ top_logprobs, int64_t* __restrict__ top_tokens) {
-  constexpr int kCount = Vector<T>::kCount, kWarps = THREADS / 32, kWidth = THREADS / kSlots;
-  constexpr int kUnroll = 4;
-  __shared__ Sums parts[kWarps];
-  __shared__ uint32_t slot_max[kSlots];
-  __shared__ uint32_t threshold, found;
-  __shared__ uint64_t candidates[kCandidates];
-  ppyb200::pdl_wait();
+struct Shared {
+  Sums parts[kWarps];
+  Sums whole;                  // of this CTA's part, read by the cluster's first
+  uint32_t thread_max[kThreads], slot_max[kSlots];
+  uint64_t candidates[kCandidates];  // (logit as a number in its order, ~index)
+  uint64_t best[kSlots];             // the part's alternatives, the largest first
+  uint32_t bound, found, listed;
+  uint16_t list[kThreads];  // threads with candidates
+};
+
+// Ranks the first `count` candidates by counting: the `top` largest into best, from place `at`.
+__device__ __forceinline__ void rank_candidates(Shared& s, int count, int top) {
+#pragma unroll 1
+  for (int c = threadIdx.x; c < count; c += kThreads) {
+    const uint64_t mine = s.candidates[c];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) rank += s.candidates[j] > mine ? 1 : 0;
+    if (rank < top) s.best[rank] = mine;
+  }
+}
+
+// The part's `top` largest logits (top <= count) into s.best, by every thread of the CTA. `odd`:
+// a NaN or +inf among them, so that the threads' maxima are not their largest elements.
+template <class T>
+__device__ __forceinline__ void find_best(Shared& s, const Row<T>& row, int index0, int top,
+                                          float max, bool odd) {
+  constexpr int kCount = Vector<T>::kCount;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t r = blockIdx.x;
-  const Row<T> row(logits + r * pitch, vocab);
-
-  Sums s;
-  if (tid < row.head) {
-    const float v[1] = {(float)row.x[tid]};
-    s.add(v);
-  }
-  int i = tid;
-  for (; i + (kUnroll - 1) * THREADS < row.vectors; i += kUnroll * THREADS) {
-    float v[kUnroll][kCount];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) Vector<T>::load(row.vector(i + u * THREADS), v[u]);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) s.add(v[u]);
-  }
-  for (; i < row.vectors; i += THREADS) {
-    float v[kCount];
-    Vector<T>::load(row.vector(i), v);
-    s.add(v);
-  }
-  if (tid < row.tail) {
-    const float v[1] = {(float)row.x[row.tail_at() + tid]};
-    s.add(v);
-  }
-
-  // the slots' maxima: 0 for a slot without elements; one with a NaN among them is searched
-  if (top > 0) {
-    uint32_t key = tid < row.head || tid < row.vectors || tid < row.tail ? ordered(s.m) : 0u;
-    if (s.z != s.z) key = 0xffffffffu;  // NaN, or +inf: a bound that keeps the slot either way
-#pragma unroll
-    for (int w = 1; w < kWidth; w <<= 1)
-      key = max(key, __shfl_xor_sync(0xffffffffu, key, w));
-    if (tid % kWidth == 0) slot_max[tid / kWidth] = key;
-  }
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    Sums o;
-    o.m = __shfl_xor_sync(0xffffffffu, s.m, w);
-    o.z = __shfl_xor_sync(0xffffffffu, s.z, w);
-    o.t = __shfl_xor_sync(0xffffffffu, s.t, w);
-    s.join(o);
-  }
-  if (lane == 0) parts[warp] = s;
-  if (tid == 0) found = 0;
-  __syncthreads();
-  s = parts[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) s.join(parts[w]);
-  const float log_z = log2f(s.z) * kLn2;
-
-  for (int c = tid; c < given; c += THREADS) {
-    const int64_t token = tokens[r * given + c];
-    logprobs[r * given + c] = token >= 0 && token < vocab
-                                  ? ((float)row.x[token] - s.m) - log_z
-                                  : __uint_as_float(0x7fc00000u);
-  }
-  if (tid == 0 && entropy != nullptr) entropy[r] = log_z - s.t / s.z * kLn2;
-  if (top == 0) return;
-
-  // the bound: the top-th largest slot maximum. Where a slot's maximum is only an upper bound
-  // (a row with a NaN or an infinity) the slots are searched first.
-  if (s.z != s.z) {
-    __shared__ uint32_t exact_max[kSlots];
-    if (tid < kSlots) exact_max[tid] = 0;
-    __syncthreads();
-    uint32_t key = 0;
-    if (tid < row.head) key = max(key, ordered((float)row.x[tid]));
-    for (int k = tid; k < row.vectors; k += THREADS) {
+  uint32_t key = row.has(tid) ? ordered(max) : 0u;  // 0: no elements
+  if (odd) {
+    if (tid < row.head) key = ::max(key, ordered((float)row.x[tid]));
+    if (tid < row.tail) key = ::max(key, ordered((float)row.x[row.tail_at() + tid]));
+#pragma unroll 1
+    for (int i = tid; i < row.vectors; i += kThreads) {
       float v[kCount];
-      Vector<T>::load(row.vector(k), v);
+      Vector<T>::unpack(row.raw(i), v);
 #pragma unroll
-      for (int e = 0; e < kCount; ++e) key = max(key, ordered(v[e]));
+      for (int e = 0; e < kCount; ++e) key = ::max(key, ordered(v[e]));
     }
-    if (tid < row.tail) key = max(key, ordered((float)row.x[row.tail_at() + tid]));
-    atomicMax(&exact_max[tid / kWidth], key);
-    __syncthreads();
-    if (tid < kSlots) slot_max[tid] = exact_max[tid];
-    __syncthreads();
   }
+  s.thread_max[tid] = key;
+  uint32_t slot = key;
+#pragma unroll
+  for (int w = 1; w < kThreads / kSlots; w <<= 1)
+    slot = ::max(slot, __shfl_xor_sync(0xffffffffu, slot, w));
+  if (tid % (kThreads / kSlots) == 0) s.slot_max[tid / (kThreads / kSlots)] = slot;
+  if (tid == 0) s.found = s.listed = 0;
+  __syncthreads();
+  // the bound: the top-th largest slot maximum
   if (tid < kSlots) {
-    const uint32_t mine = slot_max[tid];
+    const uint32_t mine = s.slot_max[tid];
     int rank = 0;
 #pragma unroll 8
     for (int j = 0; j < kSlots; ++j) {
-      const uint32_t other = slot_max[j];
+      const uint32_t other = s.slot_max[j];
       rank += other > mine || (other == mine && j < tid) ? 1 : 0;
     }
-    if (rank == top - 1) threshold = mine;
+    if (rank == top - 1) s.bound = mine;
   }
   __syncthreads();
-  const uint32_t bound = threshold;
+  const uint32_t bound = s.bound;
 
-  // a warp takes a slot: keys of at least `least` join the candidates as (key, ~index)
+  // a warp takes a thread's elements: keys of at least `least` join the candidates
   auto collect = [&](uint32_t least) {
-    for (int slot = warp; slot < kSlots; slot += kWarps) {
-      if (slot_max[slot] < least) continue;
-      auto offer = [&](float value, int index) {
-        const uint32_t key = ordered(value);
-        if (key < least) return;
-        const uint32_t place = atomicAdd(&found, 1u);
-        if (place < kCandidates) candidates[place] = ((uint64_t)key << 32) | (uint32_t)~index;
-      };
-      const int first = slot * kWidth;
-      for (int t = first + lane; t < first + kWidth; t += 32) {
-        if (t < row.head) offer((float)row.x[t], t);
-        if (t < row.tail) offer((float)row.x[row.tail_at() + t], row.tail_at() + t);
-      }
-      constexpr int kAbreast = 32 / kWidth;
-      for (int k = lane / kWidth;; k += kAbreast) {
-        const int at = first + lane % kWidth + k * THREADS;
-        if (at >= row.vectors) break;
+    if (s.thread_max[tid] >= least && row.has(tid)) s.list[atomicAdd(&s.listed, 1u)] = tid;
+    __syncthreads();
+    auto offer = [&](float value, int index) {
+      const uint32_t k = ordered(value);
+      if (k < least) return;
+      const uint32_t place = atomicAdd(&s.found, 1u);
+      if (place < kCandidates)
+        s.candidates[place] = ((uint64_t)k << 32) | (uint32_t)~(index0 + index);
+    };
+    const int listed = (int)s.listed;
+#pragma unroll 1
+    for (int l = warp; l < listed; l += kWarps) {
+      const int thread = s.list[l];
+      if (lane == 0 && thread < row.head) offer((float)row.x[thread], thread);
+      if (lane == 1 && thread < row.tail)
+        offer((float)row.x[row.tail_at() + thread], row.tail_at() + thread);
+#pragma unroll 1
+      for (int i = thread + lane * kThreads; i < row.vectors; i += 32 * kThreads) {
         float v[kCount];
-        Vector<T>::load(row.vector(at), v);
+        Vector<T>::unpack(row.raw(i), v);
 #pragma unroll
-        for (int e = 0; e < kCount; ++e) offer(v[e], row.head + at * kCount + e);
+        for (int e = 0; e < kCount; ++e) offer(v[e], row.head + i * kCount + e);
       }
     }
-  };
-  auto write = [&](int rank, uint64_t candidate) {
-    top_logprobs[r * top + rank] = (disordered((uint32_t)(candidate >> 32)) - s.m) - log_z;
-    top_tokens[r * top + rank] = (int64_t)(uint32_t)~(uint32_t)candidate;
-  };
-  auto rank_candidates = [&](int count) {
-    for (int c = tid; c < count; c += THREADS) {
-      const uint64_t mine = candidates[c];
-      int rank = 0;
-      for (int j = 0; j < count && rank < top; ++j) rank += candidates[j] > mine ? 1 : 0;
-      if (rank < top) write(rank, mine);
-    }
+    __syncthreads();
   };
   collect(bound);
-  __syncthreads();
-  if (found <= kCandidates) {
-    rank_candidates((int)found);
+  if (s.found <= kCandidates) {
+    rank_candidates(s, (int)s.found, top);
     return;
   }
   // Many elements reach the bound: usually equal ones (a row of -inf with few exceptions). Those
   // above it first, then the equal ones of lowest index, found from the front.
   __syncthreads();
-  if (tid == 0) found = 0;
+  if (tid == 0) s.found = s.listed = 0;
   __syncthreads();
   if (bound != 0xffffffffu) collect(bound + 1);
-  __syncthreads();
-  const int above = (int)found;
+  const int above = (int)s.found;
   if (above <= kCandidates) {
-    rank_candidates(above);
+    rank_candidates(s, above, top);
     int taken = above;
-    for (int j0 = 0; j0 < row.vocab && taken < top; j0 += THREADS) {
+#pragma unroll 1
+    for (int j0 = 0; j0 < row.count && taken < top; j0 += kThreads) {
       const int j = j0 + tid;
-      const bool equal = j < row.vocab && ordered((float)row.x[j]) == bound;
+      const bool equal = j < row.count && ordered((float)row.x[j]) == bound;
       const uint32_t votes = __ballot_sync(0xffffffffu, equal);
       __syncthreads();
-      if (lane == 0) slot_max[warp] = __popc(votes);
+      if (lane == 0) s.slot_max[warp] = __popc(votes);
       __syncthreads();
-      int before = taken, total = 0;
+      int before = taken;
       for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += slot_max[w];
-        total += slot_max[w];
+        if (w < warp) before += s.slot_max[w];
+        taken += s.slot_max[w];
       }
       before += __popc(votes & ((1u << lane) - 1u));
       if (equal && before < top)
-        write(before, ((uint64_t)bound << 32) | (uint32_t)~j);
-      taken += total;
+        s.best[before] = ((uint64_t)bound << 32) | (uint32_t)~(index0 + j);
     }
     return;
   }
-  // More than kCandidates above the bound (a row that climbs from slot to slot): one maximum
+  // More than kCandidates above the bound (elements that gather in few threads): one maximum
   // after the other.
   uint64_t last = ~0ull;
+#pragma unroll 1
   for (int k = 0; k < top; ++k) {
-    uint64_t best = 0;
-    for (int j = tid; j < row.vocab; j += THREADS) {
-      const uint64_t candidate = ((uint64_t)ordered((float)row.x[j]) << 32) | (uint32_t)~j;
-      if ((k == 0 || candidate < last) && candidate > best) best = candidate;
+    uint64_t most = 0;
+#pragma unroll 1
+    for (int j = tid; j < row.count; j += kThreads) {
+      const uint64_t one =
+          ((uint64_t)ordered((float)row.x[j]) << 32) | (uint32_t)~(index0 + j);
+      if ((k == 0 || one < last) && one > most) most = one;
     }
 #pragma unroll
     for (int w = 16; w > 0; w >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, w);
-      best = other > best ? other : best;
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, most, w);
+      most = other > most ? other : most;
     }
     __syncthreads();
-    if (lane == 0) candidates[warp] = best;
+    if (lane == 0) s.candidates[warp] = most;
     __syncthreads();
-    for (int w = 0; w < kWarps; ++w) best = candidates[w] > best ? candidates[w] : best;
-    if (tid == 0) write(k, best);
-    last = best;
+    for (int w = 0; w < kWarps; ++w) most = s.candidates[w] > most ? s.candidates[w] : most;
+    if (tid == 0) s.best[k] = most;
+    last = most;
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+token_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t pitch,
+                      const int64_t* __restrict__ tokens, int given, int top,
+                      float* __restrict__ logprobs, float* __restrict__ entropy,
+                      float* __restrict__ top_logprobs, int64_t* __restrict__ top_tokens) {
+  namespace cg = cooperative_groups;
+  constexpr int kCount = Vector<T>::kCount, kUnroll = 4;
+  __shared__ Shared s;
+  ppyb200::pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r = blockIdx.x / ranks;
+  const T* whole_row = logits + r * pitch;
+  // a part of the row; whole lines, so that parts start on boundaries where rows do
+  const int part = ranks == 1 ? vocab : ((vocab + ranks - 1) / ranks + 63) / 64 * 64;
+  const int index0 = min(rank * part, vocab);
+  const Row<T> row(whole_row + index0, min(part, vocab - index0));
+
+  Sums sums;
+  if (tid < row.head) {
+    const float v[1] = {(float)row.x[tid]};
+    sums.add(v);
+  }
+  if (tid < row.tail) {
+    const float v[1] = {(float)row.x[row.tail_at() + tid]};
+    sums.add(v);
+  }
+  int i = tid;
+#pragma unroll 1
+  for (; i + (kUnroll - 1) * kThreads < row.vectors; i += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) raw[u] = row.raw(i + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float v[kCount];
+      Vector<T>::unpack(raw[u], v);
+      sums.add(v);
+    }
+  }
+#pragma unroll 1
+  for (; i < row.vectors; i += kThreads) {
+    float v[kCount];
+    Vector<T>::unpack(row.raw(i), v);
+    sums.add(v);
+  }
+
+  const int local_top = min(top, row.count);
+  if (local_top > 0) {
+    const float z = sums.total_z();
+    const bool odd = __syncthreads_or(z != z) != 0;
+    find_best(s, row, index0, local_top, sums.m, odd);
+  }
+#pragma unroll 1
+  for (int w = 16; w > 0; w >>= 1)
+    sums.join(__shfl_xor_sync(0xffffffffu, sums.m, w), __shfl_xor_sync(0xffffffffu, sums.z, w),
+              __shfl_xor_sync(0xffffffffu, sums.t, w));
+  if (lane == 0) s.parts[warp] = sums;
+  __syncthreads();
+  sums = s.parts[0];
+#pragma unroll 1
+  for (int w = 1; w < kWarps; ++w) sums.join(s.parts[w].m, s.parts[w].z, s.parts[w].t);
+  if (ranks > 1) {
+    if (tid == 0) s.whole = sums;
+    cluster.sync();
+    if (rank == 0) {
+#pragma unroll 1
+      for (int q = 1; q < ranks; ++q) {
+        const Sums* other = cluster.map_shared_rank(&s.whole, q);
+        sums.join(other->m, other->z, other->t);
+      }
+      // the parts' alternatives side by side, then ranked together
+      int count = 0;
+#pragma unroll 1
+      for (int q = 0; q < ranks && top > 0; ++q) {
+        const int n = min(top, max(0, min(part, vocab - q * part)));
+        const uint64_t* other = cluster.map_shared_rank(s.best, q);
+        for (int c = tid; c < n; c += kThreads) s.candidates[count + c] = other[c];
+        count += n;
+      }
+      __syncthreads();
+      rank_candidates(s, count, top);
+      __syncthreads();
+    }
+    cluster.sync();  // the others' shared memory has been read
+    if (rank != 0) return;
+  }
+  const float z = sums.total_z(), log_z = log2f(z) * kLn2;
+  if (tid == 0 && entropy != nullptr) entropy[r] = log_z - sums.total_t() / z;
+#pragma unroll 1
+  for (int c = tid; c < given; c += kThreads) {
+    const int64_t token = tokens[r * given + c];
+    logprobs[r * given + c] = token >= 0 && token < vocab
+                                  ? ((float)whole_row[token] - sums.m) - log_z
+                                  : __uint_as_float(0x7fc00000u);
+  }
+  if (tid < top) {
+    const uint64_t one = s.best[tid];
+    top_logprobs[r * top + tid] = (disordered((uint32_t)(one >> 32)) - sums.m) - log_z;
+    top_tokens[r * top + tid] = (int64_t)(uint32_t)~(uint32_t)one;
   }
 }
 
@@ -338,15 +416,25 @@ cudaError_t launch(const void* logits, int64_t rows, int64_t vocab, int64_t pitc
                    const int64_t* tokens, int64_t given, int64_t top, float* logprobs,
                    float* entropy, float* top_logprobs, int64_t* top_tokens,
                    cudaStream_t stream) {
-  const dim3 grid((unsigned)rows);
-  const T* x = static_cast<const T*>(logits);
-  if (rows >= 2 * ppyb200_sm_count())
-    return ppyb200::launch_pdl(token_logprobs_kernel<T, 256>, grid, dim3(256), 0, stream, x,
-                               vocab, pitch, tokens, (int)given, (int)top, logprobs, entropy,
-                               top_logprobs, top_tokens);
-  return ppyb200::launch_pdl(token_logprobs_kernel<T, 1024>, grid, dim3(1024), 0, stream, x, vocab,
-                             pitch, tokens, (int)given, (int)top, logprobs, entropy, top_logprobs,
-                             top_tokens);
+  // few rows: a cluster each, while the SMs have room and a part stays above 4096 logits
+  const int64_t room = 2 * (int64_t)ppyb200_sm_count();
+  int ranks = 1;
+  while (ranks < kMostRanks && rows * ranks * 2 <= room && vocab >= ranks * 2 * 4096) ranks *= 2;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(rows * ranks));
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = (unsigned)ranks;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = ppyb200_pdl() ? 2 : 1;
+  return cudaLaunchKernelEx(&config, token_logprobs_kernel<T>, static_cast<const T*>(logits),
+                            (int)vocab, pitch, tokens, (int)given, (int)top, logprobs, entropy,
+                            top_logprobs, top_tokens);
 }
 
 }  // namespace
