@@ -42,7 +42,6 @@ int32_t refuse(const char* who, const char* what) {
 // ---------------------------------------------------------------- accept
 
 constexpr int kAcceptThreads = 128;
-constexpr int kAcceptKeys = 512;  // prefix keys a CTA
 
 // Sixteen keys of a warp against the path's rows: the sums of e^{s - lse} over the rows for key
 // gid (sum0) and gid + 8 (sum1), complete in every lane of the quad. A fragments come straight
@@ -99,8 +98,9 @@ struct KeyRows {
 };
 
 template <class T, int D>
-__global__ void __launch_bounds__(kAcceptThreads)
-accept_kernel(const ppyb200_accept_args a, const int chunks) {
+__global__ void __launch_bounds__(kAcceptThreads, D == 64 ? 8 : 5)
+accept_kernel(const __grid_constant__ ppyb200_accept_args a, const int chunks,
+              const int chunk_keys) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int path[PPYB200_PATH_STEPS];
   __shared__ int valid;  // steps up to the first that is not in order
@@ -129,7 +129,7 @@ accept_kernel(const ppyb200_accept_args a, const int chunks) {
   n = valid;
   if (bad && last && kvh == 0 && tid == 0) raise(a.status);
   if (n <= 0) return;
-  const int64_t j0 = (int64_t)blockIdx.x * kAcceptKeys;
+  const int64_t j0 = (int64_t)blockIdx.x * chunk_keys;
   if (!last && j0 >= length) return;
 
   const int rows = n * group, blocks = (rows + 7) / 8;
@@ -163,17 +163,30 @@ accept_kernel(const ppyb200_accept_args a, const int chunks) {
                                               b * a.weights_strides[1] +
                                               kvh * a.weights_strides[2];
   if (!last) {
-    if (weights == nullptr) return;
-    const int64_t end = min(j0 + kAcceptKeys, length);
-    for (int64_t j = j0 + warp * 16; j < end; j += kAcceptThreads / 2) {
+    const int64_t end = min(j0 + chunk_keys, length);
+    // sixteen keys a warp at a time, the next sixteen and their weights under way meanwhile
+    constexpr int kStep = kAcceptThreads / 2;
+    KeyRows<T, D> k;
+    auto load = [&](int64_t j, KeyRows<T, D>& to, float& weight) {
       const int64_t ja = j + gid, jb = ja + 8;
-      KeyRows<T, D> k;
-      k.load(ja < end ? keys + ja * a.keys_strides[3] : nullptr,
-             jb < end ? keys + jb * a.keys_strides[3] : nullptr, d, tig);
+      to.load(ja < end ? keys + ja * a.keys_strides[3] : nullptr,
+              jb < end ? keys + jb * a.keys_strides[3] : nullptr, d, tig);
+      const int64_t mine = tig == 0 ? ja : jb;  // lanes 0 and 1 of a quad have a key each
+      weight = tig < 2 && mine < end ? weights[mine] : 0.f;
+    };
+    float weight;
+    load(j0 + warp * 16, k, weight);
+#pragma unroll 1
+    for (int64_t j = j0 + warp * 16; j < end; j += kStep) {
+      KeyRows<T, D> next;
+      float next_weight;
+      load(j + kStep, next, next_weight);
       float s0, s1;
       k.weigh(qf, lse, rows, scale, lane, 0, 0, s0, s1);
-      if (tig == 0 && ja < end) weights[ja] += s0;
-      if (tig == 1 && jb < end) weights[jb] += s1;
+      const int64_t mine = j + gid + (tig == 0 ? 0 : 8);
+      if (tig < 2 && mine < end) weights[mine] = weight + (tig == 0 ? s0 : s1);
+      k = next;
+      weight = next_weight;
     }
     return;
   }
@@ -235,11 +248,16 @@ cudaError_t launch_accept(const ppyb200_accept_args& a, cudaStream_t stream) {
                                 PPYB200_PATH_ROWS * (D * 2 + 4));
   }, &ready);
   if (e != cudaSuccess) return e;
-  const int chunks = (int)((a.capacity + kAcceptKeys - 1) / kAcceptKeys);
+  // Two waves of eight CTAs an SM over full caches, 128 to 4096 keys each: a CTA's start (lengths,
+  // path, queries: loads that follow one another) costs as much as some hundred keys.
+  const int64_t heads = a.layers * a.batch * a.kv_heads;
+  int64_t chunk = heads * a.capacity / (16 * (int64_t)ppyb200_sm_count());
+  chunk = chunk < 128 ? 128 : chunk > 4096 ? 4096 : (chunk + 63) / 64 * 64;
+  const int chunks = a.weights == nullptr ? 0 : (int)((a.capacity + chunk - 1) / chunk);
   return ppyb200::launch_pdl(kernel,
                              dim3((unsigned)chunks + 1, (unsigned)a.kv_heads,
                                   (unsigned)(a.layers * a.batch)),
-                             dim3(kAcceptThreads), smem, stream, a, chunks);
+                             dim3(kAcceptThreads), smem, stream, a, chunks, (int)chunk);
 }
 
 // ---------------------------------------------------------------- evict

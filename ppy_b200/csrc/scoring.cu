@@ -4,14 +4,15 @@
 //   m = max x,  Z = sum e^{x - m},  log p_i = x_i - m - log Z
 //   H = - sum p log p = log Z - (sum (x - m) e^{x - m}) / Z
 //
-// m, Z and the sum T of (x - m) e^{x - m} run along the row with each other: when the maximum
-// grows by D, Z becomes e^{-D} Z and T becomes e^{-D} (T - D Z). One exponential an element, the
-// other arithmetic on pairs.
+// Z and the sum T of (x - m) e^{x - m} run along the row with a reference m: when it grows by D, Z
+// becomes e^{-D} Z and T becomes e^{-D} (T - D Z). The reference follows the maximum only when
+// that is more than kSlack above it (a thread's maximum moves at every other vector, and some
+// thread's of a warp at nearly each). One exponential an element, the other arithmetic on pairs.
 //
-// The alternatives need no second pass over the row. The k-th largest of 64 slots' maxima (of four
-// threads each) is a lower bound for the k-th largest logit, and only threads whose own maximum
-// reaches it (about k of 256) hold candidates: their elements, just read, come from L2 again. The
-// few candidates are ranked by counting. Few rows are split over a cluster of CTAs each, whose
+// The alternatives need no second pass over the row. The k-th largest of the threads' maxima is a
+// lower bound for the k-th largest logit, and only the threads whose own maximum reaches it (about
+// k of 256) hold candidates: their elements, just read, come from L2 again. The few candidates are
+// ranked by counting. Few rows are split over a cluster of CTAs each, whose
 // first joins the sums and the alternatives of the parts.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -32,9 +33,10 @@ using ppyb200::mma16::kLn2;
 using ppyb200::mma16::kLog2e;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kSlots = PPYB200_TOP_LIMIT;
+constexpr int kTop = PPYB200_TOP_LIMIT;
 constexpr int kCandidates = 1024;
 constexpr int kMostRanks = 8;    // CTAs of a cluster
+constexpr float kSlack = 8.f;    // e^8 times as many terms as there are stay far from f32's limit
 constexpr float kLeast = -200.f;  // e^kLeast = 0 in f32: stands for -inf where 0 times it is 0
 
 // A logit as an unsigned number in its order: NaN above all, the two zeros alike.
@@ -79,9 +81,9 @@ using ppyb200::fma2;
 using ppyb200::mul2;
 using ppyb200::unf2;
 
-// Maximum, Z and T of a part of a row; Z and T as two sums each until they are joined.
+// Reference, maximum, Z and T of a part of a row; Z and T as two sums each until they are joined.
 struct Sums {
-  float m = -INFINITY;
+  float m = -INFINITY, most = -INFINITY;
   uint64_t z = 0, t = 0;
 
   __device__ __forceinline__ void raise_to(float top) {
@@ -96,7 +98,8 @@ struct Sums {
     float top = v[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-    if (top > m) raise_to(top);
+    most = fmaxf(most, top);
+    if (top > m + kSlack) raise_to(top);  // -inf + kSlack: the first finite one
     const float u = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
@@ -158,11 +161,11 @@ struct Row {
 struct Shared {
   Sums parts[kWarps];
   Sums whole;                  // of this CTA's part, read by the cluster's first
-  uint32_t thread_max[kThreads], slot_max[kSlots];
   uint64_t candidates[kCandidates];  // (logit as a number in its order, ~index)
-  uint64_t best[kSlots];             // the part's alternatives, the largest first
-  uint32_t bound, found, listed;
-  uint16_t list[kThreads];  // threads with candidates
+  uint64_t best[kTop];               // the part's alternatives, the largest first
+  uint32_t found, listed;
+  uint16_t list[kThreads];   // threads with candidates
+  uint32_t votes[kWarps];
 };
 
 // Ranks the first `count` candidates by counting: the `top` largest into best, from place `at`.
@@ -196,53 +199,45 @@ __device__ __forceinline__ void find_best(Shared& s, const Row<T>& row, int inde
       for (int e = 0; e < kCount; ++e) key = ::max(key, ordered(v[e]));
     }
   }
-  s.thread_max[tid] = key;
-  uint32_t slot = key;
-#pragma unroll
-  for (int w = 1; w < kThreads / kSlots; w <<= 1)
-    slot = ::max(slot, __shfl_xor_sync(0xffffffffu, slot, w));
-  if (tid % (kThreads / kSlots) == 0) s.slot_max[tid / (kThreads / kSlots)] = slot;
   if (tid == 0) s.found = s.listed = 0;
-  __syncthreads();
-  // the bound: the top-th largest slot maximum
-  if (tid < kSlots) {
-    const uint32_t mine = s.slot_max[tid];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < kSlots; ++j) {
-      const uint32_t other = s.slot_max[j];
-      rank += other > mine || (other == mine && j < tid) ? 1 : 0;
-    }
-    if (rank == top - 1) s.bound = mine;
-  }
-  __syncthreads();
-  const uint32_t bound = s.bound;
+  // The bound, bit by bit: the largest number of 20 leading bits (all 16 of 16-bit logits) that
+  // `top` threads reach; the bits left out only let a few more candidates in. Fewer than `top`
+  // threads with elements leave 0.
+  uint32_t bound = 0;
+#pragma unroll 1
+  for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+    if (__syncthreads_count(key >= (bound | bit)) >= top) bound |= bit;
 
-  // a warp takes a thread's elements: keys of at least `least` join the candidates
+  // keys of at least `least` join the candidates: all vectors of the threads that have any, dealt
+  // to all threads
   auto collect = [&](uint32_t least) {
-    if (s.thread_max[tid] >= least && row.has(tid)) s.list[atomicAdd(&s.listed, 1u)] = tid;
+    // what is below it as a float, most elements, needs no more than a comparison
+    const float floor =
+        least > 0x007fffffu && least <= 0xff800000u ? disordered(least) : -INFINITY;
+    if (key >= least && row.has(tid)) s.list[atomicAdd(&s.listed, 1u)] = (uint16_t)tid;
     __syncthreads();
     auto offer = [&](float value, int index) {
+      if (value < floor) return;
       const uint32_t k = ordered(value);
       if (k < least) return;
       const uint32_t place = atomicAdd(&s.found, 1u);
       if (place < kCandidates)
         s.candidates[place] = ((uint64_t)k << 32) | (uint32_t)~(index0 + index);
     };
-    const int listed = (int)s.listed;
+    const int listed = (int)s.listed, each = (row.vectors + kThreads - 1) / kThreads;
+    if (tid < listed) {
+      const int thread = s.list[tid];
+      if (thread < row.head) offer((float)row.x[thread], thread);
+      if (thread < row.tail) offer((float)row.x[row.tail_at() + thread], row.tail_at() + thread);
+    }
 #pragma unroll 1
-    for (int l = warp; l < listed; l += kWarps) {
-      const int thread = s.list[l];
-      if (lane == 0 && thread < row.head) offer((float)row.x[thread], thread);
-      if (lane == 1 && thread < row.tail)
-        offer((float)row.x[row.tail_at() + thread], row.tail_at() + thread);
-#pragma unroll 1
-      for (int i = thread + lane * kThreads; i < row.vectors; i += 32 * kThreads) {
-        float v[kCount];
-        Vector<T>::unpack(row.raw(i), v);
+    for (int item = tid; item < listed * each; item += kThreads) {
+      const int l = item / each, i = s.list[l] + (item - l * each) * kThreads;
+      if (i >= row.vectors) continue;
+      float v[kCount];
+      Vector<T>::unpack(row.raw(i), v);
 #pragma unroll
-        for (int e = 0; e < kCount; ++e) offer(v[e], row.head + i * kCount + e);
-      }
+      for (int e = 0; e < kCount; ++e) offer(v[e], row.head + i * kCount + e);
     }
     __syncthreads();
   };
@@ -251,9 +246,11 @@ __device__ __forceinline__ void find_best(Shared& s, const Row<T>& row, int inde
     rank_candidates(s, (int)s.found, top);
     return;
   }
-  // Many elements reach the bound: usually equal ones (a row of -inf with few exceptions). Those
-  // above it first, then the equal ones of lowest index, found from the front.
-  __syncthreads();
+  // Many elements reach the bound: usually equal ones (a row of -inf with few exceptions). The
+  // bound in full, those above it first, then the equal ones of lowest index, from the front.
+#pragma unroll 1
+  for (uint32_t bit = 1u << 11; bit != 0; bit >>= 1)
+    if (__syncthreads_count(key >= (bound | bit)) >= top) bound |= bit;
   if (tid == 0) s.found = s.listed = 0;
   __syncthreads();
   if (bound != 0xffffffffu) collect(bound + 1);
@@ -267,12 +264,12 @@ __device__ __forceinline__ void find_best(Shared& s, const Row<T>& row, int inde
       const bool equal = j < row.count && ordered((float)row.x[j]) == bound;
       const uint32_t votes = __ballot_sync(0xffffffffu, equal);
       __syncthreads();
-      if (lane == 0) s.slot_max[warp] = __popc(votes);
+      if (lane == 0) s.votes[warp] = __popc(votes);
       __syncthreads();
       int before = taken;
       for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s.slot_max[w];
-        taken += s.slot_max[w];
+        if (w < warp) before += s.votes[w];
+        taken += s.votes[w];
       }
       before += __popc(votes & ((1u << lane) - 1u));
       if (equal && before < top)
@@ -306,8 +303,11 @@ __device__ __forceinline__ void find_best(Shared& s, const Row<T>& row, int inde
   }
 }
 
+// Eight CTAs an SM: a row's end (joins, the bound, the candidates) loads next to nothing, and the
+// other CTAs' rows keep the memory busy meanwhile (47 registers and five CTAs: 16384 rows of
+// GPT-2 logits 577 us, 32 registers 549).
 template <class T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 8)
 token_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t pitch,
                       const int64_t* __restrict__ tokens, int given, int top,
                       float* __restrict__ logprobs, float* __restrict__ entropy,
@@ -359,7 +359,7 @@ token_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t pitch,
   if (local_top > 0) {
     const float z = sums.total_z();
     const bool odd = __syncthreads_or(z != z) != 0;
-    find_best(s, row, index0, local_top, sums.m, odd);
+    find_best(s, row, index0, local_top, sums.most, odd);
   }
 #pragma unroll 1
   for (int w = 16; w > 0; w >>= 1)
