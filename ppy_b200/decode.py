@@ -11,7 +11,7 @@ ppyb200_evict); `KVCache` holds the state that belongs together. A single token 
 node, and a piece of a prompt is a chain (`parents=None`).
 
 Calls are asynchronous on the thread's stream (`runtime.set_stream`), ordered with torch's current
-stream (`runtime.launches_beside_torch`), and read sequence lengths on the device, so that they can
+stream (`torch_calls.begin`), and read sequence lengths on the device, so that they can
 be captured into a CUDA graph and replayed as the cache grows. Each call's workspace is a torch
 allocation of its own: calls on several streams and captured graphs share none.
 """
@@ -22,8 +22,11 @@ import functools
 import math
 import struct
 
+import torch
+
 from . import runtime
 from .runtime import B200Error
+from .torch_calls import begin, element_rows, end, whole
 
 __all__ = ["KVCache", "accept_nodes", "evict", "tree_attention"]
 
@@ -35,41 +38,13 @@ _ACCEPT = struct.Struct("=35qd")  # ppyb200_accept_args
 _EVICT = struct.Struct("=33q")  # ppyb200_evict_args
 
 
-def _torch():
-    import torch
-
-    return torch
-
-
-@functools.cache
-def _kinds() -> dict:
-    torch = _torch()
-    return {torch.bfloat16: 1, torch.float16: 2}
+#: Element types, as the header numbers them.
+_KINDS = {torch.bfloat16: 1, torch.float16: 2}
 
 
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise B200Error(what)
-
-
-def _element_rows(name: str, t, shape, dtype, device: int):
-    """The strides of a tensor of `shape` and `dtype` on CUDA device `device` with unit stride along
-    its last axis."""
-    strides = t.stride()
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (
-            strides[-1] != 1 and shape[-1] > 1):
-        raise B200Error(f"{name}: {dtype} {list(shape)} on cuda:{device}, unit stride along the last "
-                        f"axis (not {t.dtype} {list(t.shape)} on {t.device}, strides "
-                        f"{list(strides)})")
-    return strides
-
-
-def _whole(name: str, t, shape, dtype, device: int) -> None:
-    """A contiguous tensor of `shape` and `dtype` on CUDA device `device`."""
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (
-            not t.is_contiguous()):
-        raise B200Error(f"{name}: contiguous {dtype} {list(shape)} on cuda:{device} (not {t.dtype} "
-                        f"{list(t.shape)} on {t.device}, strides {list(t.stride())})")
 
 
 def _address(t) -> int:
@@ -103,9 +78,8 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
     bf16 or f16; head_dim a multiple of 8 up to 128; rows on 16-byte boundaries; up to 256 nodes with
     parents. `status` (int32 [1], optional) is raised to 2 when a length, count or parent is out of
     range: the call then keeps to the buffers, and takes such a parent for -1."""
-    torch = _torch()
     dtype, device = q.dtype, q.get_device()
-    kind = _kinds().get(dtype)
+    kind = _KINDS.get(dtype)
     if kind is None or device < 0 or q.dim() != 4 or keys.dim() != 4:
         raise B200Error("q: bf16 or f16 [batch, nodes, heads, head_dim], keys [batch, kv_heads, "
                         "capacity, head_dim], on a CUDA device")
@@ -113,24 +87,24 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
     cache = keys.shape
     kv_heads, capacity = cache[1], cache[2]
     new, entries = (batch, nodes, kv_heads, d), (batch, kv_heads, capacity, d)
-    q_strides = _element_rows("q", q, shape, dtype, device)
-    k_strides = _element_rows("k_new", k_new, new, dtype, device)
-    v_strides = _element_rows("v_new", v_new, new, dtype, device)
-    keys_strides = _element_rows("keys", keys, entries, dtype, device)
-    values_strides = _element_rows("values", values, entries, dtype, device)
-    _whole("lengths", lengths, (batch,), torch.int32, device)
+    q_strides = element_rows("q", q, shape, dtype, device)
+    k_strides = element_rows("k_new", k_new, new, dtype, device)
+    v_strides = element_rows("v_new", v_new, new, dtype, device)
+    keys_strides = element_rows("keys", keys, entries, dtype, device)
+    values_strides = element_rows("values", values, entries, dtype, device)
+    lengths_at = whole("lengths", lengths, (batch,), torch.int32, device)
     parents_stride = parents_at = counts_at = status_at = workspace_at = 0
     if parents is not None:
         shared = parents.dim() == 1
-        _whole("parents", parents, (nodes,) if shared else (batch, nodes), torch.int32, device)
-        parents_stride, parents_at = 0 if shared else nodes, parents.data_ptr()
+        parents_at = whole("parents", parents, (nodes,) if shared else (batch, nodes),
+                           torch.int32, device)
+        parents_stride = 0 if shared else nodes
     if counts is not None:
-        _whole("counts", counts, (batch,), torch.int32, device)
-        counts_at = counts.data_ptr()
+        counts_at = whole("counts", counts, (batch,), torch.int32, device)
     if status is not None:
-        _whole("status", status, (1,), torch.int32, device)
-        status_at = status.data_ptr()
-    with runtime.launches_beside_torch(device) as launch:
+        status_at = whole("status", status, (1,), torch.int32, device)
+    beside = begin(device)
+    try:
         made = []
         if out is None or lse is None:
             make = torch.empty if counts is None else torch.zeros
@@ -140,27 +114,27 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
             if lse is None:
                 lse = make((batch, heads, nodes), dtype=torch.float32, device=q.device)
                 made.append(lse)
-            if launch.side is not None:  # zeros were written on torch's stream
-                launch.side.wait_stream(torch.cuda.current_stream())
-        out_strides = _element_rows("out", out, shape, dtype, device)
-        _whole("lse", lse, (batch, heads, nodes), torch.float32, device)
+            if beside is not None:  # zeros were written on torch's stream
+                beside.wait_for_torch()
+        out_strides = element_rows("out", out, shape, dtype, device)
+        lse_at = whole("lse", lse, (batch, heads, nodes), torch.float32, device)
         size = _attention_workspace(device, kind, batch, nodes, heads, kv_heads, d, capacity)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
             made.append(workspace)
             workspace_at = workspace.data_ptr()
-        args = _ATTENTION.pack(
-            q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), keys.data_ptr(), values.data_ptr(),
-            lengths.data_ptr(), parents_at, counts_at, out.data_ptr(), lse.data_ptr(), status_at,
-            workspace_at, size, kind, batch, nodes, heads, kv_heads, d, capacity,
-            *q_strides[:3], *k_strides[:3], *v_strides[:3], *keys_strides[:3],
-            *values_strides[:3], *out_strides[:3], parents_stride,
-            1.0 / math.sqrt(d) if scale is None else scale)
-        if runtime.library().ppyb200_tree_attention(args) != runtime.STATUS_OK:
+        if runtime.library().ppyb200_tree_attention(_ATTENTION.pack(
+                q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), keys.data_ptr(),
+                values.data_ptr(), lengths_at, parents_at, counts_at, out.data_ptr(), lse_at,
+                status_at, workspace_at, size, kind, batch, nodes, heads, kv_heads, d, capacity,
+                *q_strides[:3], *k_strides[:3], *v_strides[:3], *keys_strides[:3],
+                *values_strides[:3], *out_strides[:3], parents_stride,
+                1.0 / math.sqrt(d) if scale is None else scale)) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
-        if launch.side is not None:
-            for t in made:
-                t.record_stream(launch.side)
+        if beside is not None:
+            beside.record(*made)
+    finally:
+        end(beside)
     return out, lse
 
 
@@ -181,41 +155,43 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
     seen[b] + 1, ... (`seen` int32 [batch]: the tokens before them). lengths and seen are the
     caller's to advance. `status` as in tree_attention: raised when the path is not in order (it is
     cut there) or a length or count is out of range."""
-    torch = _torch()
-    kind, device = _kinds().get(keys.dtype), keys.get_device()
+    kind, device = _KINDS.get(keys.dtype), keys.get_device()
     _need(kind is not None and device >= 0 and keys.dim() == 5 and q.dim() == 5,
           "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim], q [layers, batch, "
           "nodes, heads, head_dim], on a CUDA device")
     layers, batch, kv_heads, capacity, d = keys.shape
     nodes, heads = q.shape[2], q.shape[3]
     steps = path.shape[-1]
-    q_strides = _element_rows("q", q, (layers, batch, nodes, heads, d), keys.dtype, device)
-    keys_strides = _element_rows("keys", keys, keys.shape, keys.dtype, device)
-    values_strides = _element_rows("values", values, keys.shape, keys.dtype, device)
+    q_strides = element_rows("q", q, (layers, batch, nodes, heads, d), keys.dtype, device)
+    keys_strides = element_rows("keys", keys, keys.shape, keys.dtype, device)
+    values_strides = element_rows("values", values, keys.shape, keys.dtype, device)
     if weights is not None:
-        _whole("lse", lse, (layers, batch, heads, nodes), torch.float32, device)
+        whole("lse", lse, (layers, batch, heads, nodes), torch.float32, device)
     for name, t in (("lengths", lengths), ("seen", seen), ("accepted", accepted)):
-        _whole(name, t, (batch,), torch.int32, device)
-    _whole("path", path, (batch, steps), torch.int32, device)
+        whole(name, t, (batch,), torch.int32, device)
+    whole("path", path, (batch, steps), torch.int32, device)
     tables = weights if weights is not None else positions
     strides = (0, 0, 0)
     for name, t, kept in (("weights", weights, torch.float32),
                           ("positions", positions, torch.int32)):
         if t is not None:
-            _element_rows(name, t, (layers, batch, kv_heads, capacity), kept, device)
+            element_rows(name, t, (layers, batch, kv_heads, capacity), kept, device)
             _need(t.stride() == tables.stride(), "weights and positions are laid out alike")
             strides = t.stride()[:3]
     if status is not None:
-        _whole("status", status, (1,), torch.int32, device)
-    with runtime.launches_beside_torch(device):
-        args = _ACCEPT.pack(
-            q.data_ptr(), lse.data_ptr(), keys.data_ptr(), values.data_ptr(), _address(weights),
-            _address(positions), lengths.data_ptr(), seen.data_ptr(), path.data_ptr(),
-            accepted.data_ptr(), _address(status), kind, layers, batch, nodes, steps, heads,
-            kv_heads, d, capacity, *q_strides[:4], *keys_strides[:4], *values_strides[:4],
-            *strides, 1.0 / math.sqrt(d) if scale is None else scale)
-        if runtime.library().ppyb200_accept(args) != runtime.STATUS_OK:
+        whole("status", status, (1,), torch.int32, device)
+    beside = begin(device)
+    try:
+        if runtime.library().ppyb200_accept(_ACCEPT.pack(
+                q.data_ptr(), lse.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                _address(weights), _address(positions), lengths.data_ptr(), seen.data_ptr(),
+                path.data_ptr(), accepted.data_ptr(), _address(status), kind, layers, batch, nodes,
+                steps, heads, kv_heads, d, capacity, *q_strides[:4], *keys_strides[:4],
+                *values_strides[:4], *strides,
+                1.0 / math.sqrt(d) if scale is None else scale)) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
+    finally:
+        end(beside)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -238,51 +214,48 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
     afterwards. The kept entries' weights and positions go to weights_out and positions_out
     [layers, batch, kv_heads, at least budget], the tables themselves by default. Sequences of up to `budget` entries
     keep them all. lengths are the caller's to set to min(lengths, budget)."""
-    torch = _torch()
     device = keys.get_device()
-    _need(keys.dtype in _kinds() and device >= 0 and keys.dim() == 5,
+    _need(keys.dtype in _KINDS and device >= 0 and keys.dim() == 5,
           "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim] on a CUDA device")
     layers, batch, kv_heads, capacity, d = keys.shape
     budget, recent = int(budget), int(recent)
     _need(0 < budget <= capacity and recent >= 0,
           "a budget of 1 up to the capacity, and recent not negative")
-    keys_strides = _element_rows("keys", keys, keys.shape, keys.dtype, device)
-    values_strides = _element_rows("values", values, keys.shape, keys.dtype, device)
-    _element_rows("weights", weights, (layers, batch, kv_heads, capacity), torch.float32, device)
-    _element_rows("positions", positions, (layers, batch, kv_heads, capacity), torch.int32,
-                  device)
-    _need(weights.stride() == positions.stride(), "weights and positions are laid out alike")
+    keys_strides = element_rows("keys", keys, keys.shape, keys.dtype, device)
+    values_strides = element_rows("values", values, keys.shape, keys.dtype, device)
+    table = (layers, batch, kv_heads, capacity)
+    weights_strides = element_rows("weights", weights, table, torch.float32, device)
+    _need(element_rows("positions", positions, table, torch.int32, device) == weights_strides,
+          "weights and positions are laid out alike")
     weights_out = weights if weights_out is None else weights_out
     positions_out = positions if positions_out is None else positions_out
     width = weights_out.shape[-1]
     _need(width >= budget, "weights_out: at least budget entries a head")
-    _element_rows("weights_out", weights_out, (layers, batch, kv_heads, width), torch.float32,
-                  device)
-    _element_rows("positions_out", positions_out, (layers, batch, kv_heads, width), torch.int32,
-                  device)
-    _need(weights_out.stride() == positions_out.stride(),
+    table = (layers, batch, kv_heads, width)
+    out_strides = element_rows("weights_out", weights_out, table, torch.float32, device)
+    _need(element_rows("positions_out", positions_out, table, torch.int32, device) == out_strides,
           "weights_out and positions_out are laid out alike")
     for name, t in (("lengths", lengths), ("seen", seen)):
-        _whole(name, t, (batch,), torch.int32, device)
+        whole(name, t, (batch,), torch.int32, device)
     if status is not None:
-        _whole("status", status, (1,), torch.int32, device)
-    with runtime.launches_beside_torch(device) as launch:
-        kept = torch.empty((layers, batch, kv_heads, budget), dtype=torch.int32,
-                           device=keys.device)
+        whole("status", status, (1,), torch.int32, device)
+    beside = begin(device)
+    try:
+        kept = lengths.new_empty((layers, batch, kv_heads, budget))
         size = _evict_workspace(layers, batch, kv_heads, d, capacity, budget)
-        workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=keys.device)
-        if launch.side is not None:
-            kept.record_stream(launch.side)
-            workspace.record_stream(launch.side)
-        args = _EVICT.pack(
-            keys.data_ptr(), values.data_ptr(), weights.data_ptr(), positions.data_ptr(),
-            weights_out.data_ptr(), positions_out.data_ptr(), kept.data_ptr(),
-            lengths.data_ptr(), seen.data_ptr(), _address(status), workspace.data_ptr(),
-            workspace.numel(), layers, batch, kv_heads, d, capacity, budget, recent,
-            *keys_strides[:4], *values_strides[:4], *weights.stride()[:3],
-            *weights_out.stride()[:3])
-        if runtime.library().ppyb200_evict(args) != runtime.STATUS_OK:
+        workspace = lengths.new_empty(max(size // 4, 4))
+        if beside is not None:
+            beside.record(kept, workspace)
+        if runtime.library().ppyb200_evict(_EVICT.pack(
+                keys.data_ptr(), values.data_ptr(), weights.data_ptr(), positions.data_ptr(),
+                weights_out.data_ptr(), positions_out.data_ptr(), kept.data_ptr(),
+                lengths.data_ptr(), seen.data_ptr(), _address(status), workspace.data_ptr(),
+                workspace.numel() * 4, layers, batch, kv_heads, d, capacity, budget, recent,
+                *keys_strides[:4], *values_strides[:4], *weights_strides[:3],
+                *out_strides[:3])) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
+    finally:
+        end(beside)
     return kept
 
 
@@ -300,10 +273,8 @@ class KVCache:
     query heads, head_dim] and log-sum-exps f32 [layers, batch, query heads, nodes]."""
 
     def __init__(self, layers: int, batch: int, heads: int, head_dim: int, capacity: int,
-                 dtype=None, device="cuda", weights: bool = True) -> None:
-        torch = _torch()
-        dtype = torch.bfloat16 if dtype is None else dtype
-        _need(dtype in _kinds(), "a cache of bf16 or f16")
+                 dtype=torch.bfloat16, device="cuda", weights: bool = True) -> None:
+        _need(dtype in _KINDS, "a cache of bf16 or f16")
         shape = (layers, batch, heads, capacity)
         self.keys = torch.zeros(*shape, head_dim, dtype=dtype, device=device)
         self.values = torch.zeros_like(self.keys)
@@ -337,7 +308,6 @@ class KVCache:
         [batch], as `accept_nodes`; all nodes without a path, each sequence's first accepted[b]
         of them) join the cache: lengths and seen grow by `accepted`. Paths longer than
         accept_nodes takes go in pieces."""
-        torch = _torch()
         _need(self.pending is not None, "accept follows an extension")
         q, lse = self.pending
         batch, nodes, heads = q.shape[1], q.shape[2], q.shape[3]

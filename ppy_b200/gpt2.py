@@ -27,7 +27,7 @@ import ctypes
 from dataclasses import dataclass
 from pathlib import Path
 
-from . import decode, runtime, scoring
+from . import decode, runtime, scoring, torch_calls
 
 __all__ = ["Config", "GPT2", "GPT2_124M", "GraphedForward"]
 
@@ -241,11 +241,11 @@ class GPT2:
         stride = 0
         if parents is not None:
             shared = parents.dim() == 1
-            decode._whole("parents", parents, (nodes,) if shared else (batch, nodes),
+            torch_calls.whole("parents", parents, (nodes,) if shared else (batch, nodes),
                           torch.int32, ids.get_device())
             stride = 0 if shared else nodes
         if counts is not None:
-            decode._whole("counts", counts, (batch,), torch.int32, ids.get_device())
+            torch_calls.whole("counts", counts, (batch,), torch.int32, ids.get_device())
         s = cache.buffers.get((batch, nodes))
         if s is None:
             d = ids.device
@@ -264,10 +264,10 @@ class GPT2:
         pitch = self._row_pitch(logits, batch, nodes, v)
         ln = self.layernorm.device.layernorm_bf16
         heads = (batch, nodes, 3, cfg.heads, cfg.head_dim)
-        with runtime.launches_beside_torch(ids.device.index) as launch:
-            if launch.side is not None:
-                logits.record_stream(launch.side)
-                ids.record_stream(launch.side)
+        beside = torch_calls.begin(ids.get_device())
+        try:
+            if beside is not None:
+                beside.record(logits, ids)
             st = cache.status.data_ptr()
             self._check(lib.ppyb200_gpt2_embed_tree(
                 ids.data_ptr(), parents.data_ptr() if parents is not None else None, stride,
@@ -299,6 +299,8 @@ class GPT2:
             self._check(lib.ppyb200_matmul_bf16_kmajor_ld(h.data_ptr(), self.wte.data_ptr(), None,
                                                           logits.data_ptr(), pitch, tokens, v, c),
                         "lm head")
+        finally:
+            torch_calls.end(beside)
         # without weights one layer's queries stand for all: `accept` only moves rows then
         queries = s["qkv"].view(-1, *heads)[:, :, :, 0]
         lse = s["lse"]

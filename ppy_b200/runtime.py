@@ -117,49 +117,6 @@ def set_stream(stream) -> None:
     library().ppyb200_set_stream(ctypes.c_void_p(handle or _LEGACY_STREAM))
 
 
-class launches_beside_torch:
-    """Context of a call that launches on this thread's stream (set_stream) with torch tensors
-    of device `index`: the thread's device has to be theirs (a thread without one is bound to
-    it), and is the current one inside. Where torch's current stream is another than the
-    thread's, the call waits for the work already on torch's stream and torch's stream for the
-    call's, so the tensors are the caller's to use as if the call had run on it; `side` is the
-    thread's stream then, for tensors made inside (record_stream), else None."""
-
-    __slots__ = ("_guard", "_index", "side")
-
-    def __init__(self, index: int) -> None:
-        import torch
-
-        lib = library()
-        bound = lib.ppyb200_current_device()
-        self._guard = self.side = None
-        self._index = index
-        if bound != index and bound >= 0:
-            raise B200Error(f"tensors on cuda:{index}, but this thread's device is {bound} "
-                            "(runtime.init)")
-        if torch._C._cuda_getDevice() != index:
-            self._guard = torch.cuda.device(index)
-            self._guard.__enter__()
-        if bound < 0:
-            init(index)
-        handle = lib.ppyb200_stream() or 0
-        if handle != (torch._C._cuda_getCurrentRawStream(index) or _LEGACY_STREAM):
-            self.side = (torch.cuda.default_stream(index) if handle == _LEGACY_STREAM
-                         else torch.cuda.ExternalStream(handle, index))
-            self.side.wait_stream(torch.cuda.current_stream(index))
-
-    def __enter__(self) -> "launches_beside_torch":
-        return self
-
-    def __exit__(self, *exc) -> None:
-        if self.side is not None:
-            import torch
-
-            torch.cuda.current_stream(self._index).wait_stream(self.side)
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-
-
 def device_allocations() -> int:
     """cudaMalloc calls the runtime library has made since it loaded."""
     return int(library().ppyb200_device_allocations())

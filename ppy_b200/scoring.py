@@ -6,11 +6,13 @@ f16."""
 
 from __future__ import annotations
 
-import functools
 from typing import NamedTuple
+
+import torch
 
 from . import runtime
 from .runtime import B200Error
+from .torch_calls import begin, end
 
 __all__ = ["TokenLogprobs", "token_logprobs"]
 
@@ -27,11 +29,8 @@ class TokenLogprobs(NamedTuple):
     top_tokens: object
 
 
-@functools.cache
-def _kinds() -> dict:
-    import torch
-
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+#: Element types, as the header numbers them.
+_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _rows(shape, strides) -> tuple[int, int]:
@@ -57,9 +56,7 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     (-1 where none is asked for) gives NaN. Alternatives come largest first, the lowest index
     first among equals, NaN above every number. A logit of -inf has probability 0; a row with a NaN
     or +inf, or with nothing above -inf, has NaN log probabilities and entropy."""
-    import torch
-
-    kind, device = _kinds().get(logits.dtype), logits.get_device()
+    kind, device = _KINDS.get(logits.dtype), logits.get_device()
     shape = logits.shape
     if kind is None or device < 0 or len(shape) < 1 or shape[-1] < 1:
         raise B200Error("logits: f32, bf16 or f16 [..., vocab] on a CUDA device")
@@ -77,19 +74,19 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
                         f"on {logits.device}")
     if not 0 <= top <= min(TOP_LIMIT, vocab):
         raise B200Error(f"top: 0 up to {TOP_LIMIT} and the vocabulary")
-    with runtime.launches_beside_torch(device) as launch:
-        place, f32 = logits.device, torch.float32
+    beside = begin(device)
+    try:
+        logprobs = torch.empty(asked, dtype=torch.float32, device=logits.device)
         result = TokenLogprobs(
-            torch.empty(asked, dtype=f32, device=place),
-            torch.empty(leading, dtype=f32, device=place),
-            torch.empty((*leading, top), dtype=f32, device=place),
-            torch.empty((*leading, top), dtype=torch.int64, device=place))
-        if launch.side is not None:
-            for t in result:
-                t.record_stream(launch.side)
+            logprobs, logprobs.new_empty(leading) if several else torch.empty_like(logprobs),
+            logprobs.new_empty((*leading, top)), tokens.new_empty((*leading, top)))
+        if beside is not None:
+            beside.record(*result)
         if runtime.library().ppyb200_token_logprobs(
                 logits.data_ptr(), kind, rows, vocab, pitch, tokens.data_ptr(),
-                asked[-1] if several else 1, top, result[0].data_ptr(), result[1].data_ptr(),
+                asked[-1] if several else 1, top, logprobs.data_ptr(), result[1].data_ptr(),
                 result[2].data_ptr(), result[3].data_ptr()) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
+    finally:
+        end(beside)
     return result

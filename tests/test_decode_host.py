@@ -6,9 +6,9 @@ import ctypes
 
 import pytest
 
-from ppy_b200 import decode, runtime, scoring
-
 torch = pytest.importorskip("torch")
+
+from ppy_b200 import decode, runtime, scoring, torch_calls  # noqa: E402
 
 ATTENTION = ("q k_new v_new keys values lengths parents counts out lse status workspace "
              "workspace_bytes dtype batch nodes heads kv_heads head_dim capacity").split()
@@ -137,14 +137,14 @@ def test_operators_refuse_host_tensors_and_wrong_types():
 def test_argument_checks_name_the_tensor():
     x = torch.zeros(2, 3, 8, dtype=torch.bfloat16)
     on = x.get_device()  # -1: host memory
-    assert decode._element_rows("x", x.transpose(0, 1), (3, 2, 8), torch.bfloat16, on) == (8, 24, 1)
+    assert torch_calls.element_rows("x", x.transpose(0, 1), (3, 2, 8), torch.bfloat16, on) == (8, 24, 1)
     for bad in (x.transpose(1, 2), x.float(), x[:1]):
         with pytest.raises(runtime.B200Error, match="x:"):
-            decode._element_rows("x", bad, (2, 3, 8), torch.bfloat16, on)
+            torch_calls.element_rows("x", bad, (2, 3, 8), torch.bfloat16, on)
     with pytest.raises(runtime.B200Error, match="x:"):
-        decode._element_rows("x", x, (2, 3, 8), torch.bfloat16, 0)
+        torch_calls.element_rows("x", x, (2, 3, 8), torch.bfloat16, 0)
     with pytest.raises(runtime.B200Error, match="n:"):
-        decode._whole("n", torch.zeros(4, dtype=torch.int32)[::2], (2,), torch.int32, on)
+        torch_calls.whole("n", torch.zeros(4, dtype=torch.int32)[::2], (2,), torch.int32, on)
 
 
 def test_logits_rows_layout():
