@@ -18,6 +18,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include <cooperative_groups.h>
 
 #include "../../include/ppyb200.h"
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) evict_select_kernel(const p
                                                                      const int64_t most,
                                                                      const int cached) {
   namespace cg = cooperative_groups;
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ SelectShared s;
   ppyb200::pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
@@ -391,6 +393,12 @@ __global__ void __launch_bounds__(kSelectThreads, 4) evict_select_kernel(const p
     return j - begin < in_cache ? keys[j - begin]
                                 : entry_key(weights[j], positions[j], protect_from);
   };
+  // four entries from j on, begin + a multiple of four
+  auto keys_of = [&](int j) {
+    if (j - begin + 3 < in_cache) return *reinterpret_cast<const uint4*>(keys + (j - begin));
+    return make_uint4(j < end ? key_of(j) : 0u, j + 1 < end ? key_of(j + 1) : 0u,
+                      j + 2 < end ? key_of(j + 2) : 0u, j + 3 < end ? key_of(j + 3) : 0u);
+  };
   if (tid < 4) s.counts[tid] = 0;
 
   uint32_t prefix = 0;
@@ -426,13 +434,18 @@ __global__ void __launch_bounds__(kSelectThreads, 4) evict_select_kernel(const p
         }
       }
     } else {
-#pragma unroll 2
-      for (int j0 = begin; j0 < end; j0 += kSelectThreads) {
-        const int j = j0 + tid;
-        const uint32_t key = j < end ? key_of(j) : 0u;
-        const bool counts = j < end && ((key ^ prefix) & known) == 0;
-        if (__any_sync(0xffffffffu, counts))
-          count_bins(mine, (key >> shift) & (uint32_t)(bins - 1), counts);
+#pragma unroll 1
+      for (int j0 = begin; j0 < end; j0 += 4 * kSelectThreads) {
+        const uint4 four = keys_of(j0 + 4 * tid);
+        const uint32_t key[4] = {four.x, four.y, four.z, four.w};
+        bool counts[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          counts[u] = j0 + 4 * tid + u < end && ((key[u] ^ prefix) & known) == 0;
+        if (__any_sync(0xffffffffu, counts[0] || counts[1] || counts[2] || counts[3]))
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            count_bins(mine, (key[u] >> shift) & (uint32_t)(bins - 1), counts[u]);
       }
     }
     sync_all();
@@ -504,13 +517,18 @@ __global__ void __launch_bounds__(kSelectThreads, 4) evict_select_kernel(const p
   {  // entries of this stretch above and equal to the threshold, before and behind the budget
     uint32_t more[4] = {0, 0, 0, 0};
 #pragma unroll 1
-    for (int j = begin + tid; j < end; j += kSelectThreads) {
-      const uint32_t key = key_of(j);
-      const bool above = key > threshold, same = key == threshold;
-      more[0] += above && j < budget ? 1 : 0;
-      more[1] += above && j >= budget ? 1 : 0;
-      more[2] += same && j < budget ? 1 : 0;
-      more[3] += same && j >= budget ? 1 : 0;
+    for (int j = begin + 4 * tid; j < end; j += 4 * kSelectThreads) {
+      const uint4 four = keys_of(j);
+      const uint32_t key[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool above = j + u < end && key[u] > threshold;
+        const bool same = j + u < end && key[u] == threshold, front = j + u < budget;
+        more[0] += above && front ? 1 : 0;
+        more[1] += above && !front ? 1 : 0;
+        more[2] += same && front ? 1 : 0;
+        more[3] += same && !front ? 1 : 0;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -545,103 +563,83 @@ __global__ void __launch_bounds__(kSelectThreads, 4) evict_select_kernel(const p
   // in most stretches all equal entries stay or all go, and their order does not matter
   const bool ordered = own_left != 0 && own_left != own_equal;
 
-  // Rows of kSelectThreads entries, eight at once: a warp's votes give an entry's place within
-  // its row and warp, the prefix sums over rows and warps the rest.
+  // Rows of kSelectThreads entries, eight at once, first those in front of the budget: a warp's
+  // votes give an entry's place within its row and warp, the prefix sums over rows and warps the
+  // rest.
   const unsigned below = (1u << lane) - 1u;
+  auto walk = [&](auto is_front, int from, int to, uint32_t* places, int32_t* list,
+                  uint32_t count) {
+    constexpr bool kFront = decltype(is_front)::value;
 #pragma unroll 1
-  for (int j0 = begin; j0 < end; j0 += kWalkRows * kSelectThreads) {
-    uint32_t key[kWalkRows];
-    float w[kWalkRows];
-    int32_t p[kWalkRows];
-    const bool front = j0 < budget, back = min(j0 + kWalkRows * kSelectThreads, end) > budget;
-#pragma unroll
-    for (int i = 0; i < kWalkRows; ++i) {
-      const int j = j0 + i * kSelectThreads + tid;
-      key[i] = j < end ? key_of(j) : 0u;
-      if (front && j < end && j < budget) {  // under way while the places are found
-        w[i] = weights[j];
-        p[i] = positions[j];
-      }
-    }
-    uint32_t keep = 0;  // a bit a row
-    if (ordered) {
+    for (int j0 = from; j0 < to; j0 += kWalkRows * kSelectThreads) {
+      uint32_t key[kWalkRows];
+      float w[kWalkRows];
+      int32_t p[kWalkRows];
 #pragma unroll
       for (int i = 0; i < kWalkRows; ++i) {
-        const bool same = j0 + i * kSelectThreads + tid < end && key[i] == threshold;
-        const unsigned votes = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) s.equal[i * kSelectWarps + warp] = __popc(votes);
+        const int j = j0 + i * kSelectThreads + tid;
+        key[i] = j < to ? key_of(j) : 0u;
+        if (kFront && j < to) {  // under way while the places are found
+          w[i] = weights[j];
+          p[i] = positions[j];
+        }
       }
+      uint32_t keep = 0;  // a bit a row
+      if (ordered) {
+#pragma unroll 1
+        for (int i = 0; i < kWalkRows; ++i) {
+          const bool same = j0 + i * kSelectThreads + tid < to && key_of(min(
+              j0 + i * kSelectThreads + tid, to - 1)) == threshold;
+          const unsigned votes = __ballot_sync(0xffffffffu, same);
+          if (lane == 0) s.equal[i * kSelectWarps + warp] = __popc(votes);
+        }
+        __syncthreads();
+        if (warp == 0) {
+          const uint32_t all = warp_prefix<kWalkParts / 32>(s.equal);
+          if (lane == 0) s.all[0] = all;
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < kWalkRows; ++i) {
+        const int j = j0 + i * kSelectThreads + tid;
+        const bool same = j < to && key[i] == threshold;
+        bool stays = j < to && (key[i] > threshold || (same && own_left != 0));
+        if (ordered) {
+          const unsigned votes = __ballot_sync(0xffffffffu, same);
+          if (same)
+            stays = equal_before + s.equal[i * kSelectWarps + warp] + __popc(votes & below) < need;
+        }
+        if (stays) keep |= 1u << i;
+        const unsigned moving = __ballot_sync(0xffffffffu, kFront ? j < to && !stays : stays);
+        if (lane == 0) places[i * kSelectWarps + warp] = __popc(moving);
+      }
+      if (ordered) equal_before += s.all[0];
       __syncthreads();
       if (warp == 0) {
-        const uint32_t all = warp_prefix<kWalkParts / 32>(s.equal);
-        if (lane == 0) s.all[0] = all;
+        const uint32_t all = warp_prefix<kWalkParts / 32>(places);
+        if (lane == 0) s.all[1] = all;
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < kWalkRows; ++i) {
         const int j = j0 + i * kSelectThreads + tid;
-        const bool same = j < end && key[i] == threshold;
-        const unsigned votes = __ballot_sync(0xffffffffu, same);
-        const uint32_t order =
-            equal_before + s.equal[i * kSelectWarps + warp] + __popc(votes & below);
-        if (j < end && (key[i] > threshold || (same && order < need))) keep |= 1u << i;
-      }
-      equal_before += s.all[0];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kWalkRows; ++i)
-        if (j0 + i * kSelectThreads + tid < end &&
-            (key[i] > threshold || (key[i] == threshold && own_left != 0)))
-          keep |= 1u << i;
-    }
-#pragma unroll
-    for (int i = 0; i < kWalkRows; ++i) {
-      const int j = j0 + i * kSelectThreads + tid;
-      const bool stays = ((keep >> i) & 1u) != 0;
-      if (front) {
-        const unsigned gone = __ballot_sync(0xffffffffu, j < end && j < budget && !stays);
-        if (lane == 0) s.holes[i * kSelectWarps + warp] = __popc(gone);
-      }
-      if (back) {
-        const unsigned late = __ballot_sync(0xffffffffu, j >= budget && stays);
-        if (lane == 0) s.sources[i * kSelectWarps + warp] = __popc(late);
-      }
-    }
-    __syncthreads();
-    if (warp == 0 && front) {
-      const uint32_t all = warp_prefix<kWalkParts / 32>(s.holes);
-      if (lane == 0) s.all[1] = all;
-    }
-    if (warp == 1 && back) {
-      const uint32_t all = warp_prefix<kWalkParts / 32>(s.sources);
-      if (lane == 0) s.all[2] = all;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWalkRows; ++i) {
-      const int j = j0 + i * kSelectThreads + tid;
-      const bool stays = ((keep >> i) & 1u) != 0;
-      if (front) {
-        const unsigned gone = __ballot_sync(0xffffffffu, j < end && j < budget && !stays);
-        if (j < end && j < budget) {
-          if (stays) {
-            kept[j] = j;
-            weights_out[j] = w[i];
-            positions_out[j] = p[i];
-          } else {
-            holes[hole_count + s.holes[i * kSelectWarps + warp] + __popc(gone & below)] = j;
-          }
+        const bool stays = ((keep >> i) & 1u) != 0;
+        const bool moves = kFront ? j < to && !stays : stays;
+        const unsigned votes = __ballot_sync(0xffffffffu, moves);
+        if (moves) list[count + places[i * kSelectWarps + warp] + __popc(votes & below)] = j;
+        if (kFront && stays) {
+          kept[j] = j;
+          weights_out[j] = w[i];
+          positions_out[j] = p[i];
         }
       }
-      if (back) {
-        const unsigned late = __ballot_sync(0xffffffffu, j >= budget && stays);
-        if (j >= budget && stays)
-          sources[source_count + s.sources[i * kSelectWarps + warp] + __popc(late & below)] = j;
-      }
+      count += s.all[1];
     }
-    if (front) hole_count += s.all[1];
-    if (back) source_count += s.all[2];
-  }
+  };
+  const int middle = min(end, max(begin, budget));
+  walk(std::true_type{}, begin, middle, s.holes, holes, hole_count);
+  walk(std::false_type{}, middle, end, s.sources, sources, source_count);
   if (rank == 0 && tid == 0) moves[head] = (int32_t)all_holes;
   sync_all();  // the lists are complete, and no CTA reads another's shared memory any more
   for (uint32_t r = first_thread; r < all_holes; r += step) {
@@ -717,7 +715,7 @@ cudaError_t launch_select(const ppyb200_evict_args& a, int64_t heads, int64_t mo
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)(heads * ranks));
   config.blockDim = dim3(kSelectThreads);
-  config.dynamicSmemBytes = (size_t)cached * 4;
+  config.dynamicSmemBytes = (size_t)(cached + 3) / 4 * 16;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeClusterDimension;

@@ -179,14 +179,21 @@ struct Walk {
   }
 };
 
-// The nodes whose first row lies in an item are appended by the segment that starts the item, by
-// `threads` threads of which this is the `thread`-th, four pieces in flight each.
+// The nodes whose first row lies in an item are appended by the segment that starts the item: nodes
+// [x, y), none where the segment does not.
+__device__ __forceinline__ int2 appended(const Deal& deal, const Segment& s) {
+  if (!s.starts) return make_int2(0, 0);
+  const int to = (s.row0 + deal.item_rows + deal.group - 1) / deal.group;
+  return make_int2((s.row0 + deal.group - 1) / deal.group, min(s.count, to));
+}
+
+// Appends them, by `threads` threads of which this is the `thread`-th, four pieces in flight each.
 template <class T>
 __device__ __forceinline__ void append(const Args& a, const Deal& deal, const Segment& s,
                                        int thread, int threads) {
-  if (!s.starts) return;
-  const int from = (s.row0 + deal.group - 1) / deal.group;
-  const int to = min(s.count, (s.row0 + deal.item_rows + deal.group - 1) / deal.group);
+  const int2 nodes = appended(deal, s);
+  const int from = nodes.x, to = nodes.y;
+  if (from >= to) return;
   const T* k_new = static_cast<const T*>(a.k_new) + s.b * a.k_new_strides[0] +
                    s.kvh * a.k_new_strides[2];
   const T* v_new = static_cast<const T*>(a.v_new) + s.b * a.v_new_strides[0] +

@@ -29,7 +29,7 @@
 //   warps 0-7  softmax (warpgroup t = stream t; warp w reads TMEM lanes 32 (w % 4) ...)
 //   warp 8     TMA loads of Q, K and V (a ring of K and V tiles in turn), by one thread
 //   warps 9,10 one thread each: the MMAs of stream 0 and 1; warp 9 owns the TMEM
-//   warp 11    appends a segment's nodes to the cache
+//   warp 11    appends a segment's nodes to the cache, unless they are many
 //
 // Every mbarrier wait is bounded: on giving up the CTA raises the status, every role leaves its
 // loop, copies and MMAs in flight are drained and the TMEM is freed.
@@ -74,6 +74,7 @@ static_assert(2 * 128 * kSoftmaxRegs + 128 * kSupportRegs <= kWideThreads * kLau
               "register split above the launch's registers");
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr float kMoveLog2 = 8.f;
+
 constexpr int kBox = 128 * 64 * 2;  // 128 rows of 64 16-bit columns: one TMA box
 
 template <int D>
@@ -288,6 +289,12 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
   auto cache_tiles_of = [&](const Segment& seg) {
     return (seg.length + kKeysTile - 1) / kKeysTile;
   };
+  // More nodes than warp 11 appends while a tile or two are walked: the softmax warps do it, while
+  // the segment's first loads are under way.
+  auto many_of = [&](const Segment& seg) {
+    const int2 nodes = appended(deal, seg);
+    return (nodes.y - nodes.x) * d > 4096;
+  };
   Segment seg;
 
   if (warp == 8) {
@@ -457,7 +464,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     while (walk.next(a, deal, seg)) {
       if (seg.starts && lane == 0)
         Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
-      append<T>(a, deal, seg, lane, 32);
+      if (!many_of(seg)) append<T>(a, deal, seg, lane, 32);
     }
   } else {
     softmax_registers();
@@ -485,11 +492,13 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     int turn = 0;         // tiles of shared segments so far
     bool ok = true;
     while (ok && walk.next(a, deal, seg)) {
+      if (many_of(seg)) append<T>(a, deal, seg, threadIdx.x, 256);
       const int mine = count_of(seg, t);
-      const bool turns = wide.share && both_of(seg);
+      const bool turns = Shape::kOver && wide.share && both_of(seg);
       const int cache_tiles = cache_tiles_of(seg);
       const int tile_row = (wide.share ? t * wide.tile_nodes * group : 0) + row;  // of the item
       const int node = (seg.row0 + tile_row) / group;
+      const int first_node = (seg.row0 + tile_row - row) / group;  // of the stream's rows
       const bool real = row < wide.tile_nodes * group && node < seg.count;
       const bool busy = __any_sync(0xffffffffu, real) != 0;  // the warp has rows
       // the loader's, there before the first node tile's keys
@@ -508,7 +517,10 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         const int tile = seg.first + index_of(t, k);
         const bool own = tile >= cache_tiles;
         const int left = own ? 0 : seg.length - tile * kKeysTile;
-        const bool ragged = own || left < kKeysTile;
+        // a chain's node tiles before the stream's first node are seen whole
+        const bool ragged =
+            own ? a.parents != nullptr || (tile - cache_tiles + 1) * kKeysTile > first_node + 1
+                : left < kKeysTile;
         if (busy) {
           float sv[kSpan];
 #pragma unroll

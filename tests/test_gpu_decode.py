@@ -139,6 +139,11 @@ class Inputs:
     ((9,), 256, 2, 1, 64, BF16, "heads", True),        # the largest tree
     ((40,), 300, 1, 1, 72, BF16, "heads", False),      # a chain longer than that
     ((5000,), 3, 2, 1, 8, BF16, "heads", True),        # the smallest head size, many splits
+    ((90, 33), 2, 160, 1, 64, BF16, "heads", True),    # more query heads a key head than a tile
+    ((150, 0, 260), 3, 100, 1, 64, F16, "tokens", True),   # one node a tile of rows
+    (tuple(range(0, 700, 10)), 1, 4, 2, 64, BF16, "heads", False),  # 70 sequences
+    (tuple(range(5, 705, 10)), 40, 2, 1, 128, F16, "tokens", True),
+    ((3000, 9000), 1, 64, 8, 128, BF16, "tokens", False),  # a large cache, few rows
 ])
 def test_tree_attention(lengths, nodes, heads, kv, d, dtype, layout, tree):
     x = Inputs(lengths, nodes, heads, kv, d, dtype, layout, tree)
@@ -471,6 +476,10 @@ def _check_evict(s, done, kept, budget, recent):
     (1, (5000,), 1, 80, 5000, 4999, 0, BF16),     # one goes
     (1, (4097, 2049), 2, 64, 4100, 1, 0, BF16),   # one stays
     (1, (700,), 2, 64, 700, 300, 700, BF16),      # everything protected: the lowest slots stay
+    (1, (40000, 39001), 1, 8, 40000, 30000, 100, BF16),  # several CTAs a head, a tie to cut
+    (2, (20000,), 2, 8, 20001, 3000, 0, F16),
+    (1, (150000,), 1, 8, 150000, 60000, 7, BF16),  # more entries than shared memory holds
+    (300, (900, 512), 1, 8, 900, 511, 9, BF16),    # many heads
 ])
 def test_evict(layers, lengths, kv, d, cap, budget, recent, dtype):
     from ppy_b200 import decode
