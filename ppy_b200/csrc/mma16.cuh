@@ -2,7 +2,8 @@
 // fragments (mma.sync), fragment loads from shared memory (ldmatrix) and asynchronous 16-byte
 // copies into it (cp.async). The decoding kernels read each cached key and value once for a
 // few query rows, so they are bound by memory and not by the tensor pipe; fragments of 16 rows
-// fit such few rows, where a tcgen05 tile has 128.
+// fit such few rows, where a tcgen05 tile has 128. Their products run at a small part of the tcgen05
+// rate (about 170 TFLOP/s over the whole GPU), so kernels with many rows have no use for them.
 //
 // Fragments of mma.m16n8k16 (lane = 4 gid + tig):
 //   A [16 x 16]: a0 (row gid, cols 2 tig, +1), a1 (row gid + 8), a2 (cols + 8), a3 (both)
@@ -14,6 +15,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 namespace ppyb200 {
 namespace mma16 {
@@ -97,6 +100,15 @@ __device__ __forceinline__ float exp2_sfu(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two 16-bit values, zero in the place of one that is not finite (its exponent bits all ones).
+template <class T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t kExponent = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  if ((w & kExponent) == kExponent) w &= 0xffff0000u;
+  if (((w >> 16) & kExponent) == kExponent) w &= 0x0000ffffu;
+  return w;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -12,8 +12,8 @@
 // The alternatives need no second pass over the row. The k-th largest of the threads' maxima is a
 // lower bound for the k-th largest logit, and only the threads whose own maximum reaches it (about
 // k of 256) hold candidates: their elements, just read, come from L2 again. The few candidates are
-// ranked by counting. Few rows are split over a cluster of CTAs each, whose
-// first joins the sums and the alternatives of the parts.
+// ranked by counting. Few rows are split over a cluster of CTAs each, whose first joins the sums
+// and the alternatives of the parts.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -305,7 +305,9 @@ __device__ __forceinline__ void find_best(Shared& s, const Row<T>& row, int inde
 
 // Eight CTAs an SM: a row's end (joins, the bound, the candidates) loads next to nothing, and the
 // other CTAs' rows keep the memory busy meanwhile (47 registers and five CTAs: 16384 rows of
-// GPT-2 logits 577 us, 32 registers 549).
+// GPT-2 logits in f32 577 us, 32 registers 546, 6.0 TB/s of one read). Prefetching the next vectors
+// into L2 made that 589. Rows of bf16 take as many exponentials for half the bytes: 1500 of
+// 32011, 96 MB, 40 us, 2.4 TB/s.
 template <class T>
 __global__ void __launch_bounds__(kThreads, 8)
 token_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t pitch,

@@ -68,7 +68,13 @@ __device__ __forceinline__ void write_row(const Args& a, int b, int node, int he
     a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
 }
 
-// Sixteen rows a CTA; the four warps take sixteen keys each of every tile and are joined at the end.
+// Sixteen rows a CTA; the four warps take sixteen keys each of every tile and are joined at the
+// end: splitting the keys and not the head dimension leaves each warp whole scores, so the warps
+// meet once an item. Each key and value is read once for up to 16 rows, and the few products cost
+// less than the loads: what bounds it is memory where the caches are large (64 sequences of up to
+// 1000 entries, 12 heads of 64: 170 MB in 55 us with the join, 3.1 TB/s; 525 MB at 4.6 TB/s), and
+// the chain of its steps where they are small (one sequence of 1000 entries: 9.6 us with the
+// join, of which the loads themselves would take half a microsecond).
 template <class T, int D>
 __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 4 : 2)
 narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
@@ -88,294 +94,302 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
   walk.enter(a, deal, blockIdx.x);
   Segment seg;
   while (walk.next(a, deal, seg)) {
-  const int b = seg.b, kvh = seg.kvh;
-  const int64_t length = seg.length, total = length + seg.count;
-  const int row0 = seg.row0, rows = seg.count * group;
-  const int64_t t0 = seg.first, t1 = t0 + seg.tiles;
-  __syncthreads();  // the last segment's shared memory has been read
+    const int b = seg.b, kvh = seg.kvh;
+    const int64_t length = seg.length, total = length + seg.count;
+    const int row0 = seg.row0, rows = seg.count * group;
+    const int64_t t0 = seg.first, t1 = t0 + seg.tiles;
+    __syncthreads();  // the last segment's shared memory has been read
 
-  const T* q = static_cast<const T*>(a.q) + b * a.q_strides[0];
-  const T* k_new = static_cast<const T*>(a.k_new) + b * a.k_new_strides[0] +
-                   kvh * a.k_new_strides[2];
-  const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
-                   kvh * a.v_new_strides[2];
-  const T* keys = static_cast<T*>(a.keys) + b * a.keys_strides[0] + kvh * a.keys_strides[1];
-  const T* values =
-      static_cast<T*>(a.values) + b * a.values_strides[0] + kvh * a.values_strides[1];
+    const T* q = static_cast<const T*>(a.q) + b * a.q_strides[0];
+    const T* k_new = static_cast<const T*>(a.k_new) + b * a.k_new_strides[0] +
+                     kvh * a.k_new_strides[2];
+    const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
+                     kvh * a.v_new_strides[2];
+    const T* keys = static_cast<T*>(a.keys) + b * a.keys_strides[0] + kvh * a.keys_strides[1];
+    const T* values =
+        static_cast<T*>(a.values) + b * a.values_strides[0] + kvh * a.values_strides[1];
 
-  const uint32_t base = shared_address(smem);
-  auto load_tile = [&](int64_t tile, int stage) {
-    const uint32_t ks = base + stage * 2 * kTileBytes, vs = ks + kTileBytes;
-    for (int i = tid; i < kTile * kPieces; i += kThreads) {
-      const int row = i / kPieces, piece = i % kPieces;
-      const int64_t j = tile * kTile + row;
-      const bool valid = j < total && piece * 8 < d;
-      const T *ksrc = keys, *vsrc = values;
-      if (valid) {
-        if (j < length) {
-          ksrc = keys + j * a.keys_strides[2] + piece * 8;
-          vsrc = values + j * a.values_strides[2] + piece * 8;
-        } else {
-          ksrc = k_new + (j - length) * a.k_new_strides[1] + piece * 8;
-          vsrc = v_new + (j - length) * a.v_new_strides[1] + piece * 8;
-        }
-      }
-      const uint32_t at = row_piece<D>(row, piece);
-      copy16(ks + at, ksrc, valid);
-      copy16(vs + at, vsrc, valid);
-    }
-  };
-
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (t0 + s < t1) load_tile(t0 + s, s);
-    copies_commit();
-  }
-
-  ppyb200::tree::append<T>(a, deal, seg, tid, kThreads);
-
-  if (seg.starts && tid == 0)
-    Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
-
-  // query fragments: the 16 rows, zero beyond the rows and the head size
-  const int ra = row0 + gid, rb = ra + 8;
-  uint32_t qf[D / 16][4];
-  {
-    const T* qa = ra < rows ? q + (ra / group) * a.q_strides[1] +
-                                  (int64_t)(kvh * group + ra % group) * a.q_strides[2] : nullptr;
-    const T* qb = rb < rows ? q + (rb / group) * a.q_strides[1] +
-                                  (int64_t)(kvh * group + rb % group) * a.q_strides[2] : nullptr;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const int c = s * 16 + tig * 2;
-      qf[s][0] = qa != nullptr && c < d ? *reinterpret_cast<const uint32_t*>(qa + c) : 0u;
-      qf[s][1] = qb != nullptr && c < d ? *reinterpret_cast<const uint32_t*>(qb + c) : 0u;
-      qf[s][2] = qa != nullptr && c + 8 < d ? *reinterpret_cast<const uint32_t*>(qa + c + 8) : 0u;
-      qf[s][3] = qb != nullptr && c + 8 < d ? *reinterpret_cast<const uint32_t*>(qb + c + 8) : 0u;
-    }
-  }
-
-  // ancestors of this tile's rows, where the CTA reads node slots of a tree
-  const bool tree = a.parents != nullptr;
-  if (tree && t1 * kTile > length) {
-    const int32_t* parents = a.parents + b * a.parents_stride;
-    for (int r = tid; r < kRows; r += kThreads) {
-#pragma unroll
-      for (int w = 0; w < kTreeWords; ++w) below[r][w] = 0;
-      if (row0 + r < rows) {
-        int i = (row0 + r) / group;
-        below[r][i >> 5] |= 1u << (i & 31);
-        for (;;) {
-          const int p = parents[i];
-          if (p < 0 || p >= i) {  // a root; an index that is no earlier node raises
-            if (p != -1) raise(a.status);
-            break;
+    const uint32_t base = shared_address(smem);
+    auto load_tile = [&](int64_t tile, int stage) {
+      const uint32_t ks = base + stage * 2 * kTileBytes, vs = ks + kTileBytes;
+      for (int i = tid; i < kTile * kPieces; i += kThreads) {
+        const int row = i / kPieces, piece = i % kPieces;
+        const int64_t j = tile * kTile + row;
+        const bool valid = j < total && piece * 8 < d;
+        const T *ksrc = keys, *vsrc = values;
+        if (valid) {
+          if (j < length) {
+            ksrc = keys + j * a.keys_strides[2] + piece * 8;
+            vsrc = values + j * a.values_strides[2] + piece * 8;
+          } else {
+            ksrc = k_new + (j - length) * a.k_new_strides[1] + piece * 8;
+            vsrc = v_new + (j - length) * a.v_new_strides[1] + piece * 8;
           }
-          i = p;
-          below[r][i >> 5] |= 1u << (i & 31);
         }
+        const uint32_t at = row_piece<D>(row, piece);
+        copy16(ks + at, ksrc, valid);
+        copy16(vs + at, vsrc, valid);
       }
-    }
-  }
-  if (tid == 0) spoiled = 0;
-
-  float o[D / 8][4];
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  const float scale = (float)a.scale * kLog2e;  // scores in powers of two
-
-  for (int64_t t = t0; t < t1; ++t) {
-    const int stage = (int)((t - t0) % kStages);
-    copies_wait<kStages - 2>();
-    __syncthreads();
-    if (t + kStages - 1 < t1) load_tile(t + kStages - 1, (int)((t - t0 + kStages - 1) % kStages));
-    copies_commit();
-    const uint32_t ks = base + stage * 2 * kTileBytes, vs = ks + kTileBytes;
-
-    // S = Q K^T: this warp's rows against its keys of the tile
-    float s[kKeys / 8][4];
-#pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      const int row = warp * kKeys + n * 8 + (lane & 7);
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {  // 32 columns: four 8 x 8 tiles
-        uint32_t kf[4];
-        load4(kf, ks + row_piece<D>(row, c * 4 + (lane >> 3)));
-        Kind<T>::mma(s[n], qf[2 * c], kf[0], kf[1]);
-        Kind<T>::mma(s[n], qf[2 * c + 1], kf[2], kf[3]);
-      }
-    }
-    const bool tail = (t + 1) * kTile > length;
-    if (tail) {
-      // values that are not finite must not meet the zero weights of rows that do not see
-      // them: zero them here, and add them below to the rows that do
-      for (int i = tid; i < kTile * D / 2; i += kThreads) {
-        const int row = i / (D / 2), word = i % (D / 2);
-        if (t * kTile + row < length) continue;
-        uint32_t* at = reinterpret_cast<uint32_t*>(smem + (vs - base) +
-                                                   row_piece<D>(row, word / 4) + (word % 4) * 4);
-        const float2 v = Kind<T>::unpack(*at);
-        if (!isfinite(v.x) || !isfinite(v.y)) {
-          *at = Kind<T>::pack(isfinite(v.x) ? v.x : 0.f, isfinite(v.y) ? v.y : 0.f);
-          atomicOr(&spoiled, 1ull << row);
-        }
-      }
-      __syncthreads();
-    }
-    auto sees = [&](int r, int64_t j) {  // row r (in the tile of rows) and slot j
-      if (j < length) return true;
-      if (j >= total || row0 + r >= rows) return false;
-      const int n = (int)(j - length);
-      return tree ? ((below[r][n >> 5] >> (n & 31)) & 1u) != 0 : n <= (row0 + r) / group;
     };
-    float x0 = m0, x1 = m1;
+
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n)
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (t0 + s < t1) load_tile(t0 + s, s);
+      copies_commit();
+    }
+
+    ppyb200::tree::append<T>(a, deal, seg, tid, kThreads);
+
+    if (seg.starts && tid == 0)
+      Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
+
+    // query fragments: the 16 rows, zero beyond the rows and the head size
+    const int ra = row0 + gid, rb = ra + 8;
+    uint32_t qf[D / 16][4];
+    {
+      const T* qa = ra < rows ? q + (ra / group) * a.q_strides[1] +
+                                    (int64_t)(kvh * group + ra % group) * a.q_strides[2] : nullptr;
+      const T* qb = rb < rows ? q + (rb / group) * a.q_strides[1] +
+                                    (int64_t)(kvh * group + rb % group) * a.q_strides[2] : nullptr;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[n][c] *= scale;
-        if (tail) {
-          const int64_t j = t * kTile + warp * kKeys + n * 8 + tig * 2 + (c & 1);
-          if (!sees(gid + (c >> 1) * 8, j)) s[n][c] = -INFINITY;
-        }
-        if (c < 2) x0 = fmaxf(x0, s[n][c]);
-        else x1 = fmaxf(x1, s[n][c]);
+      for (int s = 0; s < D / 16; ++s) {
+        const int c = s * 16 + tig * 2;
+        qf[s][0] = qa != nullptr && c < d ? *reinterpret_cast<const uint32_t*>(qa + c) : 0u;
+        qf[s][1] = qb != nullptr && c < d ? *reinterpret_cast<const uint32_t*>(qb + c) : 0u;
+        qf[s][2] = qa != nullptr && c + 8 < d ? *reinterpret_cast<const uint32_t*>(qa + c + 8) : 0u;
+        qf[s][3] = qb != nullptr && c + 8 < d ? *reinterpret_cast<const uint32_t*>(qb + c + 8) : 0u;
       }
+    }
+
+    // ancestors of this tile's rows, where the CTA reads node slots of a tree
+    const bool tree = a.parents != nullptr;
+    if (tree && t1 * kTile > length) {
+      const int32_t* parents = a.parents + b * a.parents_stride;
+      for (int r = tid; r < kRows; r += kThreads) {
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w) below[r][w] = 0;
+        if (row0 + r < rows) {
+          int i = (row0 + r) / group;
+          below[r][i >> 5] |= 1u << (i & 31);
+          for (;;) {
+            const int p = parents[i];
+            if (p < 0 || p >= i) {  // a root; an index that is no earlier node raises
+              if (p != -1) raise(a.status);
+              break;
+            }
+            i = p;
+            below[r][i >> 5] |= 1u << (i & 31);
+          }
+        }
+      }
+    }
+    if (tid == 0) spoiled = 0;
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    const float scale = (float)a.scale * kLog2e;  // scores in powers of two
+    // the last node that rows gid and gid + 8 may see
+    const int last0 = ra >= rows ? -1 : tree ? seg.count - 1 : ra / group;
+    const int last1 = rb >= rows ? -1 : tree ? seg.count - 1 : rb / group;
+
+    for (int64_t t = t0; t < t1; ++t) {
+      const int stage = (int)((t - t0) % kStages);
+      copies_wait<kStages - 2>();
+      __syncthreads();
+      if (t + kStages - 1 < t1) load_tile(t + kStages - 1, (int)((t - t0 + kStages - 1) % kStages));
+      copies_commit();
+      const uint32_t ks = base + stage * 2 * kTileBytes, vs = ks + kTileBytes;
+
+      // S = Q K^T: this warp's rows against its keys of the tile
+      float s[kKeys / 8][4];
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n) {
+        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        const int row = warp * kKeys + n * 8 + (lane & 7);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {  // 32 columns: four 8 x 8 tiles
+          uint32_t kf[4];
+          load4(kf, ks + row_piece<D>(row, c * 4 + (lane >> 3)));
+          Kind<T>::mma(s[n], qf[2 * c], kf[0], kf[1]);
+          Kind<T>::mma(s[n], qf[2 * c + 1], kf[2], kf[3]);
+        }
+      }
+      const bool tail = (t + 1) * kTile > length;
+      const int rel = (int)(t * kTile - length);  // the node of the tile's first slot, or negative
+      if (tail) {
+        // values that are not finite must not meet the zero weights of rows that do not see
+        // them: zero them here, and add them below to the rows that do
+        const int from = max(0, -rel) * kPieces, to = min(kTile, seg.count - rel) * kPieces;
+#pragma unroll 1
+        for (int i = from + tid; i < to; i += kThreads) {
+          const int row = i / kPieces;
+          uint4* at = reinterpret_cast<uint4*>(smem + (vs - base) + row_piece<D>(row, i % kPieces));
+          const uint4 v = *at;
+          const uint4 clean = make_uint4(finite_only<T>(v.x), finite_only<T>(v.y),
+                                         finite_only<T>(v.z), finite_only<T>(v.w));
+          if (clean.x != v.x || clean.y != v.y || clean.z != v.z || clean.w != v.w) {
+            *at = clean;
+            atomicOr(&spoiled, 1ull << row);
+          }
+        }
+        __syncthreads();
+      }
+      // whether row gid (half 0) or gid + 8 (half 1) sees node n; a chain's rows see those up to
+      // their own, and every row the cache's entries (n < 0)
+      auto sees = [&](int half, int n) {
+        const int last = half == 0 ? last0 : last1;
+        if (!tree || n < 0) return n <= last;
+        return n <= last && ((below[gid + 8 * half][n >> 5] >> (n & 31)) & 1u) != 0;
+      };
+      float x0 = m0, x1 = m1;
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          s[n][c] *= scale;
+          if (tail) {
+            if (!sees(c >> 1, rel + warp * kKeys + n * 8 + tig * 2 + (c & 1)))
+              s[n][c] = -INFINITY;
+          }
+          if (c < 2) x0 = fmaxf(x0, s[n][c]);
+          else x1 = fmaxf(x1, s[n][c]);
+        }
+#pragma unroll
+      for (int w = 1; w < 4; w <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, w));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, w));
+      }
+      // a row that has seen nothing yet keeps its maximum at -inf; its terms are 2^-inf = 0
+      const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
+      const float f0 = exp2_sfu(m0 - u0), f1 = exp2_sfu(m1 - u1);
+      m0 = x0;
+      m1 = x1;
+      l0 *= f0;
+      l1 *= f1;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][0] *= f0;
+        o[n][1] *= f0;
+        o[n][2] *= f1;
+        o[n][3] *= f1;
+      }
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n) {
+        s[n][0] = exp2_sfu(s[n][0] - u0);
+        s[n][1] = exp2_sfu(s[n][1] - u0);
+        s[n][2] = exp2_sfu(s[n][2] - u1);
+        s[n][3] = exp2_sfu(s[n][3] - u1);
+        l0 += s[n][0] + s[n][1];
+        l1 += s[n][2] + s[n][3];
+      }
+      // O += P V, P rounded to the values' type (half a step, 2^-9 or 2^-12 of each weight, as
+      // the prompt attention rounds it); the sum above takes the unrounded weights
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk) {
+        const uint32_t pf[4] = {
+            Kind<T>::pack(s[2 * kk][0], s[2 * kk][1]), Kind<T>::pack(s[2 * kk][2], s[2 * kk][3]),
+            Kind<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]),
+            Kind<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+        const int row = warp * kKeys + kk * 16 + (lane & 15);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {  // 16 columns: keys 0-7 and 8-15 of two 8-wide tiles
+          uint32_t vf[4];
+          load4_transposed(vf, vs + row_piece<D>(row, c * 2 + (lane >> 4)));
+          Kind<T>::mma(o[2 * c], pf, vf[0], vf[1]);
+          Kind<T>::mma(o[2 * c + 1], pf, vf[2], vf[3]);
+        }
+      }
+      if (tail && spoiled != 0) {
+#pragma unroll 1
+        for (int key = warp * kKeys; key < (warp + 1) * kKeys; ++key) {
+          if (((spoiled >> key) & 1ull) == 0) continue;
+          const T* v = v_new + (int64_t)(rel + key) * a.v_new_strides[1];
+          const bool see0 = sees(0, rel + key), see1 = sees(1, rel + key);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int col = n * 8 + tig * 2 + c;
+              if (col >= d) continue;
+              const float value = (float)v[col];
+              if (isfinite(value)) continue;
+              if (see0) o[n][c] += value;
+              if (see1) o[n][2 + c] += value;
+            }
+        }
+      }
+      if (tail) {
+        __syncthreads();
+        if (tid == 0) spoiled = 0;
+      }
+    }
+    copies_wait<0>();
 #pragma unroll
     for (int w = 1; w < 4; w <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, w));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, w));
+      l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, w);
     }
-    // a row that has seen nothing yet keeps its maximum at -inf; its terms are 2^-inf = 0
-    const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
-    const float f0 = exp2_sfu(m0 - u0), f1 = exp2_sfu(m1 - u1);
-    m0 = x0;
-    m1 = x1;
-    l0 *= f0;
-    l1 *= f1;
+
+    // join the warps in shared memory: [kWarps][kRows][D + 2]
+    float* box = reinterpret_cast<float*>(smem);
+    constexpr int kLine = D + 2;
+    __syncthreads();
+    float* mine = box + (warp * kRows + gid) * kLine;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      o[n][0] *= f0;
-      o[n][1] *= f0;
-      o[n][2] *= f1;
-      o[n][3] *= f1;
+      const int col = n * 8 + tig * 2;
+      *reinterpret_cast<float2*>(mine + col) = make_float2(o[n][0], o[n][1]);
+      *reinterpret_cast<float2*>(mine + 8 * kLine + col) = make_float2(o[n][2], o[n][3]);
     }
-#pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n) {
-      s[n][0] = exp2_sfu(s[n][0] - u0);
-      s[n][1] = exp2_sfu(s[n][1] - u0);
-      s[n][2] = exp2_sfu(s[n][2] - u1);
-      s[n][3] = exp2_sfu(s[n][3] - u1);
-      l0 += s[n][0] + s[n][1];
-      l1 += s[n][2] + s[n][3];
+    if (tig == 0) {
+      *reinterpret_cast<float2*>(mine + D) = make_float2(m0, l0);
+      *reinterpret_cast<float2*>(mine + 8 * kLine + D) = make_float2(m1, l1);
     }
-    // O += P V, P rounded to the values' type (half a step, 2^-9 or 2^-12 of each weight, as
-    // the prompt attention rounds it); the sum above takes the unrounded weights
+    __syncthreads();
+    // a warp a row at a time, a lane two columns of every 64
+    const Results results(a, deal, D);
+    for (int r = warp; r < kRows && row0 + r < rows; r += kWarps) {
+      float m = -INFINITY, l = 0.f, sum[D / 32];
 #pragma unroll
-    for (int kk = 0; kk < kKeys / 16; ++kk) {
-      const uint32_t pf[4] = {
-          Kind<T>::pack(s[2 * kk][0], s[2 * kk][1]), Kind<T>::pack(s[2 * kk][2], s[2 * kk][3]),
-          Kind<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]),
-          Kind<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3])};
-      const int row = warp * kKeys + kk * 16 + (lane & 15);
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, box[(w * kRows + r) * kLine + D]);
+      const float u = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {  // 16 columns: keys 0-7 and 8-15 of two 8-wide tiles
-        uint32_t vf[4];
-        load4_transposed(vf, vs + row_piece<D>(row, c * 2 + (lane >> 4)));
-        Kind<T>::mma(o[2 * c], pf, vf[0], vf[1]);
-        Kind<T>::mma(o[2 * c + 1], pf, vf[2], vf[3]);
+      for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float* from = box + (w * kRows + r) * kLine;
+        const float f = exp2_sfu(from[D] - u);
+        l += f * from[D + 1];
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const float2 v = *reinterpret_cast<const float2*>(from + i * 64 + lane * 2);
+          sum[2 * i] += f * v.x;
+          sum[2 * i + 1] += f * v.y;
+        }
+      }
+      const int node = (row0 + r) / group, head = kvh * group + (row0 + r) % group;
+      if (seg.whole) {
+        write_row<T, D>(a, b, node, head, lane, m, l, sum);
+      } else {
+        const int64_t at = results.at(seg.result, r);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+          *reinterpret_cast<float2*>(results.out + at * D + i * 64 + lane * 2) =
+              make_float2(sum[2 * i], sum[2 * i + 1]);
+        if (lane == 0) results.top[at] = make_float2(m, l);
       }
     }
-    if (tail && spoiled != 0) {
-      for (int key = warp * kKeys; key < (warp + 1) * kKeys; ++key) {
-        if (((spoiled >> key) & 1ull) == 0) continue;
-        const int64_t j = t * kTile + key;
-        const T* v = v_new + (j - length) * a.v_new_strides[1];
-        const bool see0 = sees(gid, j), see1 = sees(gid + 8, j);
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int col = n * 8 + tig * 2 + c;
-            if (col >= d) continue;
-            const float value = (float)v[col];
-            if (isfinite(value)) continue;
-            if (see0) o[n][c] += value;
-            if (see1) o[n][2 + c] += value;
-          }
-      }
-    }
-    if (tail) {
-      __syncthreads();
-      if (tid == 0) spoiled = 0;
-    }
-  }
-  copies_wait<0>();
-#pragma unroll
-  for (int w = 1; w < 4; w <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, w);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, w);
-  }
-
-  // join the warps in shared memory: [kWarps][kRows][D + 2]
-  float* box = reinterpret_cast<float*>(smem);
-  constexpr int kLine = D + 2;
-  __syncthreads();
-  float* mine = box + (warp * kRows + gid) * kLine;
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n) {
-    const int col = n * 8 + tig * 2;
-    *reinterpret_cast<float2*>(mine + col) = make_float2(o[n][0], o[n][1]);
-    *reinterpret_cast<float2*>(mine + 8 * kLine + col) = make_float2(o[n][2], o[n][3]);
-  }
-  if (tig == 0) {
-    *reinterpret_cast<float2*>(mine + D) = make_float2(m0, l0);
-    *reinterpret_cast<float2*>(mine + 8 * kLine + D) = make_float2(m1, l1);
-  }
-  __syncthreads();
-  // a warp a row at a time, a lane two columns of every 64
-  const Results results(a, deal, D);
-  for (int r = warp; r < kRows && row0 + r < rows; r += kWarps) {
-    float m = -INFINITY, l = 0.f, sum[D / 32];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, box[(w * kRows + r) * kLine + D]);
-    const float u = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float* from = box + (w * kRows + r) * kLine;
-      const float f = exp2_sfu(from[D] - u);
-      l += f * from[D + 1];
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const float2 v = *reinterpret_cast<const float2*>(from + i * 64 + lane * 2);
-        sum[2 * i] += f * v.x;
-        sum[2 * i + 1] += f * v.y;
-      }
-    }
-    const int node = (row0 + r) / group, head = kvh * group + (row0 + r) % group;
-    if (seg.whole) {
-      write_row<T, D>(a, b, node, head, lane, m, l, sum);
-    } else {
-      const int64_t at = results.at(seg.result, r);
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-        *reinterpret_cast<float2*>(results.out + at * D + i * 64 + lane * 2) =
-            make_float2(sum[2 * i], sum[2 * i + 1]);
-      if (lane == 0) results.top[at] = make_float2(m, l);
-    }
-  }
   }
 }
 
 // Joins the unnormalised results of an item's segments in their order, a warp a row. What it costs
 // is the latency of its loads one after another, so the outputs of the first eight results are
-// under way before the maxima are known.
+// under way before the maxima are known (3 us where an item has ten results, f32 traffic of a
+// few MB).
 template <class T, int D>
 __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ Args a,
                                                               const Deal deal) {
@@ -463,10 +477,11 @@ bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int64_t n2
     if (n[i] > 1 && (strides[i] <= 0 || strides[i] >= (1ll << 39))) return false;
   return true;
 }
+
 // Which kernel is the faster, by the bytes of a full cache (the lengths are on the device). The
 // narrow kernel starts and ends an item in about 2 us where the wide one takes 8 to 10, and
 // reads the cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.4. Measured,
-// wide against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 21.6 / 11.6,
+// wide against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 21.6 / 9.6,
 // 64 of 500 to 1000 (197 MB) 98.7 / 54.5; 4 rows, 8 heads of 128, 64 of 1000 to 2000 (525 MB)
 // 101 / 105, 16 of 2500 to 16001 (1.1 GB) 112 / 134; 64 rows, 12 heads of 64, 2 sequences (6.5 MB)
 // 27.9 / 25.6, 4 (13 MB) 31.3 / 32.0, 64 (209 MB) 183 / 247.
@@ -476,8 +491,10 @@ bool narrow_faster(const Args& a) {
   if (rows <= kRows) return item < (1 << 20) || cache < (256 << 20);
   return rows <= 4 * kRows && cache * ((rows + kRows - 1) / kRows) < (40 << 20);
 }
+
 bool wide_takes(const Args& a) {
-  return wide_fits(a) && !narrow_faster(a) && a.scale > 0 && strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
+  return wide_fits(a) && !narrow_faster(a) && a.scale > 0 &&
+         strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
          strides_fit(a.k_new_strides, a.batch, a.nodes, a.kv_heads) &&
          strides_fit(a.v_new_strides, a.batch, a.nodes, a.kv_heads) &&
          strides_fit(a.keys_strides, a.batch, a.kv_heads, a.capacity) &&

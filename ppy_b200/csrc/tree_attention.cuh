@@ -80,16 +80,21 @@ __device__ __forceinline__ int item_tiles(const Args& a, const Deal& deal, int l
 template <int TILE, bool APART>
 struct Walk {
   int64_t span, place;  // `place`: of the next tile, on the axis
+  int own;              // tiles of the lane-th item, for `enter`
   int left, offset, ctas, cta, kvh, item;
 
   // A warp together. Extents that are out of range raise `status`.
   __device__ __forceinline__ void measure(const Args& a, const Deal& deal, int32_t* status) {
     const int lane = threadIdx.x & 31, items = (int)a.batch * deal.items;
     span = 0;
+    own = 0;
+#pragma unroll 1
     for (int i = lane; i < items; i += 32) {
       int length, count;
       sequence_extent(a, i / deal.items, length, count, status);
-      span += item_tiles<TILE, APART>(a, deal, length, count, i % deal.items);
+      const int tiles = item_tiles<TILE, APART>(a, deal, length, count, i % deal.items);
+      if (i < 32) own = tiles;
+      span += tiles;
     }
 #pragma unroll
     for (int w = 16; w > 0; w >>= 1) span += __shfl_xor_sync(0xffffffffu, span, w);
@@ -124,9 +129,10 @@ struct Walk {
     left = (int)(start_of(a, c + 1) - start);
     kvh = (int)quotient(start, span);
     int64_t rest = start - kvh * span;
+#pragma unroll 1
     for (int i0 = 0; i0 < items; i0 += 32) {
-      int64_t tiles = 0;
-      if (i0 + lane < items) {
+      int64_t tiles = i0 == 0 ? own : 0;
+      if (i0 > 0 && i0 + lane < items) {
         int length, count;
         sequence_extent(a, (i0 + lane) / deal.items, length, count, nullptr);
         tiles = item_tiles<TILE, APART>(a, deal, length, count, (i0 + lane) % deal.items);

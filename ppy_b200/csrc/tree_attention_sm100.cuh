@@ -2,8 +2,9 @@
 // query heads that share the key head): tcgen05 products with TMEM accumulators, fed by TMA.
 //
 // A CTA an SM walks its share of the work (Walk): segments of key tiles (128 keys each: the cache's,
-// then the nodes' own) of one sequence and key head, with two streams, each a query tile of 128 rows with its own softmax warpgroup and
-// MMA issuer, so that one stream's products run while the other's softmax does:
+// then the nodes' own) of one sequence and key head, with two streams, each a query tile of 128
+// rows with its own softmax warpgroup and MMA issuer, so that one stream's products run while the
+// other's softmax does:
 //   rows > 128   the streams hold two row tiles and share every key tile (read once for 256 rows)
 //   rows <= 128  the streams hold the same rows and take the key tiles in turn
 //   rows <= 64   the same, and a query tile holds its rows twice (four times up to 32 rows): each
@@ -60,6 +61,7 @@ using gemm::mbar_try_wait;
 using gemm::tc_fence_after;
 using gemm::tc_fence_before;
 using mma16::exp2_sfu;
+using mma16::finite_only;
 using mma16::Kind;
 
 constexpr int kRowsTile = 128;  // rows a stream
@@ -188,15 +190,6 @@ template <class T, int D>
 constexpr uint32_t idesc_o() {  // B (the values) MN-major
   return (1u << 4) | type_bits<T>() | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
          ((uint32_t)(kRowsTile >> 4) << 24);
-}
-
-// Two 16-bit values, zero in the place of one that is not finite (its exponent bits all ones).
-template <class T>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-  constexpr uint32_t kExponent = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-  if ((w & kExponent) == kExponent) w &= 0xffff0000u;
-  if (((w >> 16) & kExponent) == kExponent) w &= 0x0000ffffu;
-  return w;
 }
 
 // Which keys of a tile a row sees, a bit each.
