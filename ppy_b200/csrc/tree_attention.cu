@@ -40,7 +40,7 @@ constexpr int kTile = 64;       // keys a tile
 constexpr int kStages = 3;      // tiles in flight
 constexpr int kRows = 16;       // rows a CTA
 constexpr int kWarps = 4;       // along a tile's keys
-constexpr int kJoinRows = 4;    // rows of an item that a CTA joins, a warp each
+constexpr int kJoinRows = 8;    // rows of an item that a CTA joins
 constexpr int kTreeWords = PPYB200_TREE_NODES / 32;
 
 // Shared memory rows of D elements: 16-byte pieces XORed with the row's low bits, so that the
@@ -375,27 +375,25 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
       if (seg.whole) {
         write_row<T, D>(a, b, node, head, lane, m, l, sum);
       } else {
-        const int64_t at = results.at(seg.result, r);
 #pragma unroll
         for (int i = 0; i < D / 64; ++i)
-          *reinterpret_cast<float2*>(results.out + at * D + i * 64 + lane * 2) =
-              make_float2(sum[2 * i], sum[2 * i + 1]);
-        if (lane == 0) results.top[at] = make_float2(m, l);
+          *reinterpret_cast<float2*>(results.out_of(seg.result, r, i * 16 + lane / 2) +
+                                     lane % 2 * 2) = make_float2(sum[2 * i], sum[2 * i + 1]);
+        if (lane == 0) results.top_of(seg.result, r) = make_float2(m, l);
       }
     }
   }
 }
 
-// Joins the unnormalised results of an item's segments in their order, a warp a row. What it costs
-// is the latency of its loads one after another, so the outputs of the first eight results are
-// under way before the maxima are known (3 us where an item has ten results, f32 traffic of a
-// few MB).
+// Joins the unnormalised results of an item's segments in their order, a thread four columns of a
+// row. What it costs is the latency of its loads one after another, so the outputs of the first
+// eight results are under way before the maxima are known.
 template <class T, int D>
-__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ Args a,
-                                                              const Deal deal) {
+__global__ void __launch_bounds__(kJoinRows * D / 4) join_kernel(const __grid_constant__ Args a,
+                                                                 const Deal deal) {
   ppyb200::pdl_wait();
-  const int number = blockIdx.x, lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
+  const int number = blockIdx.x, piece = threadIdx.x / kJoinRows;
+  const int r = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows;
   const int items = (int)a.batch * deal.items, kvh = number / items, item = number - kvh * items;
   const int b = item / deal.items, row = (item - b * deal.items) * deal.item_rows + r;
   const int node = row / deal.group;
@@ -406,52 +404,56 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
   if (r >= deal.item_rows || node >= count) return;
   if (deal.streams == 1 && ctas.x == ctas.y) return;  // whole: written by its CTA
   const int parts = (ctas.y - ctas.x + 1) * deal.streams;
-  // the first segment starts the item, the others continue it
-  auto place = [&](int i) {
-    const int c = ctas.x + i / deal.streams;
-    return results.at(Walk<kTile, false>::result_of(deal, c, number, c == ctas.x) +
-                          i % deal.streams, r);
-  };
+  int cta = ctas.x, stream = 0;  // of the next result
   constexpr int kBatch = 8;
-  float m = -INFINITY, l = 0.f, sum[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) sum[i] = 0.f;
+  float m = -INFINITY, l = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = 0; i0 < parts; i0 += kBatch) {
-    const int n = min(kBatch, parts - i0);
-    float2 v[kBatch][D / 64];
+    float4 v[kBatch];
+    float2 top[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
+    for (int i = 0; i < kBatch; ++i) {
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      top[i] = make_float2(-INFINITY, 0.f);
+      if (i0 + i < parts) {
+        // the first segment starts the item, the others continue it
+        const int64_t at =
+            Walk<kTile, false>::result_of(deal, cta, number, cta == ctas.x) + stream;
+        if (++stream == deal.streams) {
+          stream = 0;
+          ++cta;
+        }
+        v[i] = *reinterpret_cast<const float4*>(results.out_of(at, r, piece));
+        top[i] = results.top_of(at, r);
+      }
+    }
+    float most = m;
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k)
-        if (i < n)
-          v[i][k] = *reinterpret_cast<const float2*>(results.out + place(i0 + i) * D + k * 64 +
-                                                     lane * 2);
-    const float2 top = lane < n ? results.top[place(i0 + lane)] : make_float2(-INFINITY, 0.f);
-    float most = fmaxf(m, top.x);
-#pragma unroll
-    for (int w = 4; w > 0; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
-    most = __shfl_sync(0xffffffffu, most, 0);
+    for (int i = 0; i < kBatch; ++i) most = fmaxf(most, top[i].x);
     const float u = most == -INFINITY ? 0.f : most, f = exp2_sfu(m - u);
-    const float mine = exp2_sfu(top.x - u);
     m = most;
     l *= f;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) sum[k] *= f;
+    for (int k = 0; k < 4; ++k) sum[k] *= f;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const float g = __shfl_sync(0xffffffffu, mine, i);
-      const float z = __shfl_sync(0xffffffffu, top.y, i);
-      if (i < n) {
-        l += g * z;
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) {
-          sum[2 * k] += g * v[i][k].x;
-          sum[2 * k + 1] += g * v[i][k].y;
-        }
-      }
+      const float g = exp2_sfu(top[i].x - u);
+      l += g * top[i].y;
+      sum[0] += g * v[i].x;
+      sum[1] += g * v[i].y;
+      sum[2] += g * v[i].z;
+      sum[3] += g * v[i].w;
     }
   }
-  write_row<T, D>(a, b, node, kvh * deal.group + row % deal.group, lane, m, l, sum);
+  const int head = kvh * deal.group + row % deal.group;
+  const float inv = 1.f / l;
+  if (piece * 4 < a.head_dim) {
+    T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
+             (int64_t)head * a.out_strides[2] + piece * 4;
+    *reinterpret_cast<uint2*>(out) = make_uint2(Kind<T>::pack(sum[0] * inv, sum[1] * inv),
+                                                Kind<T>::pack(sum[2] * inv, sum[3] * inv));
+  }
+  if (piece == 0 && a.lse != nullptr)
+    a.lse[((int64_t)b * a.heads + head) * a.nodes + node] = (m + log2f(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- host
@@ -533,7 +535,7 @@ template <class T, int D>
 cudaError_t join(const Args& a, const Plan& p, cudaStream_t stream) {
   const dim3 grid((unsigned)(a.kv_heads * a.batch * p.deal.items),
                   (unsigned)((p.deal.item_rows + kJoinRows - 1) / kJoinRows));
-  return ppyb200::launch_pdl(join_kernel<T, D>, grid, dim3(32 * kJoinRows), 0, stream, a, p.deal);
+  return ppyb200::launch_pdl(join_kernel<T, D>, grid, dim3(kJoinRows * D / 4), 0, stream, a, p.deal);
 }
 
 template <class T, int D>

@@ -282,11 +282,12 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
   auto cache_tiles_of = [&](const Segment& seg) {
     return (seg.length + kKeysTile - 1) / kKeysTile;
   };
-  // More nodes than warp 11 appends while a tile or two are walked: the softmax warps do it, while
-  // the segment's first loads are under way.
+  // One warp appends 1024 elements of K and V in about a microsecond, while the others walk a tile.
+  // The softmax warps do more than that, while the segment's first loads are under way (64 nodes of
+  // 64: a microsecond there, and six by the one warp, which ended a short segment).
   auto many_of = [&](const Segment& seg) {
     const int2 nodes = appended(deal, seg);
-    return (nodes.y - nodes.x) * d > 4096;
+    return (nodes.y - nodes.x) * d > 1024;
   };
   Segment seg;
 
@@ -681,7 +682,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       }
       if (ok && busy) {
         const bool spoiled = mine > 0 && *(volatile int*)&s.spoiled[mark & 7] == mark;
-        const int64_t at = results.at(seg.result + (wide.share ? 0 : t * COPIES + key0 / kSpan), tile_row);
+        const int64_t result = seg.result + (wide.share ? 0 : t * COPIES + key0 / kSpan);
         const int head = seg.kvh * group + tile_row % group;
         const float inv = 1.f / l;
         T* out = static_cast<T*>(a.out) + seg.b * a.out_strides[0] + node * a.out_strides[1] +
@@ -727,7 +728,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           } else if (real) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(results.out + at * D + c * 32 + e) =
+              *reinterpret_cast<float4*>(results.out_of(result, tile_row, c * 8 + e / 4)) =
                   make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
@@ -737,7 +738,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
             a.lse[((int64_t)seg.b * a.heads + head) * a.nodes + node] =
                 (m_log2 + log2f(l)) * mma16::kLn2;
         } else if (real) {
-          results.top[at] = make_float2(m_log2, l);
+          results.top_of(result, tile_row) = make_float2(m_log2, l);
         }
       }
       __syncwarp();
