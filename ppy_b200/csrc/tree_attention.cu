@@ -481,17 +481,17 @@ bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int64_t n2
 }
 
 // Which kernel is the faster, by the bytes of a full cache (the lengths are on the device). The
-// narrow kernel starts and ends an item in about 2 us where the wide one takes 8 to 10, and
-// reads the cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.4. Measured,
-// wide against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 21.6 / 9.6,
-// 64 of 500 to 1000 (197 MB) 98.7 / 54.5; 4 rows, 8 heads of 128, 64 of 1000 to 2000 (525 MB)
-// 101 / 105, 16 of 2500 to 16001 (1.1 GB) 112 / 134; 64 rows, 12 heads of 64, 2 sequences (6.5 MB)
-// 27.9 / 25.6, 4 (13 MB) 31.3 / 32.0, 64 (209 MB) 183 / 247.
+// narrow kernel starts and ends an item in about 2 us where the wide one takes 6, and reads the
+// cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.4. Measured, wide
+// against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 20.1 / 10.2,
+// 64 of 750 (144 MB) 101.6 / 51.9; 4 rows, 8 heads of 128, 64 of 1500 (384 MB) 117.9 / 93.3, 16 of
+// 8000 (504 MB) 98.6 / 110.1; 32 rows, 12 heads of 64, 8 of 1000 (26 MB) 29.6 / 26.5; 64 rows,
+// 2 sequences (6 MB) 23.4 / 23.0, 4 (13 MB) 25.4 / 28.8, 64 (204 MB) 161 / 240.
 bool narrow_faster(const Args& a) {
   const int64_t rows = a.nodes * (a.heads / a.kv_heads), item = a.capacity * a.head_dim * 4;
-  const int64_t cache = a.batch * a.kv_heads * item;
-  if (rows <= kRows) return item < (1 << 20) || cache < (256 << 20);
-  return rows <= 4 * kRows && cache * ((rows + kRows - 1) / kRows) < (40 << 20);
+  const int64_t cache = a.batch * a.kv_heads * item, tiles = (rows + kRows - 1) / kRows;
+  if (tiles <= 1) return item < (1 << 20) || cache < (256 << 20);
+  return tiles <= 4 && cache * tiles * tiles < (160 << 20);
 }
 
 bool wide_takes(const Args& a) {

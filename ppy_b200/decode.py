@@ -75,8 +75,8 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
     are left as they were, zeros when made here). Node i is written to slot lengths[b] + i of keys
     and values; `lengths` stay as they are (`accept_nodes` says which nodes join).
 
-    bf16 or f16; head_dim a multiple of 8 up to 128; rows on 16-byte boundaries; up to 256 nodes with
-    parents. `status` (int32 [1], optional) is raised to 2 when a length, count or parent is out of
+    bf16 or f16; head_dim a multiple of 8 up to 128; rows on 16-byte boundaries; up to 256 nodes
+    with parents. `status` (int32 [1], optional) is raised to 2 when a length, count or parent is out of
     range: the call then keeps to the buffers, and takes such a parent for -1."""
     dtype, device = q.dtype, q.get_device()
     kind = _KINDS.get(dtype)
@@ -212,8 +212,8 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
     slot first among equals). Kept entries in slots below the budget stay where they are; those
     behind it move into the holes, both in ascending order, so slots are in no order of position
     afterwards. The kept entries' weights and positions go to weights_out and positions_out
-    [layers, batch, kv_heads, at least budget], the tables themselves by default. Sequences of up to `budget` entries
-    keep them all. lengths are the caller's to set to min(lengths, budget)."""
+    [layers, batch, kv_heads, at least budget], the tables themselves by default. Sequences of up
+    to `budget` entries keep them all. lengths are the caller's to set to min(lengths, budget)."""
     device = keys.get_device()
     _need(keys.dtype in _KINDS and device >= 0 and keys.dim() == 5,
           "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim] on a CUDA device")
