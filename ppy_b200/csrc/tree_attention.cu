@@ -73,7 +73,7 @@ __device__ __forceinline__ void write_row(const Args& a, int b, int node, int he
 // meet once an item. Each key and value is read once for up to 16 rows, and the few products cost
 // less than the loads: what bounds it is memory where the caches are large (64 sequences of up to
 // 1000 entries, 12 heads of 64: 170 MB in 55 us with the join, 3.1 TB/s; 525 MB at 4.6 TB/s), and
-// the chain of its steps where they are small (one sequence of 1000 entries: 9.6 us with the
+// the chain of its steps where they are small (one sequence of 1000 entries: 10 us with the
 // join, of which the loads themselves would take half a microsecond).
 template <class T, int D>
 __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 4 : 2)

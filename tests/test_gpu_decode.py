@@ -198,6 +198,40 @@ def test_tree_attention_hidden_values_that_are_not_finite():
             assert torch.equal(out[0, i, h][fine], clean[0, i, h][fine])
 
 
+@pytest.mark.parametrize("lengths,nodes,heads,kv,d,dtype,layout,tree,cap", [
+    ((4000, 129), 1, 8, 2, 64, BF16, "heads", False, 270_000),  # 4 rows: four copies of each
+    ((700, 0), 5, 6, 2, 128, F16, "heads", True, 140_000),      # 15 rows
+    ((2500, 128), 10, 6, 2, 64, BF16, "tokens", True, 50_000),  # 30 rows, groups of three
+    ((1111,), 12, 8, 2, 128, BF16, "heads", True, 60_000),      # 48 rows: two copies
+    ((1, 640), 64, 2, 2, 64, F16, "heads", True, 30_000),       # 64 rows
+    ((90, 1500), 20, 14, 2, 64, BF16, "heads", True, 2_000),    # groups of seven: 140 rows
+    ((300, 31), 45, 6, 2, 128, F16, "tokens", False, 2_000),    # 135 rows in two uneven tiles
+])
+def test_tree_attention_few_rows_over_a_large_cache(lengths, nodes, heads, kv, d, dtype, layout,
+                                                    tree, cap):
+    x = Inputs(lengths, nodes, heads, kv, d, dtype, layout, tree,
+               spare=cap - max(lengths) - nodes)
+    x.check(*x.call())
+
+
+@pytest.mark.parametrize("nodes,cap", [(12, 300_000), (30, 50_000), (64, 30_000)])
+def test_tree_attention_hidden_values_over_a_large_cache(nodes, cap):
+    """As above, for the kernel that large caches take: an infinity shows in the rows that see
+    it, and in no other."""
+    x = Inputs((70, 128), nodes, 4, 4, 64, seed=6, spare=cap - 128 - nodes)
+    clean, clean_lse = x.call()
+    x.v_new[1, 2, 1, 9] = math.inf
+    out, lse = x.call()
+    assert torch.equal(lse, clean_lse) and torch.equal(out[0], clean[0])
+    parents = x.parents[1].tolist()
+    for i in range(nodes):
+        hit = 2 in _ancestors(parents, i)
+        assert bool(out[1, i, 1, 9].isinf()) == hit
+        fine = torch.ones(4, 64, dtype=torch.bool, device="cuda")
+        fine[1, 9] = not hit
+        assert torch.equal(out[1, i][fine], clean[1, i][fine])
+
+
 def test_tree_attention_out_of_range_raises_status_and_keeps_to_the_buffers():
     x = Inputs((60, 20, 30), 4, 2, 2, 64, spare=0)  # a capacity of 64
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
