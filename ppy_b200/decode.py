@@ -105,15 +105,12 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
         status_at = whole("status", status, (1,), torch.int32, device)
     beside = begin(device)
     try:
-        made = []
         if out is None or lse is None:
             make = torch.empty if counts is None else torch.zeros
             if out is None:
                 out = make(shape, dtype=dtype, device=q.device)
-                made.append(out)
             if lse is None:
                 lse = make((batch, heads, nodes), dtype=torch.float32, device=q.device)
-                made.append(lse)
             if beside is not None:  # zeros were written on torch's stream
                 beside.wait_for_torch()
         out_strides = element_rows("out", out, shape, dtype, device)
@@ -121,7 +118,6 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
         size = _attention_workspace(device, kind, batch, nodes, heads, kv_heads, d, capacity)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-            made.append(workspace)
             workspace_at = workspace.data_ptr()
         if runtime.library().ppyb200_tree_attention(_ATTENTION.pack(
                 q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), keys.data_ptr(),
@@ -131,8 +127,6 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
                 *values_strides[:3], *out_strides[:3], parents_stride,
                 1.0 / math.sqrt(d) if scale is None else scale)) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
-        if beside is not None:
-            beside.record(*made)
     finally:
         end(beside)
     return out, lse
@@ -244,8 +238,6 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
         kept = lengths.new_empty((layers, batch, kv_heads, budget))
         size = _evict_workspace(layers, batch, kv_heads, d, capacity, budget)
         workspace = lengths.new_empty(max(size // 4, 4))
-        if beside is not None:
-            beside.record(kept, workspace)
         if runtime.library().ppyb200_evict(_EVICT.pack(
                 keys.data_ptr(), values.data_ptr(), weights.data_ptr(), positions.data_ptr(),
                 weights_out.data_ptr(), positions_out.data_ptr(), kept.data_ptr(),

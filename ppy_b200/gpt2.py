@@ -266,8 +266,6 @@ class GPT2:
         heads = (batch, nodes, 3, cfg.heads, cfg.head_dim)
         beside = torch_calls.begin(ids.get_device())
         try:
-            if beside is not None:
-                beside.record(logits, ids)
             st = cache.status.data_ptr()
             self._check(lib.ppyb200_gpt2_embed_tree(
                 ids.data_ptr(), parents.data_ptr() if parents is not None else None, stride,

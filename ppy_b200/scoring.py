@@ -76,12 +76,10 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
         raise B200Error(f"top: 0 up to {TOP_LIMIT} and the vocabulary")
     beside = begin(device)
     try:
-        logprobs = torch.empty(asked, dtype=torch.float32, device=logits.device)
+        logprobs = torch.empty_like(tokens, dtype=torch.float32)
         result = TokenLogprobs(
             logprobs, logprobs.new_empty(leading) if several else torch.empty_like(logprobs),
             logprobs.new_empty((*leading, top)), tokens.new_empty((*leading, top)))
-        if beside is not None:
-            beside.record(*result)
         if runtime.library().ppyb200_token_logprobs(
                 logits.data_ptr(), kind, rows, vocab, pitch, tokens.data_ptr(),
                 asked[-1] if several else 1, top, logprobs.data_ptr(), result[1].data_ptr(),

@@ -7,6 +7,9 @@ own current stream. A function that takes torch tensors brackets its launches wi
 
 from __future__ import annotations
 
+import functools
+import threading
+
 import torch
 
 from . import runtime
@@ -18,12 +21,32 @@ __all__ = ["Beside", "begin", "element_rows", "end", "whole"]
 # which costs as much as a launch
 _current_device = torch._C._cuda_getDevice
 _current_raw_stream = torch._C._cuda_getCurrentRawStream
+_external_stream = functools.lru_cache(maxsize=256)(torch.cuda.ExternalStream)
+
+
+class _Thread(threading.local):
+    def __init__(self) -> None:
+        self.events = {}  # an event of each device
+
+
+_thread = _Thread()
+
+
+def _order(index: int, before, after) -> None:
+    """What comes on `after` waits for what `before` holds by now. One event a thread and device:
+    a wait keeps to the record before it, so the next record may follow at once."""
+    event = _thread.events.get(index)
+    if event is None:
+        event = _thread.events[index] = torch.cuda.Event()
+    event.record(before)
+    after.wait_event(event)
 
 
 class Beside:
     """A call whose launches go to another stream than torch's current one, or to another device
-    than the current one. `side` is the stream when it is another: tensors made within the call
-    are recorded on it (`record`)."""
+    than the current one. `side` is the stream when it is another. Tensors made within the call
+    belong to torch's current stream, which is behind the launches from `end` on, so they need no
+    record on the side stream."""
 
     __slots__ = ("_guard", "_index", "side")
 
@@ -43,22 +66,17 @@ class Beside:
         current = torch.cuda.current_stream(index)
         if handle != (current.cuda_stream or runtime._LEGACY_STREAM):
             self.side = (torch.cuda.default_stream(index) if handle == runtime._LEGACY_STREAM
-                         else torch.cuda.ExternalStream(handle, index))
-            self.side.wait_stream(current)
+                         else _external_stream(handle, index))
+            _order(index, current, self.side)
 
     def wait_for_torch(self) -> None:
         """The launches that follow wait for what torch's stream holds by now."""
         if self.side is not None:
-            self.side.wait_stream(torch.cuda.current_stream(self._index))
-
-    def record(self, *tensors) -> None:
-        if self.side is not None:
-            for t in tensors:
-                t.record_stream(self.side)
+            _order(self._index, torch.cuda.current_stream(self._index), self.side)
 
     def end(self) -> None:
         if self.side is not None:
-            torch.cuda.current_stream(self._index).wait_stream(self.side)
+            _order(self._index, self.side, torch.cuda.current_stream(self._index))
         if self._guard is not None:
             self._guard.__exit__(None, None, None)
 

@@ -712,3 +712,42 @@ def test_gpt2_extends_in_a_graph():
         assert cache.lengths.tolist() == [34, 34]
     finally:
         runtime.set_stream(torch.cuda.current_stream())
+
+
+def test_calls_beside_torchs_stream_from_two_threads():
+    """Two threads, each with a torch stream of its own and the library's stream of the thread,
+    make and drop their tensors at once: results stay those of one call alone."""
+    import threading
+
+    from ppy_b200 import scoring
+
+    x = [Inputs((900, 300), 8, 4, 2, 64, seed=i, spare=40) for i in range(2)]
+    logits = [torch.randn(64, 5001, device="cuda",
+                          generator=torch.Generator(device="cuda").manual_seed(9 + i))
+              for i in range(2)]
+    tokens = torch.arange(64, device="cuda")
+    want = [(x[i].call(), scoring.token_logprobs(logits[i], tokens, 3)) for i in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(40):
+                    out, lse = x[i].call()
+                    scores = scoring.token_logprobs(logits[i] * 1.0, tokens, 3)
+                    junk = torch.full((64, 5001), math.nan, device="cuda")
+                    same = (torch.equal(out, want[i][0][0]) and torch.equal(lse, want[i][0][1])
+                            and all(torch.equal(a, b) for a, b in zip(scores, want[i][1])))
+                    del junk
+                    if not same:
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001 - reported below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
