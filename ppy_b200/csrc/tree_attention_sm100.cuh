@@ -282,9 +282,9 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
   auto cache_tiles_of = [&](const Segment& seg) {
     return (seg.length + kKeysTile - 1) / kKeysTile;
   };
-  // One warp appends 1024 elements of K and V in about a microsecond, while the others walk a tile.
-  // The softmax warps do more than that, while the segment's first loads are under way (64 nodes of
-  // 64: a microsecond there, and six by the one warp, which ended a short segment).
+  // Up to 1024 elements of K and V one warp appends (two rounds of loads and stores) while the others
+  // walk a tile. The softmax warps do more than that, while the segment's first loads are under way:
+  // 64 nodes of 64 took the one warp 6 us, past the end of a short segment.
   auto many_of = [&](const Segment& seg) {
     const int2 nodes = appended(deal, seg);
     return (nodes.y - nodes.x) * d > 1024;
