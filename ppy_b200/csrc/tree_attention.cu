@@ -22,6 +22,7 @@
 #include "mma16.cuh"
 #include "ppyb200_device.cuh"
 #include "tree_attention.cuh"
+#include "tree_attention_plan.cuh"
 #include "tree_attention_sm100.cuh"
 
 namespace {
@@ -29,16 +30,19 @@ namespace {
 using namespace ppyb200::mma16;
 using ppyb200::tree::Args;
 using ppyb200::tree::Deal;
+using ppyb200::tree::Plan;
 using ppyb200::tree::Results;
 using ppyb200::tree::Segment;
 using ppyb200::tree::Walk;
-using ppyb200::tree::WideRows;
+using ppyb200::tree::plan_for;
 using ppyb200::tree::raise;
 using ppyb200::tree::sequence_extent;
+using ppyb200::tree::wide_fits;
+using ppyb200::tree::wide_takes;
 
-constexpr int kTile = 64;       // keys a tile
+constexpr int kTile = ppyb200::tree::kNarrowTile;
+constexpr int kRows = ppyb200::tree::kNarrowRows;
 constexpr int kStages = 3;      // tiles in flight
-constexpr int kRows = 16;       // rows a CTA
 constexpr int kWarps = 4;       // along a tile's keys
 constexpr int kJoinRows = 8;    // rows of an item that a CTA joins
 constexpr int kTreeWords = PPYB200_TREE_NODES / 32;
@@ -140,7 +144,7 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
 
     ppyb200::tree::append<T>(a, deal, seg, tid, kThreads);
 
-    if (seg.starts && tid == 0)
+    if (deal.join && seg.starts && tid == 0)
       Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
 
     // query fragments: the 16 rows, zero beyond the rows and the head size
@@ -458,79 +462,6 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) join_kernel(const __grid_co
 
 // ---------------------------------------------------------------- host
 
-struct Plan {
-  bool wide;
-  WideRows rows;  // of the wide kernel
-  Deal deal;
-  bool join;  // some item may have several results
-  int64_t workspace;
-};
-
-int padded_dim(int64_t head_dim) { return head_dim <= 64 ? 64 : 128; }
-
-// What the tensor-core kernel takes: a positive scale (it keeps maxima of unscaled scores), query
-// heads a key head that fit a row tile, and tensors that tensor maps describe.
-bool wide_fits(const Args& a) {
-  return a.heads / a.kv_heads <= ppyb200::tree::kRowsTile && a.head_dim > 32;
-}
-bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int64_t n2) {
-  const int64_t n[3] = {n0, n1, n2};
-  for (int i = 0; i < 3; ++i)
-    if (n[i] > 1 && (strides[i] <= 0 || strides[i] >= (1ll << 39))) return false;
-  return true;
-}
-
-// Which kernel is the faster, by the bytes of a full cache (the lengths are on the device). The
-// narrow kernel starts and ends an item in about 2 us where the wide one takes 6, and reads the
-// cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.4. Measured, wide
-// against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 20.1 / 10.2,
-// 64 of 750 (144 MB) 101.6 / 51.9; 4 rows, 8 heads of 128, 64 of 1500 (384 MB) 117.9 / 93.3, 16 of
-// 8000 (504 MB) 98.6 / 110.1; 32 rows, 12 heads of 64, 8 of 1000 (26 MB) 29.6 / 26.5; 64 rows,
-// 2 sequences (6 MB) 23.4 / 23.0, 4 (13 MB) 25.4 / 28.8, 64 (204 MB) 161 / 240.
-bool narrow_faster(const Args& a) {
-  const int64_t rows = a.nodes * (a.heads / a.kv_heads), item = a.capacity * a.head_dim * 4;
-  const int64_t cache = a.batch * a.kv_heads * item, tiles = (rows + kRows - 1) / kRows;
-  if (tiles <= 1) return item < (1 << 20) || cache < (256 << 20);
-  return tiles <= 4 && cache * tiles * tiles < (160 << 20);
-}
-
-bool wide_takes(const Args& a) {
-  return wide_fits(a) && !narrow_faster(a) && a.scale > 0 &&
-         strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
-         strides_fit(a.k_new_strides, a.batch, a.nodes, a.kv_heads) &&
-         strides_fit(a.v_new_strides, a.batch, a.nodes, a.kv_heads) &&
-         strides_fit(a.keys_strides, a.batch, a.kv_heads, a.capacity) &&
-         strides_fit(a.values_strides, a.batch, a.kv_heads, a.capacity);
-}
-
-Plan plan_for(const Args& a, bool wide, int sm_count) {
-  Plan p = {};
-  p.wide = wide;
-  const int64_t group = a.heads / a.kv_heads, rows = a.nodes * group;
-  p.deal.group = (int)group;
-  p.deal.least = 2;
-  if (wide) {
-    p.rows = ppyb200::tree::wide_rows(a);
-    p.deal.streams = p.rows.share ? 1 : 2 * p.rows.copies;
-    p.deal.item_rows = (int)(p.rows.tile_nodes * group * (p.rows.share ? 2 : 1));
-    p.deal.grid = sm_count;
-  } else {
-    p.deal.streams = 1;
-    p.deal.item_rows = kRows;
-    p.deal.grid = sm_count * (a.head_dim <= 64 ? 4 : 2);
-  }
-  p.deal.items = (int)((rows + p.deal.item_rows - 1) / p.deal.item_rows);
-  // no more CTAs than a full cache has work for
-  const int64_t tile = wide ? ppyb200::tree::kKeysTile : kTile;
-  const int64_t work = a.batch * a.kv_heads * p.deal.items *
-                       ((a.capacity + tile - 1) / tile + (wide ? (a.nodes + tile - 1) / tile : 0));
-  const int64_t most = work / p.deal.least;
-  if (p.deal.grid > most) p.deal.grid = most < 1 ? 1 : (int)most;
-  p.join = p.deal.streams > 1 || p.deal.grid > 1;
-  p.workspace = p.join ? Results::bytes(a, p.deal, padded_dim(a.head_dim)) : 0;
-  return p;
-}
-
 template <class T, int D>
 cudaError_t join(const Args& a, const Plan& p, cudaStream_t stream) {
   const dim3 grid((unsigned)(a.kv_heads * a.batch * p.deal.items),
@@ -560,7 +491,7 @@ cudaError_t launch_dim(const Args& a, const Plan& p, cudaStream_t stream) {
                         : p.rows.copies == 4 ? launch_wide<T, D, 4>(a, p.deal, p.rows, stream)
                         : p.rows.copies == 2 ? launch_wide<T, D, 2>(a, p.deal, p.rows, stream)
                                              : launch_wide<T, D, 1>(a, p.deal, p.rows, stream);
-  return e == cudaSuccess && p.join ? join<T, D>(a, p, stream) : e;
+  return e == cudaSuccess && p.deal.join ? join<T, D>(a, p, stream) : e;
 }
 
 template <class T>
@@ -633,7 +564,7 @@ int32_t ppyb200_tree_attention(const ppyb200_tree_attention_args* args) {
   const cudaError_t e = a.dtype == PPYB200_BF16 ? launch_type<__nv_bfloat16>(a, p, stream)
                                                 : launch_type<__half>(a, p, stream);
   if (e != cudaSuccess) return ppyb200_check((int32_t)e, "ppyb200_tree_attention");
-  ppyb200_count_launches(p.join ? 2 : 1);
+  ppyb200_count_launches(p.deal.join ? 2 : 1);
   return PPYB200_OK;
 }
 

@@ -43,6 +43,7 @@ struct Deal {
   int item_rows;
   int group;      // query heads a key head
   int streams;    // results a segment leaves: several where streams or copies split its keys
+  bool join;      // results go through the workspace; without it there is none to write to
 };
 
 struct Segment {

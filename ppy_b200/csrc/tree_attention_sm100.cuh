@@ -48,6 +48,7 @@
 #include "mma16.cuh"
 #include "tmem.cuh"
 #include "tree_attention.cuh"
+#include "tree_attention_plan.cuh"
 
 namespace ppyb200 {
 namespace tree {
@@ -64,8 +65,6 @@ using mma16::exp2_sfu;
 using mma16::finite_only;
 using mma16::Kind;
 
-constexpr int kRowsTile = 128;  // rows a stream
-constexpr int kKeysTile = 128;  // keys a tile
 constexpr int kWideThreads = 384;
 // Registers a thread after the split (setmaxnreg): the softmax warpgroups hold a row of 128 scores
 // and take what the third warpgroup gives up. The launch holds kLaunchRegs x 384, and the split
@@ -135,12 +134,6 @@ struct Entry {
 // [heads][nodes][batch].
 struct WideMaps {
   CUtensorMap q, keys, values, k_new, v_new;
-};
-
-struct WideRows {
-  int tile_nodes;  // nodes of a row tile (tile_nodes x group <= 128 / copies)
-  bool share;      // two row tiles an item, sharing the key tiles; else two streams over the keys
-  int copies;      // of the rows in a query tile (1 when shared)
 };
 
 template <class Layout>
@@ -456,7 +449,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
     support_registers();
     // ---- append, and where the join finds an item's results
     while (walk.next(a, deal, seg)) {
-      if (seg.starts && lane == 0)
+      if (deal.join && seg.starts && lane == 0)
         Results(a, deal, D).ctas[seg.number] = make_int2(blockIdx.x, seg.last_cta);
       if (!many_of(seg)) append<T>(a, deal, seg, lane, 32);
     }
@@ -781,17 +774,6 @@ inline bool wide_map(CUtensorMap* map, const void* base, bool bf16, int64_t colu
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// How the rows lie in tiles; tile_nodes 0 when a key head's group does not fit a tile.
-inline WideRows wide_rows(const Args& a) {
-  WideRows w;
-  const int group = (int)(a.heads / a.kv_heads);
-  w.copies = a.nodes <= 32 / group ? 4 : a.nodes <= 64 / group ? 2 : 1;
-  w.tile_nodes = kRowsTile / w.copies / group;
-  w.share = w.tile_nodes > 0 && a.nodes > w.tile_nodes;
-  if (w.tile_nodes > a.nodes) w.tile_nodes = (int)a.nodes;
-  return w;
 }
 
 template <class T, int D, int COPIES>
