@@ -322,8 +322,10 @@ class KVCache:
         self.pending = None
 
     def evict(self, budget: int, recent: int = 0):
-        """Cut every sequence to `budget` entries (see `evict`); returns `kept`."""
+        """Cut every sequence to `budget` entries (see `evict`); returns `kept`. Not while an
+        extension is pending: its nodes lie behind the lengths that this changes."""
         _need(self.weights is not None, "eviction takes a cache with weights")
+        _need(self.pending is None, "an extension is pending: accept it, or none of it, first")
         kept = evict(self.keys, self.values, self.weights, self.positions, self.lengths,
                      self.seen, budget, recent, status=self.status)
         self.lengths.clamp_(max=budget)

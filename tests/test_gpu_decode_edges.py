@@ -54,3 +54,37 @@ def test_small_caches_keep_to_their_workspace(lengths, nodes, heads, kv, d, cap,
     assert status == runtime.STATUS_OK, runtime.last_error()
     x.check(out, lse)
     assert bool((guarded[size:] == 77).all())
+
+
+# ---------------------------------------------------------------- the order of calls
+
+
+def _model_and_cache(batch, capacity, layers=1, seed=5):
+    from ppy_b200 import gpt2
+
+    model = gpt2.GPT2(gpt2.Config(layers=layers), seed=seed)
+    return model, model.new_cache(batch, capacity=capacity)
+
+
+def _ids(batch, length, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(0, 50257, (batch, length), device="cuda", generator=g)
+
+
+def test_evict_waits_for_the_pending_extension():
+    """A cache cut between an extension and its acceptance would take other rows for the nodes'."""
+    from ppy_b200.runtime import B200Error
+
+    model, cache = _model_and_cache(2, 64)
+    model.extend(cache, _ids(2, 30))
+    cache.accept()
+    model.extend(cache, _ids(2, 3, seed=1))
+    nodes = cache.keys[:, :, :, 30:33].clone()
+    with pytest.raises(B200Error, match="pending"):
+        cache.evict(16)
+    assert cache.lengths.tolist() == [30, 30]
+    cache.accept(accepted=torch.tensor([2, 0], dtype=torch.int32, device="cuda"))
+    assert torch.equal(cache.keys[:, 0, :, 30:32], nodes[:, 0, :, :2])
+    cache.evict(16)
+    cache.check()
+    assert cache.lengths.tolist() == [16, 16] and cache.seen.tolist() == [32, 30]
