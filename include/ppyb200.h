@@ -318,6 +318,20 @@ typedef struct ppyb200_accept_args {
 
 int32_t ppyb200_accept(const ppyb200_accept_args *args);
 
+/* A piece of a path that has more steps than one call takes: `steps` (of args) steps from step
+ * `first` on, of a path of path_steps with path_stride between sequences (0: one path for all);
+ * accepted counts the whole path's. lengths and seen have grown by what the pieces before took;
+ * nodes and slots are those of the attention, as for a whole path. taken[b] (may be NULL) gets the
+ * steps taken so far, this piece's among them; taken_before is that of the piece before (another
+ * buffer; NULL for the first): a sequence whose path was cut there takes no further step. */
+typedef struct ppyb200_accept_part_args {
+  const int32_t *taken_before;
+  int32_t *taken;
+  int64_t first, path_steps, path_stride;
+} ppyb200_accept_part_args;
+
+int32_t ppyb200_accept_part(const ppyb200_accept_args *args, const ppyb200_accept_part_args *part);
+
 /* Every key head of sequences longer than `budget` keeps `budget` entries: those with a position
  * of at least seen[b] - recent first, then by weight from the largest, NaN last; the lowest slot
  * first among equals. Kept entries in slots below the budget stay; those behind it fill the

@@ -104,7 +104,8 @@ struct KeyRows {
 // by memory: 1152 key heads of 1700 to 4000 entries, 64 wide, 81 us, 5.1 TB/s.
 template <class T, int D>
 __global__ void __launch_bounds__(kAcceptThreads, D == 64 ? 8 : 5)
-accept_kernel(const __grid_constant__ ppyb200_accept_args a, const int chunks,
+accept_kernel(const __grid_constant__ ppyb200_accept_args a,
+              const __grid_constant__ ppyb200_accept_part_args part, const int chunks,
               const int chunk_keys) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int path[PPYB200_PATH_STEPS];
@@ -116,23 +117,32 @@ accept_kernel(const __grid_constant__ ppyb200_accept_args a, const int chunks,
   const int kvh = blockIdx.y, group = (int)(a.heads / a.kv_heads), d = (int)a.head_dim;
   const bool last = (int)blockIdx.x == chunks;  // the CTA of the path's own entries
 
+  // the piece's steps: none where the piece before was cut
+  const int first = (int)part.first, steps = (int)a.steps;
+  const int before = first > 0 ? part.taken_before[b] : 0;
   int64_t length = a.lengths[b];
   int n = a.accepted[b];
-  bool bad = length < 0 || length > a.capacity || n < 0 || n > a.steps;
+  const int shortest = before == first ? first : 0;
+  bool bad = length < shortest || length > a.capacity || n < 0 || n > part.path_steps;
+  n = before != first || length < first ? 0 : min(max(n - first, 0), steps);
   length = length < 0 ? 0 : (length > a.capacity ? a.capacity : length);
-  n = n < 0 ? 0 : (n > (int)a.steps ? (int)a.steps : n);
+  const int64_t nodes_at = length - first;  // the slot of the attention's first node
   if (tid == 0) valid = n;
   __syncthreads();
   for (int t = tid; t < n; t += kAcceptThreads) {
-    const int p = a.path[b * a.steps + t];
-    const int before = t > 0 ? a.path[b * a.steps + t - 1] : -1;
+    const int32_t* from = a.path + b * part.path_stride + first + t;
+    const int p = from[0];
     path[t] = p;
-    if (p <= before || p >= a.nodes || length + p >= a.capacity) atomicMin(&valid, t);
+    if (p <= (first + t > 0 ? from[-1] : -1) || p >= a.nodes || nodes_at + p >= a.capacity)
+      atomicMin(&valid, t);
   }
   __syncthreads();
   if (valid < n) bad = true;
   n = valid;
-  if (bad && last && kvh == 0 && tid == 0) raise(a.status);
+  if (last && kvh == 0 && tid == 0) {
+    if (bad) raise(a.status);
+    if (layer == 0 && part.taken != nullptr) part.taken[b] = before + n;
+  }
   if (n <= 0) return;
   const int64_t j0 = (int64_t)blockIdx.x * chunk_keys;
   if (!last && j0 >= length) return;
@@ -201,8 +211,8 @@ accept_kernel(const __grid_constant__ ppyb200_accept_args a, const int chunks,
     for (int t = warp * 16; t < n; t += kAcceptThreads / 2) {
       const int ta = t + gid, tb = ta + 8;
       KeyRows<T, D> k;
-      k.load(ta < n ? keys + (length + path[ta]) * a.keys_strides[3] : nullptr,
-             tb < n ? keys + (length + path[tb]) * a.keys_strides[3] : nullptr, d, tig);
+      k.load(ta < n ? keys + (nodes_at + path[ta]) * a.keys_strides[3] : nullptr,
+             tb < n ? keys + (nodes_at + path[tb]) * a.keys_strides[3] : nullptr, d, tig);
       float s0, s1;
       k.weigh(qf, lse, rows, scale, lane, ta * group, tb * group, s0, s1);
       if (tig == 0 && ta < n) weights[length + ta] = s0;
@@ -222,7 +232,7 @@ accept_kernel(const __grid_constant__ ppyb200_accept_args a, const int chunks,
   __syncthreads();
   for (int i = tid; i < n * pieces * 2; i += kAcceptThreads) {
     const int piece = i % pieces, t = (i / pieces) >> 1;
-    const int64_t slot = length + path[t];
+    const int64_t slot = nodes_at + path[t];
     box[i] = ((i / pieces) & 1) == 0
                  ? *reinterpret_cast<const uint4*>(keys + slot * a.keys_strides[3] + piece * 8)
                  : *reinterpret_cast<const uint4*>(values + slot * a.values_strides[3] +
@@ -240,7 +250,8 @@ accept_kernel(const __grid_constant__ ppyb200_accept_args a, const int chunks,
 }
 
 template <class T, int D>
-cudaError_t launch_accept(const ppyb200_accept_args& a, cudaStream_t stream) {
+cudaError_t launch_accept(const ppyb200_accept_args& a, const ppyb200_accept_part_args& part,
+                          cudaStream_t stream) {
   static ppyb200::DeviceOnce once;
   const int64_t rows = (a.steps * (a.heads / a.kv_heads) + 7) / 8 * 8;
   const int64_t queries = rows * (D * 2 + 4), box = a.steps * a.head_dim * 4;
@@ -262,7 +273,7 @@ cudaError_t launch_accept(const ppyb200_accept_args& a, cudaStream_t stream) {
   return ppyb200::launch_pdl(kernel,
                              dim3((unsigned)chunks + 1, (unsigned)a.kv_heads,
                                   (unsigned)(a.layers * a.batch)),
-                             dim3(kAcceptThreads), smem, stream, a, chunks, (int)chunk);
+                             dim3(kAcceptThreads), smem, stream, a, part, chunks, (int)chunk);
 }
 
 // ---------------------------------------------------------------- evict
@@ -753,10 +764,11 @@ const char* refusal(const ppyb200_evict_args& a) {
 
 extern "C" {
 
-int32_t ppyb200_accept(const ppyb200_accept_args* args) {
-  if (args == nullptr) return refuse("ppyb200_accept", "no arguments");
-  const ppyb200_accept_args& a = *args;
+int32_t ppyb200_accept_part(const ppyb200_accept_args* args,
+                            const ppyb200_accept_part_args* part) {
   const char* who = "ppyb200_accept";
+  if (args == nullptr || part == nullptr) return refuse(who, "no arguments");
+  const ppyb200_accept_args& a = *args;
   if (a.dtype != PPYB200_BF16 && a.dtype != PPYB200_F16) return refuse(who, "dtype is bf16 or f16");
   if (a.layers < 0 || a.batch < 0 || a.nodes < 0 || a.steps < 0 || a.capacity < 0 ||
       a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0)
@@ -772,18 +784,27 @@ int32_t ppyb200_accept(const ppyb200_accept_args* args) {
     return refuse(who, "every row of q and the cache starts on a 16-byte boundary");
   if (a.weights != nullptr && (a.q == nullptr || a.lse == nullptr))
     return refuse(who, "weights take q and lse");
+  if (part->first < 0 || part->path_steps > INT32_MAX || part->path_stride < 0 ||
+      part->first + a.steps > part->path_steps || (part->first > 0 && part->taken_before == nullptr))
+    return refuse(who, "a piece lies within its path and follows the steps taken before it");
   if (a.layers == 0 || a.batch == 0 || a.steps == 0) return PPYB200_OK;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(ppyb200_stream());
   cudaError_t e;
   if (a.dtype == PPYB200_BF16)
-    e = a.head_dim <= 64 ? launch_accept<__nv_bfloat16, 64>(a, stream)
-                         : launch_accept<__nv_bfloat16, 128>(a, stream);
+    e = a.head_dim <= 64 ? launch_accept<__nv_bfloat16, 64>(a, *part, stream)
+                         : launch_accept<__nv_bfloat16, 128>(a, *part, stream);
   else
-    e = a.head_dim <= 64 ? launch_accept<__half, 64>(a, stream)
-                         : launch_accept<__half, 128>(a, stream);
+    e = a.head_dim <= 64 ? launch_accept<__half, 64>(a, *part, stream)
+                         : launch_accept<__half, 128>(a, *part, stream);
   if (e != cudaSuccess) return ppyb200_check((int32_t)e, who);
   ppyb200_count_launches(1);
   return PPYB200_OK;
+}
+
+int32_t ppyb200_accept(const ppyb200_accept_args* args) {
+  if (args == nullptr) return refuse("ppyb200_accept", "no arguments");
+  const ppyb200_accept_part_args whole = {nullptr, nullptr, 0, args->steps, args->steps};
+  return ppyb200_accept_part(args, &whole);
 }
 
 int64_t ppyb200_evict_workspace(const ppyb200_evict_args* args) {

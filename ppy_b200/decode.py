@@ -35,6 +35,7 @@ TREE_NODES, PATH_STEPS, PATH_ROWS = 256, 64, 512
 
 _ATTENTION = struct.Struct("=39qd")  # ppyb200_tree_attention_args
 _ACCEPT = struct.Struct("=35qd")  # ppyb200_accept_args
+_PART = struct.Struct("=5q")  # ppyb200_accept_part_args
 _EVICT = struct.Struct("=33q")  # ppyb200_evict_args
 
 
@@ -133,7 +134,7 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
 
 
 def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, accepted,
-                 scale=None, status=None) -> None:
+                 scale=None, status=None, taken=None) -> None:
     """The verified path of the last attention joins the caches of every layer, in place.
 
     q [layers, batch, nodes, heads, head_dim] and lse f32 [layers, batch, heads, nodes] are that
@@ -147,15 +148,27 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
     keys and values move to slots lengths[b], lengths[b] + 1, ..., their weights start with what
     the path paid them, and positions (int32, laid out as weights; None: not kept) get seen[b],
     seen[b] + 1, ... (`seen` int32 [batch]: the tokens before them). lengths and seen are the
-    caller's to advance. `status` as in tree_attention: raised when the path is not in order (it is
-    cut there) or a length or count is out of range."""
+    caller's to advance, by `taken` (int32 [batch], optional), which gets the steps that were taken:
+    a path is cut before a step that is out of order or behind the capacity. `status` as in
+    tree_attention: raised when a path was cut, or a length or count is out of range."""
+    _need(path.dim() == 2, "path: int32 [batch, steps]")
+    _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accepted, scale, status,
+            taken)
+
+
+def _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accepted, scale, status,
+            taken, first=0, steps=None, before=None) -> None:
+    """`accept_nodes` for `steps` steps from step `first` on, all without them; path as there, or
+    [steps] for every sequence. `before` is what the piece of the path before this one left in
+    `taken`."""
     kind, device = _KINDS.get(keys.dtype), keys.get_device()
     _need(kind is not None and device >= 0 and keys.dim() == 5 and q.dim() == 5,
           "keys: bf16 or f16 [layers, batch, kv_heads, capacity, head_dim], q [layers, batch, "
           "nodes, heads, head_dim], on a CUDA device")
     layers, batch, kv_heads, capacity, d = keys.shape
     nodes, heads = q.shape[2], q.shape[3]
-    steps = path.shape[-1]
+    length = path.shape[-1]
+    steps = length if steps is None else steps
     q_strides = element_rows("q", q, (layers, batch, nodes, heads, d), keys.dtype, device)
     keys_strides = element_rows("keys", keys, keys.shape, keys.dtype, device)
     values_strides = element_rows("values", values, keys.shape, keys.dtype, device)
@@ -163,7 +176,10 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
         whole("lse", lse, (layers, batch, heads, nodes), torch.float32, device)
     for name, t in (("lengths", lengths), ("seen", seen), ("accepted", accepted)):
         whole(name, t, (batch,), torch.int32, device)
-    whole("path", path, (batch, steps), torch.int32, device)
+    whole("path", path, (batch, length) if path.dim() == 2 else (length,), torch.int32, device)
+    for t in (taken, before):
+        if t is not None:
+            whole("taken", t, (batch,), torch.int32, device)
     tables = weights if weights is not None else positions
     strides = (0, 0, 0)
     for name, t, kept in (("weights", weights, torch.float32),
@@ -174,15 +190,19 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
             strides = t.stride()[:3]
     if status is not None:
         whole("status", status, (1,), torch.int32, device)
+    if taken is not None and (layers == 0 or steps == 0):
+        taken.zero_()
     beside = begin(device)
     try:
-        if runtime.library().ppyb200_accept(_ACCEPT.pack(
+        if runtime.library().ppyb200_accept_part(_ACCEPT.pack(
                 q.data_ptr(), lse.data_ptr(), keys.data_ptr(), values.data_ptr(),
                 _address(weights), _address(positions), lengths.data_ptr(), seen.data_ptr(),
                 path.data_ptr(), accepted.data_ptr(), _address(status), kind, layers, batch, nodes,
                 steps, heads, kv_heads, d, capacity, *q_strides[:4], *keys_strides[:4],
                 *values_strides[:4], *strides,
-                1.0 / math.sqrt(d) if scale is None else scale)) != runtime.STATUS_OK:
+                1.0 / math.sqrt(d) if scale is None else scale), _PART.pack(
+                    _address(before), _address(taken), first, length,
+                    length if path.dim() == 2 else 0)) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
     finally:
         end(beside)
@@ -298,27 +318,31 @@ class KVCache:
     def accept(self, path=None, accepted=None) -> None:
         """The nodes path[b, :accepted[b]] of the last extension (int32 [batch, steps] and
         [batch], as `accept_nodes`; all nodes without a path, each sequence's first accepted[b]
-        of them) join the cache: lengths and seen grow by `accepted`. Paths longer than
-        accept_nodes takes go in pieces."""
+        of them) join the cache: lengths and seen grow by the steps taken, fewer than `accepted`
+        where the path is cut. Paths longer than accept_nodes takes go in pieces."""
         _need(self.pending is not None, "accept follows an extension")
         q, lse = self.pending
-        batch, nodes, heads = q.shape[1], q.shape[2], q.shape[3]
-        device = self.keys.device
+        nodes, heads, device = q.shape[2], q.shape[3], self.keys.device
         if path is None:
-            path = torch.arange(nodes, dtype=torch.int32, device=device).expand(batch, nodes)
+            path = torch.arange(nodes, dtype=torch.int32, device=device)
+        else:
+            _need(path.dim() == 2, "path: int32 [batch, steps]")
+            path = path.contiguous()
+        steps = path.shape[-1]
         if accepted is None:
-            accepted = torch.full((batch,), path.shape[1], dtype=torch.int32, device=device)
-        most = min(PATH_STEPS, PATH_ROWS // (heads // self.keys.shape[2]))
-        for at in range(0, path.shape[1], most):
-            part = path[:, at:at + most] - at
-            count = (accepted - at).clamp(0, part.shape[1])
-            # the nodes from `at` on: a path ascends, so its step `at` is node `at` or later
-            part_lse = lse[..., at:].contiguous() if self.weights is not None else lse
-            accept_nodes(q[:, :, at:], part_lse, self.keys, self.values,
-                         self.weights, self.positions, self.lengths, self.seen,
-                         part.contiguous(), count, status=self.status)
-            self.lengths += count
-            self.seen += count
+            accepted = torch.full_like(self.lengths, steps)
+        group = heads // self.keys.shape[2]
+        _need(group <= PATH_ROWS, "up to 512 query heads a key head")
+        most, before = min(PATH_STEPS, PATH_ROWS // group), None
+        for first in range(0, steps, most):
+            taken = torch.empty_like(self.lengths)
+            _accept(q, lse, self.keys, self.values, self.weights, self.positions, self.lengths,
+                    self.seen, path, accepted, None, self.status, taken, first,
+                    min(most, steps - first), before)
+            grown = taken if before is None else taken - before
+            self.lengths += grown
+            self.seen += grown
+            before = taken
         self.pending = None
 
     def evict(self, budget: int, recent: int = 0):

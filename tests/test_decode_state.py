@@ -22,3 +22,29 @@ def test_evict_refuses_while_an_extension_is_pending():
     cache.reset()  # forgets the extension too
     with pytest.raises(runtime.B200Error, match="CUDA device"):
         cache.evict(4)
+
+
+def _part(**changes):
+    values = dict(taken_before=0, taken=0, first=0, path_steps=2, path_stride=2)
+    values.update(changes)
+    return decode._PART.pack(*values.values())
+
+
+@pytest.mark.parametrize("part", [
+    dict(first=-1), dict(first=1, taken_before=64), dict(first=64, path_steps=66),
+    dict(path_steps=1), dict(path_stride=-1), dict(path_steps=1 << 31),
+])
+def test_pieces_of_a_path_that_are_refused(part):
+    lib = runtime.library()
+    args = decode._ACCEPT.pack(*(0,) * 11, 1, 1, 1, 4, 2, 4, 2, 64, 128, *(64,) * 15, 0.125)
+    assert lib.ppyb200_accept_part(args, _part(**part)) == runtime.STATUS_RAISED
+    assert "piece" in runtime.last_error()
+    assert lib.ppyb200_accept_part(args, None) == runtime.STATUS_RAISED
+
+
+def test_accept_refuses_paths_of_other_shapes():
+    cache = _cache()
+    cache.pending = (torch.zeros(1, 2, 3, 2, 64), torch.zeros(1, 2, 2, 3))
+    with pytest.raises(runtime.B200Error, match="path"):
+        cache.accept(torch.zeros(3, dtype=torch.int32))
+    assert cache.pending is not None

@@ -88,3 +88,128 @@ def test_evict_waits_for_the_pending_extension():
     cache.evict(16)
     cache.check()
     assert cache.lengths.tolist() == [16, 16] and cache.seen.tolist() == [32, 30]
+
+
+def _plain_accept(cache, before, path, accepted, nodes):
+    """What lengths, seen, positions, keys and values are after `path` (a list per sequence) of an
+    extension of `nodes` nodes: steps up to the first that is out of order or not in the cache."""
+    for b, steps in enumerate(path):
+        length, seen = int(before["lengths"][b]), int(before["seen"][b])
+        want, last = [], -1
+        for p in steps[:max(0, int(accepted[b]))]:
+            if p <= last or p >= nodes or length + p >= cache.capacity:
+                break
+            want.append(p)
+            last = p
+        n = len(want)
+        assert int(cache.lengths[b]) == length + n and int(cache.seen[b]) == seen + n
+        old = [length + p for p in want]
+        for name in ("keys", "values"):
+            now = getattr(cache, name)[:, b]
+            assert torch.equal(now[:, :, :length], before[name][:, b, :, :length])
+            assert torch.equal(now[:, :, length:length + n], before[name][:, b][:, :, old])
+            assert torch.equal(now[:, :, length + n:], before[name][:, b, :, length + n:])
+        assert bool((cache.positions[:, b, :, length:length + n] == torch.arange(
+            seen, seen + n, device="cuda")).all())
+
+
+def _pending_cache(lengths, nodes, capacity, heads=2, kv=2, d=64, seed=3):
+    """A cache with an extension of random keys, values and queries behind `lengths`."""
+    from ppy_b200 import decode
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    batch = len(lengths)
+    cache = decode.KVCache(2, batch, kv, d, capacity)
+    cache.keys.normal_(generator=g)
+    cache.values.normal_(generator=g)
+    cache.lengths.copy_(torch.tensor(lengths))
+    cache.seen.copy_(torch.tensor(lengths) + 5)
+    cache.pending = (torch.randn(2, batch, nodes, heads, d, device="cuda", generator=g).to(BF16),
+                     5 + torch.rand(2, batch, heads, nodes, device="cuda", generator=g))
+    before = {k: getattr(cache, k).clone() for k in ("keys", "values", "lengths", "seen")}
+    return cache, before
+
+
+@pytest.mark.parametrize("path,accepted,raises", [
+    ([[0, 2, 3], [1, 4, 5]], [3, 2], False),
+    ([[0, 2, 2], [4, 1, 5]], [3, 3], True),       # cut after two steps, and after one
+    ([[5, 6, 7], [0, 1, 2]], [3, 3], True),       # nodes that do not exist
+    ([[0, 1, 2], [-1, 0, 1]], [3, 3], True),
+    ([[0, 1, 2], [0, 1, 2]], [4, -1], True),      # counts out of range: all, and none
+    ([[0, 1, 2], [0, 1, 2]], [0, 0], False),
+])
+def test_cache_grows_by_the_steps_taken(path, accepted, raises):
+    from ppy_b200.runtime import B200Error
+
+    cache, before = _pending_cache((20, 7), 6, 64)
+    cache.accept(torch.tensor(path, dtype=torch.int32, device="cuda"),
+                 torch.tensor(accepted, dtype=torch.int32, device="cuda"))
+    if raises:
+        with pytest.raises(B200Error, match="out of range"):
+            cache.check()
+    cache.check()
+    _plain_accept(cache, before, path, accepted, 6)
+
+
+def test_cache_never_grows_past_its_capacity():
+    """An extension that does not fit: the nodes that do are taken, and the cache stays usable."""
+    from ppy_b200.runtime import B200Error
+
+    cache, before = _pending_cache((60, 64, 20), 6, 64)
+    cache.accept()
+    with pytest.raises(B200Error, match="out of range"):
+        cache.check()
+    assert cache.lengths.tolist() == [64, 64, 26] and cache.seen.tolist() == [69, 69, 31]
+    _plain_accept(cache, before, [list(range(6))] * 3, [6, 6, 6], 6)
+
+
+@pytest.mark.parametrize("heads,kv,cut", [(2, 2, None), (2, 2, 64), (8, 1, 70), (2, 2, 130),
+                                          (16, 1, 31)])
+def test_long_paths_in_pieces(heads, kv, cut):
+    """Paths of 150 of 200 nodes, in pieces of 64 steps (32 with 16 heads on a key head), ascending
+    across the pieces; cut for one sequence by a step that repeats the one before. Weights and
+    rows are those of the same steps taken one after the other."""
+    from ppy_b200 import decode
+
+    nodes, lengths = 200, (90, 0, 33)
+    g = torch.Generator().manual_seed(7)
+    path = torch.stack([torch.randperm(nodes, generator=g)[:150].sort().values for _ in lengths])
+    if cut is not None:
+        path[1, cut] = path[1, cut - 1]
+    accepted = [150, 150, 97]
+    cache, before = _pending_cache(lengths, nodes, 400, heads, kv)
+    q, lse = cache.pending
+    other, _ = _pending_cache(lengths, nodes, 400, heads, kv)
+    cache.accept(path.to(torch.int32).cuda(),
+                 torch.tensor(accepted, dtype=torch.int32, device="cuda"))
+    assert int(cache.status) == (0 if cut is None else 2)
+    _plain_accept(cache, before, path.tolist(), accepted, nodes)
+    taken = [150, 150 if cut is None else cut, 97]
+    # one step a call: the node's slot, counted from the length as it is now, moves down with it
+    for step in range(150):
+        node = path[:, step].clamp(min=0)
+        on = torch.tensor([int(step < n) for n in taken], dtype=torch.int32, device="cuda")
+        index = node.cuda()[None, :, None, None, None]
+        here = torch.zeros(3, 1, dtype=torch.int32, device="cuda")
+        # bring the node's row to the slot at the length, where a tree of one node has it
+        for b in range(3):
+            if step < taken[b]:
+                at, to = lengths[b] + int(node[b]), int(other.lengths[b])
+                for t in (other.keys, other.values):
+                    t[:, b, :, to] = t[:, b, :, at].clone()
+        decode.accept_nodes(q.gather(2, index.expand(2, 3, 1, heads, 64)),
+                            lse.gather(3, index[..., 0].permute(0, 1, 3, 2).expand(2, 3, heads, 1)),
+                            other.keys, other.values, other.weights, other.positions,
+                            other.lengths, other.seen, here, on)
+        other.lengths += on
+        other.seen += on
+    # a score is off by at most ds on either side, f32 sums of the same terms in another order by
+    # half a step a term
+    ds = 66 * 2.0 ** -23 / 8 * float((q.abs().double().transpose(2, 3).reshape(2, 3, kv, -1, 64)
+                                      @ before["keys"].abs().double().transpose(3, 4)).max())
+    terms = 150 * heads // kv
+    for b, n in enumerate(taken):
+        end = lengths[b] + n
+        assert torch.equal(cache.keys[:, b, :, :end], other.keys[:, b, :, :end])
+        got, want = cache.weights[:, b, :, :end].double(), other.weights[:, b, :, :end].double()
+        assert bool(((got - want).abs() <= (2 * ds + 2 * terms * 2.0 ** -24) * want).all())
