@@ -323,9 +323,10 @@ int32_t ppyb200_accept(const ppyb200_accept_args *args);
  * accepted counts the whole path's. lengths and seen have grown by what the pieces before took;
  * nodes and slots are those of the attention, as for a whole path. taken[b] (may be NULL) gets the
  * steps taken so far, this piece's among them; taken_before is that of the piece before (another
- * buffer; NULL for the first): a sequence whose path was cut there takes no further step. */
+ * buffer; NULL for the first): a sequence whose path was cut there takes no further step. counts
+ * (may be NULL) are the attention's: a step at a node at or behind counts[b] is cut, too. */
 typedef struct ppyb200_accept_part_args {
-  const int32_t *taken_before;
+  const int32_t *counts, *taken_before;
   int32_t *taken;
   int64_t first, path_steps, path_stride;
 } ppyb200_accept_part_args;

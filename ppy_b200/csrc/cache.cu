@@ -127,13 +127,14 @@ accept_kernel(const __grid_constant__ ppyb200_accept_args a,
   n = before != first || length < first ? 0 : min(max(n - first, 0), steps);
   length = length < 0 ? 0 : (length > a.capacity ? a.capacity : length);
   const int64_t nodes_at = length - first;  // the slot of the attention's first node
+  const int nodes = part.counts == nullptr ? (int)a.nodes : min((int)a.nodes, part.counts[b]);
   if (tid == 0) valid = n;
   __syncthreads();
   for (int t = tid; t < n; t += kAcceptThreads) {
     const int32_t* from = a.path + b * part.path_stride + first + t;
     const int p = from[0];
     path[t] = p;
-    if (p <= (first + t > 0 ? from[-1] : -1) || p >= a.nodes || nodes_at + p >= a.capacity)
+    if (p <= (first + t > 0 ? from[-1] : -1) || p >= nodes || nodes_at + p >= a.capacity)
       atomicMin(&valid, t);
   }
   __syncthreads();
@@ -803,7 +804,7 @@ int32_t ppyb200_accept_part(const ppyb200_accept_args* args,
 
 int32_t ppyb200_accept(const ppyb200_accept_args* args) {
   if (args == nullptr) return refuse("ppyb200_accept", "no arguments");
-  const ppyb200_accept_part_args whole = {nullptr, nullptr, 0, args->steps, args->steps};
+  const ppyb200_accept_part_args whole = {nullptr, nullptr, nullptr, 0, args->steps, args->steps};
   return ppyb200_accept_part(args, &whole);
 }
 

@@ -21,6 +21,7 @@ from __future__ import annotations
 import functools
 import math
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -28,14 +29,14 @@ from . import runtime
 from .runtime import B200Error
 from .torch_calls import begin, element_rows, end, whole
 
-__all__ = ["KVCache", "accept_nodes", "evict", "tree_attention"]
+__all__ = ["Extension", "KVCache", "accept_nodes", "evict", "tree_attention"]
 
 #: The header's limits (include/ppyb200.h).
 TREE_NODES, PATH_STEPS, PATH_ROWS = 256, 64, 512
 
 _ATTENTION = struct.Struct("=39qd")  # ppyb200_tree_attention_args
 _ACCEPT = struct.Struct("=35qd")  # ppyb200_accept_args
-_PART = struct.Struct("=5q")  # ppyb200_accept_part_args
+_PART = struct.Struct("=6q")  # ppyb200_accept_part_args
 _EVICT = struct.Struct("=33q")  # ppyb200_evict_args
 
 
@@ -134,7 +135,7 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
 
 
 def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, accepted,
-                 scale=None, status=None, taken=None) -> None:
+                 scale=None, status=None, taken=None, counts=None) -> None:
     """The verified path of the last attention joins the caches of every layer, in place.
 
     q [layers, batch, nodes, heads, head_dim] and lse f32 [layers, batch, heads, nodes] are that
@@ -149,15 +150,16 @@ def accept_nodes(q, lse, keys, values, weights, positions, lengths, seen, path, 
     the path paid them, and positions (int32, laid out as weights; None: not kept) get seen[b],
     seen[b] + 1, ... (`seen` int32 [batch]: the tokens before them). lengths and seen are the
     caller's to advance, by `taken` (int32 [batch], optional), which gets the steps that were taken:
-    a path is cut before a step that is out of order or behind the capacity. `status` as in
-    tree_attention: raised when a path was cut, or a length or count is out of range."""
+    a path is cut before a step that is out of order, behind the capacity, or no node of the
+    sequence (`counts`, int32 [batch], as the attention had them). `status` as in tree_attention:
+    raised when a path was cut, or a length or count is out of range."""
     _need(path.dim() == 2, "path: int32 [batch, steps]")
     _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accepted, scale, status,
-            taken)
+            taken, counts)
 
 
 def _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accepted, scale, status,
-            taken, first=0, steps=None, before=None) -> None:
+            taken, counts, first=0, steps=None, before=None) -> None:
     """`accept_nodes` for `steps` steps from step `first` on, all without them; path as there, or
     [steps] for every sequence. `before` is what the piece of the path before this one left in
     `taken`."""
@@ -177,9 +179,9 @@ def _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accep
     for name, t in (("lengths", lengths), ("seen", seen), ("accepted", accepted)):
         whole(name, t, (batch,), torch.int32, device)
     whole("path", path, (batch, length) if path.dim() == 2 else (length,), torch.int32, device)
-    for t in (taken, before):
+    for name, t in (("taken", taken), ("taken", before), ("counts", counts)):
         if t is not None:
-            whole("taken", t, (batch,), torch.int32, device)
+            whole(name, t, (batch,), torch.int32, device)
     tables = weights if weights is not None else positions
     strides = (0, 0, 0)
     for name, t, kept in (("weights", weights, torch.float32),
@@ -201,7 +203,7 @@ def _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accep
                 steps, heads, kv_heads, d, capacity, *q_strides[:4], *keys_strides[:4],
                 *values_strides[:4], *strides,
                 1.0 / math.sqrt(d) if scale is None else scale), _PART.pack(
-                    _address(before), _address(taken), first, length,
+                    _address(counts), _address(before), _address(taken), first, length,
                     length if path.dim() == 2 else 0)) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
     finally:
@@ -271,6 +273,16 @@ def evict(keys, values, weights, positions, lengths, seen, budget, recent=0, wei
     return kept
 
 
+class Extension(NamedTuple):
+    """What an extension leaves for `KVCache.accept`: its queries [layers, batch, nodes, query
+    heads, head_dim], log-sum-exps f32 [layers, batch, query heads, nodes], and each sequence's
+    real nodes, int32 [batch] (None: all)."""
+
+    queries: object
+    lse: object
+    counts: object = None
+
+
 class KVCache:
     """Keys and values of `batch` sequences over `layers` layers, with what decoding keeps beside
     them, as plain torch tensors:
@@ -281,8 +293,7 @@ class KVCache:
         positions      int32, laid out as weights: the token position of each entry
         lengths, seen  int32 [batch]: entries in the cache, and tokens accepted so far
 
-    `pending` is what the last extension left for `accept`: its queries [layers, batch, nodes,
-    query heads, head_dim] and log-sum-exps f32 [layers, batch, query heads, nodes]."""
+    `pending` is what the last extension left for `accept` (an `Extension`)."""
 
     def __init__(self, layers: int, batch: int, heads: int, head_dim: int, capacity: int,
                  dtype=torch.bfloat16, device="cuda", weights: bool = True) -> None:
@@ -318,13 +329,14 @@ class KVCache:
     def accept(self, path=None, accepted=None) -> None:
         """The nodes path[b, :accepted[b]] of the last extension (int32 [batch, steps] and
         [batch], as `accept_nodes`; all nodes without a path, each sequence's first accepted[b]
-        of them) join the cache: lengths and seen grow by the steps taken, fewer than `accepted`
+        of them, or as many as it has) join the cache: lengths and seen grow by the steps taken, fewer than `accepted`
         where the path is cut. Paths longer than accept_nodes takes go in pieces."""
         _need(self.pending is not None, "accept follows an extension")
-        q, lse = self.pending
+        q, lse, counts = Extension(*self.pending)
         nodes, heads, device = q.shape[2], q.shape[3], self.keys.device
         if path is None:
             path = torch.arange(nodes, dtype=torch.int32, device=device)
+            accepted = counts if accepted is None else accepted
         else:
             _need(path.dim() == 2, "path: int32 [batch, steps]")
             path = path.contiguous()
@@ -337,7 +349,7 @@ class KVCache:
         for first in range(0, steps, most):
             taken = torch.empty_like(self.lengths)
             _accept(q, lse, self.keys, self.values, self.weights, self.positions, self.lengths,
-                    self.seen, path, accepted, None, self.status, taken, first,
+                    self.seen, path, accepted, None, self.status, taken, counts, first,
                     min(most, steps - first), before)
             grown = taken if before is None else taken - before
             self.lengths += grown

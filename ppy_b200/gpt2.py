@@ -246,6 +246,7 @@ class GPT2:
             stride = 0 if shared else nodes
         if counts is not None:
             torch_calls.whole("counts", counts, (batch,), torch.int32, ids.get_device())
+            counts = counts.clone()  # `accept` needs them too, and the caller may have changed them
         s = cache.buffers.get((batch, nodes))
         if s is None:
             d = ids.device
@@ -302,8 +303,8 @@ class GPT2:
         # without weights one layer's queries stand for all: `accept` only moves rows then
         queries = s["qkv"].view(-1, *heads)[:, :, :, 0]
         lse = s["lse"]
-        cache.pending = (queries.expand(cfg.layers, *queries.shape[1:]),
-                         lse.expand(cfg.layers, *lse.shape[1:]))
+        cache.pending = decode.Extension(queries.expand(cfg.layers, *queries.shape[1:]),
+                                         lse.expand(cfg.layers, *lse.shape[1:]), counts)
         return logits
 
     def score(self, ids, top: int = 0, logits=None) -> scoring.TokenLogprobs:

@@ -25,7 +25,7 @@ def test_evict_refuses_while_an_extension_is_pending():
 
 
 def _part(**changes):
-    values = dict(taken_before=0, taken=0, first=0, path_steps=2, path_stride=2)
+    values = dict(counts=0, taken_before=0, taken=0, first=0, path_steps=2, path_stride=2)
     values.update(changes)
     return decode._PART.pack(*values.values())
 

@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_gpu_decode import BF16, F16, Inputs, bound  # noqa: F401 - the fixture
+from test_gpu_decode import BF16, F16, Inputs, _near, bound  # noqa: F401 - the fixture
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,40 @@ def test_long_paths_in_pieces(heads, kv, cut):
         assert torch.equal(cache.keys[:, b, :, :end], other.keys[:, b, :, :end])
         got, want = cache.weights[:, b, :, :end].double(), other.weights[:, b, :, :end].double()
         assert bool(((got - want).abs() <= (2 * ds + 2 * terms * 2.0 ** -24) * want).all())
+
+
+def test_padded_extensions_are_accepted_without_their_padding():
+    """Prompts of different lengths in one batch: accept() takes each sequence's own nodes, and the
+    next token's logits are those of each prompt by itself. The counts may change meanwhile."""
+    model, cache = _model_and_cache(3, 64)
+    ids, token = _ids(3, 20), _ids(3, 1, seed=1)
+    counts = torch.tensor([20, 3, 11], dtype=torch.int32, device="cuda")
+    model.extend(cache, _ids(3, 20, seed=2))  # leaves other nodes behind, never accepted
+    model.extend(cache, ids, counts=counts)
+    counts.fill_(1)
+    cache.accept()
+    cache.check()
+    assert cache.lengths.tolist() == [20, 3, 11] == cache.seen.tolist()
+    logits = model.extend(cache, token)
+    for b, n in enumerate((20, 3, 11)):
+        alone = model.new_cache(1, capacity=64)
+        model.extend(alone, ids[b:b + 1, :n])
+        alone.accept()
+        _near(cache.keys[:, b, :, :n], alone.keys[:, 0, :, :n])
+        _near(logits[b], model.extend(alone, token[b:b + 1])[0])
+        total = cache.weights[:, b, :, :n].sum(-1)
+        assert bool(((total - n).abs() <= 1e-3 * n).all())
+
+
+def test_a_path_ends_at_a_sequences_nodes():
+    from ppy_b200.runtime import B200Error
+
+    cache, before = _pending_cache((20, 7, 9), 6, 64)
+    counts = torch.tensor([6, 3, 0], dtype=torch.int32, device="cuda")
+    cache.pending = (*cache.pending, counts)
+    path = [[0, 4, 5], [1, 2, 4], [0, 1, 2]]
+    cache.accept(torch.tensor(path, dtype=torch.int32, device="cuda"))
+    with pytest.raises(B200Error, match="out of range"):
+        cache.check()
+    assert cache.lengths.tolist() == [23, 9, 9]
+    _plain_accept(cache, before, path, [3, 2, 0], 6)
