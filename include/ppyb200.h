@@ -263,7 +263,8 @@ int32_t ppyb200_attention_causal_bf16(const uint16_t *qkv, uint16_t *out, int64_
  * head_dim: q, k_new, v_new and out by (batch, node, head), keys and values by (batch, head,
  * slot); parents by its batch stride (0: one tree for all). out has q's type; lse (may be NULL)
  * is f32 [batch][heads][nodes], the natural log of each row's sum of e^score. Rows of nodes at
- * and behind counts[b] are left as they were, and so are the slots behind the last node.
+ * and behind counts[b] are left as they were, and so are the slots behind the last node; out and
+ * lse of nodes that do not fit behind the length are zeros.
  * bf16 or f16, head_dim a multiple of 8 up to 128, rows on 16-byte boundaries. A length or count
  * outside the buffers is held inside them, a parent that is no earlier node is taken for -1; both
  * raise *status (may be NULL) to 2. q, k_new and v_new do not overlap the cache or out. No

@@ -94,7 +94,7 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
   const int gid = lane >> 2, tig = lane & 3;
   const int group = deal.group, d = (int)a.head_dim;
   Walk<kTile, false> walk;
-  walk.measure(a, deal, blockIdx.x == 0 ? a.status : nullptr);
+  walk.measure(a, deal, blockIdx.x == 0);
   walk.enter(a, deal, blockIdx.x);
   Segment seg;
   while (walk.next(a, deal, seg)) {

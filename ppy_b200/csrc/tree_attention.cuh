@@ -29,6 +29,22 @@ __device__ __forceinline__ void sequence_extent(const Args& a, int b, int& lengt
   if (length != l || count != n) raise(status);
 }
 
+// Zeros as the results of the nodes from `count` on that did not fit behind the length.
+__device__ __forceinline__ void clear_dropped(const Args& a, int b, int count) {
+  const int nodes = (int)a.nodes, n = a.counts != nullptr ? min(a.counts[b], nodes) : nodes;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_strides[0];
+#pragma unroll 1
+  for (int node = count; node < n; ++node)
+#pragma unroll 1
+    for (int head = 0; head < (int)a.heads; ++head) {
+      uint16_t* row = out + node * a.out_strides[1] + head * a.out_strides[2];
+#pragma unroll 1
+      for (int x = 0; x < (int)a.head_dim; x += 8)
+        *reinterpret_cast<uint4*>(row + x) = make_uint4(0, 0, 0, 0);
+      if (a.lse != nullptr) a.lse[((int64_t)b * a.heads + head) * nodes + node] = 0.f;
+    }
+}
+
 // How the work is dealt to CTAs. An item is a piece of one sequence's rows (item_rows of them) under
 // one key head; its work is the key tiles it reads. All items, key head by key head, lie on one
 // axis of tiles, and CTA c of G takes the tiles [c W / G, (c + 1) W / G) of it: equal shares
@@ -84,15 +100,16 @@ struct Walk {
   int own;              // tiles of the lane-th item, for `enter`
   int left, offset, ctas, cta, kvh, item;
 
-  // A warp together. Extents that are out of range raise `status`.
-  __device__ __forceinline__ void measure(const Args& a, const Deal& deal, int32_t* status) {
+  // A warp together. The first CTA's warps report extents that are out of range.
+  __device__ __forceinline__ void measure(const Args& a, const Deal& deal, bool report) {
     const int lane = threadIdx.x & 31, items = (int)a.batch * deal.items;
     span = 0;
     own = 0;
 #pragma unroll 1
     for (int i = lane; i < items; i += 32) {
       int length, count;
-      sequence_extent(a, i / deal.items, length, count, status);
+      sequence_extent(a, i / deal.items, length, count, report ? a.status : nullptr);
+      if (report && count < (int)a.nodes) clear_dropped(a, i / deal.items, count);
       const int tiles = item_tiles<TILE, APART>(a, deal, length, count, i % deal.items);
       if (i < 32) own = tiles;
       span += tiles;

@@ -259,7 +259,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
   // the set-up above overlaps the previous kernel; its results are needed from here on
   pdl_wait();
   Walk<kKeysTile, true> walk;
-  walk.measure(a, deal, blockIdx.x == 0 ? a.status : nullptr);
+  walk.measure(a, deal, blockIdx.x == 0);
   walk.enter(a, deal, blockIdx.x);
   const int group = deal.group, d = (int)a.head_dim;
   // Stream t of a segment walks its tiles t, t + 2, ..., or all of them when the streams share

@@ -74,7 +74,7 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
 
     out [batch, nodes, heads, head_dim] of q's type and lse f32 [batch, heads, nodes], the natural
     log of the sum of e^score of each row (made here unless given; behind a sequence's nodes they
-    are left as they were, zeros when made here). Node i is written to slot lengths[b] + i of keys
+    are left as they were, zeros when made here, and zeros for nodes that do not fit in the cache). Node i is written to slot lengths[b] + i of keys
     and values; `lengths` stay as they are (`accept_nodes` says which nodes join).
 
     bf16 or f16; head_dim a multiple of 8 up to 128; rows on 16-byte boundaries; up to 256 nodes

@@ -250,3 +250,38 @@ def test_a_path_ends_at_a_sequences_nodes():
         cache.check()
     assert cache.lengths.tolist() == [23, 9, 9]
     _plain_accept(cache, before, path, [3, 2, 0], 6)
+
+
+# ---------------------------------------------------------------- outputs
+
+
+@pytest.mark.parametrize("nodes,heads,kv,cap,tree", [
+    (5, 4, 2, 200, True),        # the kernel of few rows
+    (70, 8, 2, 300, False),      # the tensor-core kernel
+    (12, 8, 2, 40_000, True),    # that, with copies of its rows
+])
+@pytest.mark.parametrize("padded", [False, True])
+def test_nodes_that_do_not_fit_have_zeros(nodes, heads, kv, cap, tree, padded):
+    lengths = (cap - nodes, cap - 3, cap, 10)
+    counts = (nodes, nodes - 1, 4, 2) if padded else None
+    x = Inputs(lengths, nodes, heads, kv, 64, tree=tree, counts=counts, spare=0)
+    x.keys, x.values = x.keys[:, :, :cap], x.values[:, :, :cap]
+    out = torch.full_like(x.q, 7.0, memory_format=torch.contiguous_format)
+    lse = torch.full((4, heads, nodes), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x.call(out=out, lse=lse, status=status)
+    assert int(status) == 2
+    made, made_lse = x.call()
+    for b, length in enumerate(lengths):
+        n = nodes if counts is None else counts[b]
+        fit = min(n, cap - length)
+        assert bool(lse[b, :, :fit].ne(5.0).all()) and bool(out[b, :fit].ne(7.0).any(-1).all())
+        assert not out[b, fit:n].any() and not lse[b, :, fit:n].any()
+        assert bool((out[b, n:] == 7.0).all()) and bool((lse[b, :, n:] == 5.0).all())
+        assert not made[b, fit:].any() and not made_lse[b, :, fit:].any()
+    # what fits is right: the same nodes as counts that say so
+    y = Inputs(lengths, nodes, heads, kv, 64, tree=tree, spare=0, counts=[
+        min(nodes if counts is None else counts[b], cap - n) for b, n in enumerate(lengths)])
+    y.keys, y.values = y.keys[:, :, :cap], y.values[:, :, :cap]
+    want, want_lse = y.call()
+    assert torch.equal(made, want) and torch.equal(made_lse, want_lse)
