@@ -64,7 +64,7 @@ inline bool narrow_faster(const Args& a) {
 }
 
 inline bool wide_takes(const Args& a) {
-  return wide_fits(a) && !narrow_faster(a) && a.scale > 0 &&
+  return wide_fits(a) && !narrow_faster(a) && a.scale > 0 && a.capacity > 0 &&
          strides_fit(a.q_strides, a.batch, a.nodes, a.heads) &&
          strides_fit(a.k_new_strides, a.batch, a.nodes, a.kv_heads) &&
          strides_fit(a.v_new_strides, a.batch, a.nodes, a.kv_heads) &&

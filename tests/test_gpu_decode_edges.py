@@ -285,3 +285,13 @@ def test_nodes_that_do_not_fit_have_zeros(nodes, heads, kv, cap, tree, padded):
     y.keys, y.values = y.keys[:, :, :cap], y.values[:, :, :cap]
     want, want_lse = y.call()
     assert torch.equal(made, want) and torch.equal(made_lse, want_lse)
+
+
+@pytest.mark.parametrize("nodes", [1, 80])
+def test_a_cache_without_slots(nodes):
+    """No node fits: zeros and the status, from either kernel's sizes."""
+    x = Inputs((0,), nodes, 4, 2, 64, tree=False)
+    x.keys, x.values = x.keys[:, :, :0], x.values[:, :, :0]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = x.call(status=status)
+    assert int(status) == 2 and not out.any() and not lse.any()
