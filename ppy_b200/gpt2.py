@@ -244,6 +244,9 @@ class GPT2:
             torch_calls.whole("parents", parents, (nodes,) if shared else (batch, nodes),
                           torch.int32, ids.get_device())
             stride = 0 if shared else nodes
+            if nodes > decode.TREE_NODES:
+                raise runtime.B200Error(f"a tree has at most {decode.TREE_NODES} nodes (a chain "
+                                        "may be longer)")
         if counts is not None:
             torch_calls.whole("counts", counts, (batch,), torch.int32, ids.get_device())
             counts = counts.clone()  # `accept` needs them too, and the caller may have changed them
@@ -265,6 +268,7 @@ class GPT2:
         pitch = self._row_pitch(logits, batch, nodes, v)
         ln = self.layernorm.device.layernorm_bf16
         heads = (batch, nodes, 3, cfg.heads, cfg.head_dim)
+        cache.pending = None  # from here on its buffers and slots are this extension's
         beside = torch_calls.begin(ids.get_device())
         try:
             st = cache.status.data_ptr()

@@ -295,3 +295,19 @@ def test_a_cache_without_slots(nodes):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     out, lse = x.call(status=status)
     assert int(status) == 2 and not out.any() and not lse.any()
+
+
+def test_a_refused_extension_leaves_the_pending_one():
+    from ppy_b200.runtime import B200Error
+
+    model, cache = _model_and_cache(1, 400)
+    ids = _ids(1, 300)
+    model.extend(cache, ids)
+    parents = torch.arange(-1, 299, dtype=torch.int32, device="cuda")
+    with pytest.raises(B200Error, match="256 nodes"):
+        model.extend(cache, _ids(1, 300, seed=1), parents)
+    cache.accept()
+    alone = model.new_cache(1, capacity=400)
+    model.extend(alone, ids)
+    alone.accept()
+    assert torch.equal(cache.keys, alone.keys) and torch.equal(cache.weights, alone.weights)
