@@ -307,18 +307,25 @@ class KVCache:
         self.seen = torch.zeros(batch, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.pending = None
-        self.buffers: dict = {}  # an extension's activations, by its shape
+        self.buffers: dict = {}  # the activations of the largest extension so far
 
     @property
     def capacity(self) -> int:
         return self.keys.shape[3]
 
+    def release(self) -> None:
+        """Give back the activations, a pending extension's among them."""
+        self.pending = None
+        for t in self.buffers.values():  # work on them may be under way on this stream
+            t.record_stream(torch.cuda.current_stream(t.device))
+        self.buffers.clear()
+
     def reset(self) -> None:
-        """Forget every sequence."""
+        """Forget every sequence, and release the activations."""
+        self.release()
         self.lengths.zero_()
         self.seen.zero_()
         self.status.zero_()
-        self.pending = None
 
     def check(self) -> None:
         """Raise if an index given to a call since the last check was out of range (syncs)."""

@@ -24,6 +24,7 @@ here, the same numbers side by side.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -218,6 +219,27 @@ class GPT2:
                               cfg.context if capacity is None else capacity,
                               device=self.device, weights=weights)
 
+    def _activations(self, cache: decode.KVCache, batch: int, nodes: int) -> dict:
+        """An extension's activations: views of the largest set that the cache needed so far. A
+        captured extension gets a set of its own, from the graph's memory, since the cache's may be
+        replaced before the graph is replayed."""
+        import torch
+
+        cfg, tokens = self.config, batch * nodes
+        layers, c = cfg.layers if cache.weights is not None else 1, cfg.width
+        shapes = {"x": (tokens, c), "h": (tokens, c), "qkv": (layers, tokens, 3 * c),
+                  "lse": (layers, batch, cfg.heads, nodes), "att": (tokens, c),
+                  "f": (tokens, 4 * c)}
+        kept = {} if torch.cuda.is_current_stream_capturing() else cache.buffers
+        if not kept or kept["x"].numel() < tokens * c:
+            if kept:
+                cache.release()
+            for name, shape in shapes.items():
+                kept[name] = torch.empty(
+                    math.prod(shape), device=cache.keys.device,
+                    dtype=torch.float32 if name in ("x", "lse") else torch.bfloat16)
+        return {name: kept[name][:math.prod(shape)].view(shape) for name, shape in shapes.items()}
+
     def extend(self, cache: decode.KVCache, ids, parents=None, counts=None, logits=None):
         """Logits [batch, nodes, vocab] (f32, laid out as forward's) of drafted tokens `ids` (int64
         [batch, nodes]) behind the sequences of `cache`: a tree by `parents` (int32 [batch, nodes]
@@ -250,25 +272,17 @@ class GPT2:
         if counts is not None:
             torch_calls.whole("counts", counts, (batch,), torch.int32, ids.get_device())
             counts = counts.clone()  # `accept` needs them too, and the caller may have changed them
-        s = cache.buffers.get((batch, nodes))
-        if s is None:
-            d = ids.device
-            layers = cfg.layers if cache.weights is not None else 1
-            s = {"x": torch.empty(tokens, c, dtype=torch.float32, device=d),
-                 "h": torch.empty(tokens, c, dtype=torch.bfloat16, device=d),
-                 "qkv": torch.empty(layers, tokens, 3 * c, dtype=torch.bfloat16, device=d),
-                 "lse": torch.zeros(layers, batch, cfg.heads, nodes, device=d),
-                 # rows behind a sequence's nodes are left alone: zeros from the start
-                 "att": torch.zeros(tokens, c, dtype=torch.bfloat16, device=d),
-                 "f": torch.empty(tokens, 4 * c, dtype=torch.bfloat16, device=d)}
-            cache.buffers[(batch, nodes)] = s
-        x, h, att, f, lib = s["x"], s["h"], s["att"], s["f"], self.lib
         if logits is None:
             logits = self.new_logits(batch, nodes)
         pitch = self._row_pitch(logits, batch, nodes, v)
+        cache.pending = None  # from here on its buffers and slots are this extension's
+        s = self._activations(cache, batch, nodes)
+        if counts is not None:  # the attention leaves rows behind a sequence's nodes alone
+            s["att"].zero_()
+            s["lse"].zero_()
+        x, h, att, f, lib = s["x"], s["h"], s["att"], s["f"], self.lib
         ln = self.layernorm.device.layernorm_bf16
         heads = (batch, nodes, 3, cfg.heads, cfg.head_dim)
-        cache.pending = None  # from here on its buffers and slots are this extension's
         beside = torch_calls.begin(ids.get_device())
         try:
             st = cache.status.data_ptr()

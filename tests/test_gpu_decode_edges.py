@@ -311,3 +311,90 @@ def test_a_refused_extension_leaves_the_pending_one():
     model.extend(alone, ids)
     alone.accept()
     assert torch.equal(cache.keys, alone.keys) and torch.equal(cache.weights, alone.weights)
+
+
+# ---------------------------------------------------------------- memory between calls
+
+
+def test_activations_do_not_pile_up():
+    """Extensions of many shapes hold one set of activations, as large as the largest of them, and a
+    reset gives it back; what they compute is what caches of their own get."""
+    model, cache = _model_and_cache(2, 300, layers=2)
+    model.extend(cache, _ids(2, 1))  # everything that is made once
+    cache.reset()
+    # bytes asked of the allocator: what it hands out is rounded up, by up to 1 MB a tensor
+    asked = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]  # noqa: E731
+    start, largest = asked(), 0
+    for step, length in enumerate((200, 3, 17, 1, 64, 5, 130)):
+        cache.reset() if step else None
+        ids = _ids(2, length, seed=step)
+        logits = model.extend(cache, ids)
+        held = asked() - start - 2 * length * (8 + 4 * 50272)  # ids and padded logits
+        tokens, c = 2 * length, model.config.width
+        # x, h, two layers' qkv, att and f, and the log sums
+        assert held == tokens * c * (4 + 2 + 2 * 6 + 2 + 8) + 2 * tokens * 12 * 4
+        del logits, ids
+    cache.reset()
+    for length in (64, 5, 200, 1, 130):  # without a reset in between: as large as the largest
+        ids = _ids(2, length, seed=length)
+        got = model.extend(cache, ids)
+        alone = model.new_cache(2, capacity=300)
+        model.extend(cache, ids)
+        assert torch.equal(got, model.extend(alone, ids))
+        largest = max(largest, length)
+        sizes = {name: t.numel() for name, t in cache.buffers.items()}
+        assert sizes["x"] == 2 * largest * model.config.width
+        cache.pending = None
+        del got, alone
+
+
+def test_a_captured_extension_has_its_own_activations():
+    """The cache's set may be replaced by a larger one, or released, between capture and replay."""
+    from ppy_b200 import runtime
+
+    model, cache = _model_and_cache(2, 200)
+    prompt, tokens = _ids(2, 90, seed=3), _ids(2, 3, seed=4)
+    stream = torch.cuda.Stream()
+    runtime.set_stream(stream)
+    try:
+        with torch.cuda.stream(stream):
+            token, logits = torch.zeros(2, 1, dtype=torch.int64, device="cuda"), model.new_logits(2, 1)
+            model.extend(cache, token, logits=logits)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                model.extend(cache, token, logits=logits)
+                cache.accept()
+            cache.reset()
+            model.extend(cache, prompt)
+            cache.accept()
+            other = model.new_cache(2, capacity=200)
+            model.extend(other, prompt)
+            other.accept()
+            for i in range(3):
+                if i == 1:
+                    cache.release()
+                junk = torch.full((1 << 22,), math.nan, device="cuda")
+                token.copy_(tokens[:, i:i + 1])
+                graph.replay()
+                want = model.extend(other, tokens[:, i:i + 1])
+                other.accept()
+                assert torch.equal(logits, want), i
+                del junk
+            assert torch.equal(cache.lengths, other.lengths)
+            assert torch.equal(cache.weights, other.weights)
+        stream.synchronize()
+    finally:
+        runtime.set_stream(torch.cuda.current_stream())
+
+
+def test_padded_rows_stay_finite_after_other_extensions():
+    """The activations of an extension before lie in the rows behind a sequence's nodes."""
+    model, cache = _model_and_cache(2, 64)
+    model.extend(cache, _ids(2, 8))
+    for t in cache.buffers.values():
+        t.fill_(math.nan)
+    cache.pending = None
+    logits = model.extend(cache, _ids(2, 8), counts=torch.tensor([8, 2], dtype=torch.int32,
+                                                                 device="cuda"))
+    assert bool(logits.isfinite().all())
