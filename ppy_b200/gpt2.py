@@ -328,14 +328,21 @@ class GPT2:
     def score(self, ids, top: int = 0, logits=None) -> scoring.TokenLogprobs:
         """Log probabilities of tokens 1, 2, ... of `ids` [batch, length] given those before them,
         the entropy of each prediction and its `top` alternatives (`scoring.token_logprobs`), all
-        [batch, length - 1, ...], from one forward (`logits` as for it)."""
+        [batch, length - 1, ...], from one forward over the length rounded up to a multiple of
+        128, which is to lie within the context (`logits`, where given, has room for that length)."""
         import torch
 
-        logits = self.forward(ids, logits)
-        following = torch.full_like(ids, -1, memory_format=torch.contiguous_format)
-        following[:, :-1] = ids[:, 1:]
+        batch, length = ids.shape
+        if ids.dtype != torch.int64 or ids.get_device() < 0 or length == 0:
+            raise runtime.B200Error("ids: int64 [batch, length] on a CUDA device, not empty")
+        # tokens behind the last are seen by none before them
+        whole = (length + 127) // 128 * 128
+        padded = torch.nn.functional.pad(ids, (0, whole - length))
+        following = torch.full_like(padded, -1)
+        following[:, :length - 1] = ids[:, 1:]
+        logits = self.forward(padded, logits)
         scored = scoring.token_logprobs(logits, following, top)
-        return scoring.TokenLogprobs(*(t[:, :-1] for t in scored))
+        return scoring.TokenLogprobs(*(t[:, :length - 1] for t in scored))
 
     def profile(self, ids, logits=None) -> dict:
         """One forward with CUDA events around every call: {kernel: [launches, ms, flops]}.

@@ -398,3 +398,39 @@ def test_padded_rows_stay_finite_after_other_extensions():
     logits = model.extend(cache, _ids(2, 8), counts=torch.tensor([8, 2], dtype=torch.int32,
                                                                  device="cuda"))
     assert bool(logits.isfinite().all())
+
+
+# ---------------------------------------------------------------- scoring texts
+
+
+@pytest.mark.parametrize("batch,length", [(1, 1), (2, 2), (3, 37), (2, 128), (1, 129), (1, 1000)])
+def test_score_texts_of_any_length(batch, length):
+    from oracle import gpt2 as oracle_gpt2
+
+    model, _ = _model_and_cache(1, 1)
+    ids = _ids(batch, length + 3, seed=length)[:, :length]  # rows of a larger tensor
+    scores = model.score(ids, top=3)
+    assert scores.logprobs.shape == scores.entropy.shape == (batch, length - 1)
+    assert scores.top_tokens.shape == scores.top_logprobs.shape == (batch, length - 1, 3)
+    room = model.new_logits(batch, (length + 127) // 128 * 128)
+    again = model.score(ids, top=3, logits=room)
+    assert all(torch.equal(a, b) for a, b in zip(scores, again))
+    rows = room[:, :length - 1].double()
+    want = torch.log_softmax(rows, -1)
+    # the bound of the scores given their logits (test_gpu_scoring.py)
+    picked = want.gather(-1, ids[:, 1:, None])[..., 0]
+    assert bool(((scores.logprobs.double() - picked).abs() < 1e-4).all())
+    assert bool((scores.top_logprobs.double() - want.topk(3, -1).values).abs().lt(1e-4).all())
+    if length > 1:  # and the logits are those of the text without its padding
+        _near(rows, oracle_gpt2.forward(model, ids.contiguous())[:, :-1])
+
+
+def test_score_refusals():
+    from ppy_b200.runtime import B200Error
+
+    model, _ = _model_and_cache(1, 1)
+    for ids in (_ids(1, 5).int(), _ids(1, 5).cpu(), _ids(1, 0), _ids(1, 1025)):
+        with pytest.raises(B200Error):
+            model.score(ids)
+    with pytest.raises(B200Error, match="logits"):
+        model.score(_ids(1, 5), logits=model.new_logits(1, 5))
