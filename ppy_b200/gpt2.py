@@ -340,7 +340,11 @@ class GPT2:
         padded = torch.nn.functional.pad(ids, (0, whole - length))
         following = torch.full_like(padded, -1)
         following[:, :length - 1] = ids[:, 1:]
-        logits = self.forward(padded, logits)
+        beside = torch_calls.begin(ids.get_device())
+        try:
+            logits = self.forward(padded, logits)
+        finally:
+            torch_calls.end(beside)
         scored = scoring.token_logprobs(logits, following, top)
         return scoring.TokenLogprobs(*(t[:, :length - 1] for t in scored))
 

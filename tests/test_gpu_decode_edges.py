@@ -425,6 +425,26 @@ def test_score_texts_of_any_length(batch, length):
         _near(rows, oracle_gpt2.forward(model, ids.contiguous())[:, :-1])
 
 
+def test_score_beside_torchs_stream():
+    """ids made on torch's stream while the launches go to another: no wait by the caller."""
+    from ppy_b200 import runtime
+
+    model, _ = _model_and_cache(1, 1)
+    ids = _ids(2, 200)
+    want = model.score(ids, top=2)
+    torch.cuda.synchronize()
+    try:
+        for stream in (None, torch.cuda.Stream()):
+            runtime.set_stream(stream)
+            for _ in range(5):
+                held = torch.randn(4096, 4096, device="cuda")
+                held = held @ held  # work before the inputs on torch's stream
+                got = model.score(ids + 0, top=2)
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+    finally:
+        runtime.set_stream(torch.cuda.current_stream())
+
+
 def test_score_refusals():
     from ppy_b200.runtime import B200Error
 
