@@ -18,6 +18,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "../../include/ppyb200.h"
 #include "mma16.cuh"
 #include "ppyb200_device.cuh"
@@ -53,6 +55,12 @@ template <int D>
 __device__ __forceinline__ uint32_t row_piece(int row, int piece) {
   return (uint32_t)(row * D * 2 + ((piece ^ (row & 7)) << 4));
 }
+
+// Weights are held times 2^kLift until they are divided by their sum, which is lifted too: f16 ends
+// at 2^-24, and where a long cache has many small weights, what they lose together would show
+// (60000 weights of e^-18 beside one of 1 were zeros). 2^15 is f16's last power of two.
+template <class T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
 
 // A row's result from its sums, by a warp: lane l holds columns 64 i + 2 l, +1.
 template <class T, int D>
@@ -270,6 +278,7 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
       // a row that has seen nothing yet keeps its maximum at -inf; its terms are 2^-inf = 0
       const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
       const float f0 = exp2_sfu(m0 - u0), f1 = exp2_sfu(m1 - u1);
+      const float v0 = u0 - kLift<T>, v1 = u1 - kLift<T>;
       m0 = x0;
       m1 = x1;
       l0 *= f0;
@@ -283,10 +292,10 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
       }
 #pragma unroll
       for (int n = 0; n < kKeys / 8; ++n) {
-        s[n][0] = exp2_sfu(s[n][0] - u0);
-        s[n][1] = exp2_sfu(s[n][1] - u0);
-        s[n][2] = exp2_sfu(s[n][2] - u1);
-        s[n][3] = exp2_sfu(s[n][3] - u1);
+        s[n][0] = exp2_sfu(s[n][0] - v0);
+        s[n][1] = exp2_sfu(s[n][1] - v0);
+        s[n][2] = exp2_sfu(s[n][2] - v1);
+        s[n][3] = exp2_sfu(s[n][3] - v1);
         l0 += s[n][0] + s[n][1];
         l1 += s[n][2] + s[n][3];
       }
@@ -332,6 +341,8 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
       }
     }
     copies_wait<0>();
+    m0 -= kLift<T>;  // from here on the reference that the sums go by
+    m1 -= kLift<T>;
 #pragma unroll
     for (int w = 1; w < 4; w <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, w);

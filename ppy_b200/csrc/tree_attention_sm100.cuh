@@ -15,7 +15,7 @@
 //   S = Q K^T   M = 128, N = 128, both operands K-major with the 128-byte swizzle; the query rows
 //               of a tile come as one box [nodes][heads of the group][64 columns]
 //   softmax     a row a thread, f32, the running maximum moved only when a score exceeds it by
-//               2^8 (the weights of the tile are at most 2^8 then, exact for the quotient)
+//               2^kMove (the weights of the tile are at most that then, exact for the quotient)
 //   O += P V    P from TMEM in the values' type (rounded to half a step, as the prompt
 //               attention's), V as it lies in the cache: [keys][64 columns] boxes are the
 //               MN-major form of the operand, no transposed copy
@@ -74,7 +74,14 @@ constexpr uint32_t kLaunchRegs = 168, kSoftmaxRegs = 224, kSupportRegs = 56;
 static_assert(2 * 128 * kSoftmaxRegs + 128 * kSupportRegs <= kWideThreads * kLaunchRegs,
               "register split above the launch's registers");
 constexpr uint32_t kWaitLimit = 1u << 22;
-constexpr float kMoveLog2 = 8.f;
+// The running maximum moves when a score exceeds it by more than 2^kMove, and weights are held
+// times 2^kLift until they are divided by their sum (lifted too): the two together stay within
+// f16's 2^15, whose small weights would vanish without the lift; bf16 has f32's range. A slack of
+// 2^4 in place of 2^8 costs f16 nothing measurable: maxima settle within the first tiles.
+template <class T>
+constexpr float kMove = std::is_same<T, __half>::value ? 4.f : 8.f;
+template <class T>
+constexpr float kLift = std::is_same<T, __half>::value ? 11.f : 0.f;
 
 constexpr int kBox = 128 * 64 * 2;  // 128 rows of 64 16-bit columns: one TMA box
 
@@ -540,9 +547,9 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
             mx[3] = max3(mx[3], sv[c + 6], sv[c + 7]);
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          // the maximum moves by more than kMoveLog2, or stays; a row that has seen nothing yet
+          // the maximum moves by more than 2^kMove, or stays; a row that has seen nothing yet
           // stays at -inf, its weights 2^-inf = 0
-          const bool move = top != -INFINITY && !((top - m) * scale_log2 <= kMoveLog2);
+          const bool move = top != -INFINITY && !((top - m) * scale_log2 <= kMove<T>);
           float alpha = 1.f;
           if (move) {
             alpha = m == -INFINITY ? 0.f : exp2_sfu((m - top) * scale_log2);
@@ -550,7 +557,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
             l *= alpha;
           }
           __syncwarp();
-          const float shift = m == -INFINITY ? 0.f : -m * scale_log2;
+          const float shift = m == -INFINITY ? 0.f : kLift<T> - m * scale_log2;
           const uint64_t shift2 = f2(shift, shift);
           if (!Shape::kOver && k > 0) {
             // the product before this tile's reads P, which the stores below replace
@@ -725,7 +732,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
                   make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        const float m_log2 = m == -INFINITY ? m : m * scale_log2;
+        const float m_log2 = m == -INFINITY ? m : m * scale_log2 - kLift<T>;
         if (real && seg.whole) {
           if (a.lse != nullptr)
             a.lse[((int64_t)seg.b * a.heads + head) * a.nodes + node] =

@@ -454,3 +454,38 @@ def test_score_refusals():
             model.score(ids)
     with pytest.raises(B200Error, match="logits"):
         model.score(_ids(1, 5), logits=model.new_logits(1, 5))
+
+
+# ---------------------------------------------------------------- small weights, infinities
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("length,nodes,heads,kv,cap", [
+    (60_000, 1, 1, 1, 60_100),     # the kernel of few rows
+    (60_000, 70, 1, 1, 60_100),    # the tensor-core kernel
+    (60_000, 12, 4, 4, 300_000),   # that, with copies of its rows
+])
+def test_many_small_weights(length, nodes, heads, kv, cap, dtype):
+    """One entry of weight 1 and value 0, the rest of weight e^-18 and value 1, nodes of weight 1 and
+    value 0: the small weights add up to all there is. Scores are exact; a weight is rounded to u
+    of itself, or to 2^-36 of the largest where it is subnormal, the result to u of itself; 2^-18
+    for exponentials and sums."""
+    u = {F16: 2.0 ** -11, BF16: 2.0 ** -8}[dtype]
+    x = Inputs((length,), nodes, heads, kv, 64, dtype, tree=False, spare=cap - length - nodes)
+    x.q.zero_()[..., 0] = 1
+    x.k_new.zero_()
+    x.v_new.zero_()
+    x.keys[:, :, :length] = 0
+    x.keys[:, :, 1:length, 0] = -18
+    x.values[:, :, :length] = 1
+    x.values[:, :, 0] = 0
+    out, lse = x.call(scale=1.0)
+    small = (length - 1) * math.exp(-18)
+    ones = torch.arange(2, nodes + 2, dtype=torch.float64, device="cuda")[:, None]
+    want = small / (ones + small)
+    assert bool(((out[0].double() - want[..., None]).abs()
+                 <= (2 * u + 2.0 ** -18) * want[..., None] + 2.0 ** -36 * length).all())
+    # up to 592 parts (four CTAs an SM) are added in f32 one after the other, each sum rounded by up to
+    # 2^-24 of itself: what they add is below the sum's own last bits
+    assert bool(((lse[0].double().t() - (ones + small).log()).abs()
+                 <= 2.0 ** -18 + 592 * 2.0 ** -24).all())
