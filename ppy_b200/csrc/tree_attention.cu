@@ -400,6 +400,32 @@ narrow_kernel(const __grid_constant__ Args a, const Deal deal) {
   }
 }
 
+// One column of a row whose values are not all finite, from those alone: the infinity that they add
+// up to, or NaN. For sums that came out as NaN because a result held an infinity times zero: a copy
+// of the rows weighs the keys of the others with zero.
+template <class T>
+__device__ __noinline__ float odd_value(const Args& a, int b, int kvh, int length, int node,
+                                        int col) {
+  const T* values = static_cast<const T*>(a.values) + b * a.values_strides[0] +
+                    kvh * a.values_strides[1] + col;
+  const T* v_new = static_cast<const T*>(a.v_new) + b * a.v_new_strides[0] +
+                   kvh * a.v_new_strides[2] + col;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int64_t j = 0; j < length; ++j) {
+    const float v = (float)values[j * a.values_strides[2]];
+    if (!isfinite(v)) sum += v;
+  }
+#pragma unroll 1
+  for (int i = node; i >= 0;) {  // the node and its ancestors
+    const float v = (float)v_new[i * a.v_new_strides[1]];
+    if (!isfinite(v)) sum += v;
+    const int p = a.parents == nullptr ? i - 1 : a.parents[b * a.parents_stride + i];
+    i = p < i ? p : -1;
+  }
+  return isfinite(sum) ? __uint_as_float(0x7fc00000u) : sum;
+}
+
 // Joins the unnormalised results of an item's segments in their order, a thread four columns of a
 // row. What it costs is the latency of its loads one after another, so the outputs of the first
 // eight results are under way before the maxima are known.
@@ -462,6 +488,12 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) join_kernel(const __grid_co
   const int head = kvh * deal.group + row % deal.group;
   const float inv = 1.f / l;
   if (piece * 4 < a.head_dim) {
+    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (all != all && l == l) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (sum[k] != sum[k]) sum[k] = odd_value<T>(a, b, kvh, length, node, piece * 4 + k);
+    }
     T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + node * a.out_strides[1] +
              (int64_t)head * a.out_strides[2] + piece * 4;
     *reinterpret_cast<uint2*>(out) = make_uint2(Kind<T>::pack(sum[0] * inv, sum[1] * inv),

@@ -489,3 +489,35 @@ def test_many_small_weights(length, nodes, heads, kv, cap, dtype):
     # 2^-24 of itself: what they add is below the sum's own last bits
     assert bool(((lse[0].double().t() - (ones + small).log()).abs()
                  <= 2.0 ** -18 + 592 * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lengths,nodes,heads,kv,d,cap,tree", [
+    ((70, 300), 5, 4, 2, 64, 400, True),          # the kernel of few rows
+    ((300, 31), 45, 6, 2, 128, 2_000, False),     # the tensor-core kernel
+    ((4000, 129), 1, 8, 2, 64, 270_000, False),   # four copies of its rows
+    ((1111, 500), 12, 8, 2, 128, 60_000, True),   # two copies
+])
+def test_infinities_in_the_cache(lengths, nodes, heads, kv, d, cap, tree, dtype):
+    """A cached value that is not finite is seen by every row of its key head: an infinity gives
+    infinities, two of opposite signs or a NaN give NaN, in that column and no other."""
+    x = Inputs(lengths, nodes, heads, kv, d, dtype, tree=tree, spare=cap - max(lengths) - nodes)
+    clean, clean_lse = x.call()
+    x.values[0, 0, 3, 1] = math.inf
+    x.values[0, 0, 64, 7] = -math.inf
+    x.values[0, 0, [5, 20], [9, 9]] = math.inf
+    x.values[0, 0, 2, 12] = math.inf
+    x.values[0, 0, 29, 12] = -math.inf
+    x.values[0, 0, 6, 14] = math.nan
+    x.v_new[0, 0, 0, 17] = -math.inf  # a node's, for the rows that see it
+    x.values[0, 0, 30, 17] = -math.inf
+    out, lse = x.call()
+    assert torch.equal(lse, clean_lse)
+    group = heads // kv
+    rows = out[0, :, :group].float()
+    for col, want in ((1, math.inf), (7, -math.inf), (9, math.inf), (17, -math.inf)):
+        assert bool((rows[..., col] == want).all()), col
+    assert bool(rows[..., [12, 14]].isnan().all())
+    same = torch.ones_like(out, dtype=torch.bool)
+    same[0, :, :group, [1, 7, 9, 12, 14, 17]] = False
+    assert torch.equal(out[same], clean[same])
