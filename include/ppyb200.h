@@ -267,7 +267,8 @@ int32_t ppyb200_attention_causal_bf16(const uint16_t *qkv, uint16_t *out, int64_
  * lse of nodes that do not fit behind the length are zeros.
  * bf16 or f16, head_dim a multiple of 8 up to 128, rows on 16-byte boundaries. A length or count
  * outside the buffers is held inside them, a parent that is no earlier node is taken for -1; both
- * raise *status (may be NULL) to 2. q, k_new and v_new do not overlap the cache or out. No
+ * raise *status (may be NULL) to 2, and so does a bounded wait given up inside the kernel, which
+ * leaves NaN in the rows without a result. q, k_new and v_new do not overlap the cache or out. No
  * counterpart in the reference beyond its prompt attention (examples/46_gpt2/gpt2.ppy:52). */
 typedef struct ppyb200_tree_attention_args {
   const void *q, *k_new, *v_new;
@@ -291,6 +292,11 @@ typedef struct ppyb200_tree_attention_args {
  * overlap, captured graphs among them, take one each. */
 int64_t ppyb200_tree_attention_workspace(const ppyb200_tree_attention_args *args);
 int32_t ppyb200_tree_attention(const ppyb200_tree_attention_args *args);
+
+/* For tests: how often the tensor-core kernel tries each of its waits before it gives up, in the
+ * calls that follow (0: it gives up at once; negative: the default). A call that gave up raises
+ * *status to 2 and leaves NaN in out and lse of the rows that it has no result for. */
+void ppyb200_tree_attention_wait_limit(int64_t tries);
 
 /* A verified path joins the cache. path[b][0 .. accepted[b]) are nodes of the last attention in
  * ascending order; q and lse are that attention's (layer by layer), its nodes at slots

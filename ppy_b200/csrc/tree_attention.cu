@@ -18,6 +18,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/ppyb200.h"
@@ -527,13 +528,17 @@ cudaError_t launch_narrow(const Args& a, const Plan& p, cudaStream_t stream) {
                              a, p.deal);
 }
 
+std::atomic<uint32_t> wait_limit{ppyb200::tree::kWaitLimit};
+
 template <class T, int D>
 cudaError_t launch_dim(const Args& a, const Plan& p, cudaStream_t stream) {
   using ppyb200::tree::launch_wide;
-  const cudaError_t e = !p.wide ? launch_narrow<T, D>(a, p, stream)
-                        : p.rows.copies == 4 ? launch_wide<T, D, 4>(a, p.deal, p.rows, stream)
-                        : p.rows.copies == 2 ? launch_wide<T, D, 2>(a, p.deal, p.rows, stream)
-                                             : launch_wide<T, D, 1>(a, p.deal, p.rows, stream);
+  const uint32_t limit = wait_limit.load(std::memory_order_relaxed);
+  const cudaError_t e =
+      !p.wide ? launch_narrow<T, D>(a, p, stream)
+      : p.rows.copies == 4 ? launch_wide<T, D, 4>(a, p.deal, p.rows, limit, stream)
+      : p.rows.copies == 2 ? launch_wide<T, D, 2>(a, p.deal, p.rows, limit, stream)
+                           : launch_wide<T, D, 1>(a, p.deal, p.rows, limit, stream);
   return e == cudaSuccess && p.deal.join ? join<T, D>(a, p, stream) : e;
 }
 
@@ -571,6 +576,12 @@ const char* refusal(const ppyb200_tree_attention_args& a) {
 }  // namespace
 
 extern "C" {
+
+void ppyb200_tree_attention_wait_limit(int64_t tries) {
+  wait_limit.store(tries < 0 || tries > ppyb200::tree::kWaitLimit ? ppyb200::tree::kWaitLimit
+                                                                  : (uint32_t)tries,
+                   std::memory_order_relaxed);
+}
 
 int64_t ppyb200_tree_attention_workspace(const ppyb200_tree_attention_args* args) {
   if (args == nullptr || refusal(*args) != nullptr || args->batch == 0 || args->nodes == 0)

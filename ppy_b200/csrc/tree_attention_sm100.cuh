@@ -33,7 +33,8 @@
 //   warp 11    appends a segment's nodes to the cache, unless they are many
 //
 // Every mbarrier wait is bounded: on giving up the CTA raises the status, every role leaves its
-// loop, copies and MMAs in flight are drained and the TMEM is freed.
+// loop, copies and MMAs in flight are drained and the TMEM is freed. Rows left without a result get
+// NaN, so that a caller without a status word does not take old memory for one.
 #pragma once
 
 #include <cuda.h>
@@ -73,7 +74,7 @@ constexpr int kWideThreads = 384;
 constexpr uint32_t kLaunchRegs = 168, kSoftmaxRegs = 224, kSupportRegs = 56;
 static_assert(2 * 128 * kSoftmaxRegs + 128 * kSupportRegs <= kWideThreads * kLaunchRegs,
               "register split above the launch's registers");
-constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr uint32_t kWaitLimit = 1u << 22;  // tries of an mbarrier wait, unless a test sets others
 // The running maximum moves when a score exceeds it by more than 2^kMove, and weights are held
 // times 2^kLift until they are divided by their sum (lifted too): the two together stay within
 // f16's 2^15, whose small weights would vanish without the lift; bf16 has f32's range. A slack of
@@ -145,8 +146,8 @@ struct WideMaps {
 
 template <class Layout>
 __device__ __forceinline__ bool wide_wait(Layout& s, uint64_t* bar, uint32_t parity,
-                                          int32_t* status) {
-  for (uint32_t tries = 0; tries < kWaitLimit; ++tries) {
+                                          int32_t* status, uint32_t limit) {
+  for (uint32_t tries = 0; tries < limit; ++tries) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*(volatile int*)&s.abort) return false;
   }
@@ -156,8 +157,8 @@ __device__ __forceinline__ bool wide_wait(Layout& s, uint64_t* bar, uint32_t par
 }
 template <class Layout>
 __device__ __forceinline__ bool wide_warp_wait(Layout& s, uint64_t* bar, uint32_t parity,
-                                               int32_t* status) {
-  return __all_sync(0xffffffffu, wide_wait(s, bar, parity, status)) != 0;
+                                               int32_t* status, uint32_t limit) {
+  return __all_sync(0xffffffffu, wide_wait(s, bar, parity, status, limit)) != 0;
 }
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
@@ -223,10 +224,41 @@ __device__ __forceinline__ Sight node_sight(const uint8_t* parents, int node, in
   }
 }
 
+// After a wait that gave up: NaN as the result of a softmax thread's row of every segment of the CTA's,
+// those that it had finished among them. A function of its own, for the registers' sake.
+template <class T, int D, int COPIES>
+__device__ __noinline__ void leave_nan(const Args& a, const Deal& deal, const WideRows& wide) {
+  const int lane_row = threadIdx.x % 128, t = threadIdx.x / 128;
+  const int row = lane_row % (128 / COPIES), copy = lane_row / (128 / COPIES);
+  const float nan = __uint_as_float(0x7fc00000u);
+  const Results results(a, deal, D);
+  Walk<kKeysTile, true> walk;
+  walk.measure(a, deal, false);
+  walk.enter(a, deal, blockIdx.x);
+  Segment seg;
+  while (walk.next(a, deal, seg)) {
+    const int tile_row = (wide.share ? t * wide.tile_nodes * deal.group : 0) + row;
+    const int node = (seg.row0 + tile_row) / deal.group;
+    const int head = seg.kvh * deal.group + tile_row % deal.group;
+    if (row >= wide.tile_nodes * deal.group || node >= seg.count) continue;
+    if (!seg.whole) {
+      results.top_of(seg.result + (wide.share ? 0 : t * COPIES + copy), tile_row) =
+          make_float2(nan, nan);
+      continue;
+    }
+    T* out = static_cast<T*>(a.out) + seg.b * a.out_strides[0] + node * a.out_strides[1] +
+             head * a.out_strides[2];
+    for (int x = 0; x < (int)a.head_dim; x += 2)
+      *reinterpret_cast<uint32_t*>(out + x) = Kind<T>::pack(nan, nan);
+    if (a.lse != nullptr) a.lse[((int64_t)seg.b * a.heads + head) * a.nodes + node] = nan;
+  }
+}
+
 template <class T, int D, int COPIES>
 __global__ void __launch_bounds__(kWideThreads, 1)
 wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args a,
-            const Deal deal, const WideRows wide) {
+            const __grid_constant__ Deal deal, const __grid_constant__ WideRows wide,
+            const uint32_t limit) {
   using Shape = WideShape<D>;
   constexpr int kSpan = 128 / COPIES;  // rows of a copy, and keys of a tile that it weighs
   extern __shared__ uint8_t smem_raw[];
@@ -310,7 +342,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           parent[i] = i * 32 + lane < seg.count ? from[i * 32 + lane] : -1;
       }
       if (lane == 0) {
-        ok = wide_wait(s, &s.q_empty, (uint32_t)((segments & 1) ^ 1), a.status);
+        ok = wide_wait(s, &s.q_empty, (uint32_t)((segments & 1) ^ 1), a.status, limit);
         if (ok) {
           const int streams = both_of(seg) ? 2 : 1;
           const int node0 = seg.row0 / group;
@@ -346,7 +378,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
             const int t = wide.share ? 0 : (tile - seg.first) & 1;
             for (int v = 0; v < 2; ++v) {
               const Entry<D> entry(wide.share, t, t == 0 ? loaded[0] : loaded[1]);
-              if (!wide_wait(s, &s.empty[entry.slot], entry.parity ^ 1, a.status)) {
+              if (!wide_wait(s, &s.empty[entry.slot], entry.parity ^ 1, a.status, limit)) {
                 ok = false;
                 break;
               }
@@ -387,7 +419,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       int base = 0, n = 0, segments = 0;  // tiles so far: of both streams, and of this one
       bool ok = true;
       auto full = [&](const Entry<D>& entry) {
-        return wide_wait(s, &s.full[entry.slot], entry.parity, a.status);
+        return wide_wait(s, &s.full[entry.slot], entry.parity, a.status, limit);
       };
       auto entry_of = [&](int k, int v) {  // K (v = 0) or V of this stream's tile k
         return Entry<D>(wide.share, t, 2 * ((wide.share ? base : n) + k) + v);
@@ -397,7 +429,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         const Entry<D> entry = entry_of(k, 0);
         if (!full(entry)) return false;
         if (!Shape::kOver && n + k > 0 &&
-            !wide_wait(s, &s.s_free[t], (uint32_t)((n + k - 1) & 1), a.status))
+            !wide_wait(s, &s.s_free[t], (uint32_t)((n + k - 1) & 1), a.status, limit))
           return false;
         tc_fence_after();
         const uint8_t* key = s.ring[entry.slot];
@@ -415,7 +447,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       // O += P V of tile k
       auto product = [&](int k) -> bool {
         const Entry<D> entry = entry_of(k, 1);
-        if (!full(entry) || !wide_wait(s, &s.p_full[t], (uint32_t)((n + k) & 1), a.status))
+        if (!full(entry) || !wide_wait(s, &s.p_full[t], (uint32_t)((n + k) & 1), a.status, limit))
           return false;
         tc_fence_after();
         const uint64_t value = smem_desc_mn(s.ring[entry.slot]);
@@ -429,7 +461,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       };
       for (; ok && walk.next(a, deal, seg); ++segments) {
         const int mine = count_of(seg, t);
-        if (!wide_wait(s, &s.q_full, (uint32_t)(segments & 1), a.status)) break;
+        if (!wide_wait(s, &s.q_full, (uint32_t)(segments & 1), a.status, limit)) break;
         if (mine == 0) {
           mbar_arrive(&s.q_empty);
           for (int i = 0; wide.share && ok && i < 2 * seg.tiles; ++i) {
@@ -503,7 +535,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       float m = -INFINITY, l = 0.f;  // m in raw score units
       for (int k = 0; k < mine; ++k) {
         const uint32_t phase = (uint32_t)((n + k) & 1);
-        if (!wide_warp_wait(s, &s.s_full[t], phase, a.status)) {
+        if (!wide_warp_wait(s, &s.s_full[t], phase, a.status, limit)) {
           ok = false;
           break;
         }
@@ -561,7 +593,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           const uint64_t shift2 = f2(shift, shift);
           if (!Shape::kOver && k > 0) {
             // the product before this tile's reads P, which the stores below replace
-            if (!wide_warp_wait(s, &s.o_done[t], phase ^ 1, a.status)) {
+            if (!wide_warp_wait(s, &s.o_done[t], phase ^ 1, a.status, limit)) {
               ok = false;
               break;
             }
@@ -571,7 +603,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           // take twice as long and leave the tensor core idle for as long.
           if (turns && (t == 1 || turn > 0) &&
               !wide_warp_wait(s, &s.turn[t], (uint32_t)((turn - (t == 0 ? 1 : 0)) & 1),
-                              a.status)) {
+                              a.status, limit)) {
             ok = false;
             break;
           }
@@ -625,7 +657,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           // a phase of p_full would stand for another's
           if (!Shape::kOver) {
             if (lane == 0) mbar_arrive(&s.s_free[t]);
-            if (k > 0 && !wide_warp_wait(s, &s.o_done[t], phase ^ 1, a.status)) {
+            if (k > 0 && !wide_warp_wait(s, &s.o_done[t], phase ^ 1, a.status, limit)) {
               ok = false;
               break;
             }
@@ -633,7 +665,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
           if (turns) {
             if ((t == 1 || turn > 0) &&
                 !wide_warp_wait(s, &s.turn[t], (uint32_t)((turn - (t == 0 ? 1 : 0)) & 1),
-                                a.status)) {
+                                a.status, limit)) {
               ok = false;
               break;
             }
@@ -644,7 +676,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
         if (ragged) {
           // clean the tile's values: thread = key
           const Entry<D> entry(wide.share, t, 2 * ((wide.share ? base : n) + k) + 1);
-          if (!wide_warp_wait(s, &s.full[entry.slot], entry.parity, a.status)) {
+          if (!wide_warp_wait(s, &s.full[entry.slot], entry.parity, a.status, limit)) {
             ok = false;
             break;
           }
@@ -677,7 +709,7 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       }
       // the row's result, once the stream's last product has completed
       if (ok && mine > 0) {
-        ok = wide_warp_wait(s, &s.o_done[t], (uint32_t)((n + mine - 1) & 1), a.status);
+        ok = wide_warp_wait(s, &s.o_done[t], (uint32_t)((n + mine - 1) & 1), a.status, limit);
         tc_fence_after();
       }
       if (ok && busy) {
@@ -747,6 +779,8 @@ wide_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ Args 
       n += mine;
       ++mark;
     }
+    __syncwarp();
+    if (!ok) leave_nan<T, D, COPIES>(a, deal, wide);
   }
   tc_fence_before();
   __syncthreads();
@@ -785,7 +819,7 @@ inline bool wide_map(CUtensorMap* map, const void* base, bool bf16, int64_t colu
 
 template <class T, int D, int COPIES>
 inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& w,
-                               cudaStream_t stream) {
+                               uint32_t wait_limit, cudaStream_t stream) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const int64_t d = a.head_dim, kv = a.kv_heads;
   WideMaps maps;
@@ -817,7 +851,7 @@ inline cudaError_t launch_wide(const Args& a, const Deal& deal, const WideRows& 
   if (e != cudaSuccess) return e;
   if (ready != 1) return cudaErrorInvalidKernelImage;
   return launch_pdl(kernel, dim3((unsigned)deal.grid), dim3(kWideThreads), smem, stream, maps, a,
-                    deal, w);
+                    deal, w, wait_limit);
 }
 
 }  // namespace tree

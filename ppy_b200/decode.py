@@ -79,7 +79,8 @@ def tree_attention(q, k_new, v_new, keys, values, lengths, parents=None, counts=
 
     bf16 or f16; head_dim a multiple of 8 up to 128; rows on 16-byte boundaries; up to 256 nodes
     with parents. `status` (int32 [1], optional) is raised to 2 when a length, count or parent is out of
-    range: the call then keeps to the buffers, and takes such a parent for -1."""
+    range: the call then keeps to the buffers, and takes such a parent for -1. It is raised, too,
+    when a wait inside the kernel was given up: rows without a result are NaN then."""
     dtype, device = q.dtype, q.get_device()
     kind = _KINDS.get(dtype)
     if kind is None or device < 0 or q.dim() != 4 or keys.dim() != 4:
@@ -328,10 +329,12 @@ class KVCache:
         self.status.zero_()
 
     def check(self) -> None:
-        """Raise if an index given to a call since the last check was out of range (syncs)."""
+        """Raise if an index given to a call since the last check was out of range, or a kernel
+        gave up (syncs)."""
         if int(self.status.item()) != 0:
             self.status.zero_()
-            raise B200Error("a length, count, parent, path, position or token id was out of range")
+            raise B200Error("a length, count, parent, path, position or token id was out of range, "
+                            "or a kernel gave up a wait and left NaN")
 
     def accept(self, path=None, accepted=None) -> None:
         """The nodes path[b, :accepted[b]] of the last extension (int32 [batch, steps] and

@@ -82,6 +82,8 @@ def library() -> ctypes.CDLL:
         for name in ("ppyb200_tree_attention", "ppyb200_accept", "ppyb200_evict"):
             getattr(lib, name).argtypes = [ctypes.c_char_p]
             getattr(lib, name).restype = ctypes.c_int32
+        lib.ppyb200_tree_attention_wait_limit.argtypes = [ctypes.c_int64]
+        lib.ppyb200_tree_attention_wait_limit.restype = None
         lib.ppyb200_accept_part.argtypes = [ctypes.c_char_p, ctypes.c_char_p]
         lib.ppyb200_accept_part.restype = ctypes.c_int32
         for name in ("ppyb200_tree_attention_workspace", "ppyb200_evict_workspace"):

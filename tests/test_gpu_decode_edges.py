@@ -521,3 +521,40 @@ def test_infinities_in_the_cache(lengths, nodes, heads, kv, d, cap, tree, dtype)
     same = torch.ones_like(out, dtype=torch.bool)
     same[0, :, :group, [1, 7, 9, 12, 14, 17]] = False
     assert torch.equal(out[same], clean[same])
+
+
+@pytest.mark.parametrize("lengths,nodes,heads,kv,d,cap,tree", [
+    ((300, 31), 45, 6, 2, 128, 2_000, False),            # two row tiles that share their keys
+    ((4000, 129), 1, 8, 2, 64, 270_000, False),          # four copies of the rows
+    ((1111, 5), 12, 8, 2, 128, 60_000, True),            # two
+    ((1, 640), 64, 2, 2, 64, 30_000, True),
+    ((60,), 20, 8, 1, 64, 128, True),                    # one CTA, no workspace
+    (tuple(range(1, 161, 8)), 40, 32, 8, 64, 300, True),  # more items than CTAs
+])
+def test_a_wait_given_up_leaves_no_old_memory(lengths, nodes, heads, kv, d, cap, tree):
+    """Every wait gives up before it tries: the status says so, and rows without a result are NaN,
+    with or without a status word. The next call is right."""
+    from ppy_b200 import runtime
+
+    counts = [max(1, nodes - 3 * b) for b in range(len(lengths))]
+    x = Inputs(lengths, nodes, heads, kv, d, tree=tree, counts=counts,
+               spare=cap - max(lengths) - nodes)
+    lib = runtime.library()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(x.q, 7.0, memory_format=torch.contiguous_format)
+    lse = torch.full((len(lengths), heads, nodes), 5.0, device="cuda")
+    try:
+        lib.ppyb200_tree_attention_wait_limit(0)
+        x.call(out=out, lse=lse, status=status)
+        made, made_lse = x.call()
+    finally:
+        lib.ppyb200_tree_attention_wait_limit(-1)
+    assert int(status) == 2
+    for b, n in enumerate(counts):
+        for o, s in ((out, lse), (made, made_lse)):
+            assert bool(o[b, :n].isnan().all()) and bool(s[b, :, :n].isnan().all())
+        assert bool((out[b, n:] == 7.0).all()) and bool((lse[b, :, n:] == 5.0).all())
+    for b, n in enumerate(lengths):
+        x.keys[b, :, n:] = math.nan
+        x.values[b, :, n:] = math.nan
+    x.check(*x.call())
