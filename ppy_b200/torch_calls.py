@@ -60,14 +60,18 @@ class Beside:
         if torch.cuda.current_device() != index:
             self._guard = torch.cuda.device(index)
             self._guard.__enter__()
-        if bound < 0:
-            runtime.init(index)
-        handle = lib.ppyb200_stream() or 0
-        current = torch.cuda.current_stream(index)
-        if handle != (current.cuda_stream or runtime._LEGACY_STREAM):
-            self.side = (torch.cuda.default_stream(index) if handle == runtime._LEGACY_STREAM
-                         else _external_stream(handle, index))
-            _order(index, current, self.side)
+        try:
+            if bound < 0:
+                runtime.init(index)
+            handle = lib.ppyb200_stream() or 0
+            current = torch.cuda.current_stream(index)
+            if handle != (current.cuda_stream or runtime._LEGACY_STREAM):
+                self.side = (torch.cuda.default_stream(index) if handle == runtime._LEGACY_STREAM
+                             else _external_stream(handle, index))
+                _order(index, current, self.side)
+        except BaseException:
+            self._leave()
+            raise
 
     def wait_for_torch(self) -> None:
         """The launches that follow wait for what torch's stream holds by now."""
@@ -75,8 +79,13 @@ class Beside:
             _order(self._index, torch.cuda.current_stream(self._index), self.side)
 
     def end(self) -> None:
-        if self.side is not None:
-            _order(self._index, self.side, torch.cuda.current_stream(self._index))
+        try:
+            if self.side is not None:
+                _order(self._index, self.side, torch.cuda.current_stream(self._index))
+        finally:
+            self._leave()
+
+    def _leave(self) -> None:
         if self._guard is not None:
             self._guard.__exit__(None, None, None)
 

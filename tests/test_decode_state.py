@@ -48,3 +48,54 @@ def test_accept_refuses_paths_of_other_shapes():
     with pytest.raises(runtime.B200Error, match="path"):
         cache.accept(torch.zeros(3, dtype=torch.int32))
     assert cache.pending is not None
+
+
+def test_a_call_that_fails_leaves_the_current_device(monkeypatch):
+    """A call with tensors of another device than the current one makes that the current one until
+    it ends, also when the order of the streams cannot be set up or restored."""
+    from ppy_b200 import torch_calls
+
+    left = []
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            left.append(("enter", self.index))
+
+        def __exit__(self, *_):
+            left.append(("exit", self.index))
+
+    class Library:
+        @staticmethod
+        def ppyb200_current_device():
+            return -1
+
+        @staticmethod
+        def ppyb200_stream():
+            return 64
+
+    class Stream:
+        cuda_stream = 128
+
+    def refuse(*_):
+        raise runtime.B200Error("no")
+
+    monkeypatch.setattr(runtime, "library", lambda: Library)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: Stream)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(runtime, "init", refuse)
+    with pytest.raises(runtime.B200Error):
+        torch_calls.Beside(1)
+    assert left == [("enter", 1), ("exit", 1)]
+    left.clear()
+    orders = iter((None, refuse))
+    monkeypatch.setattr(runtime, "init", lambda index: None)
+    monkeypatch.setattr(torch_calls, "_external_stream", lambda *_: Stream)
+    monkeypatch.setattr(torch_calls, "_order", lambda *_: (next(orders) or (lambda: None))())
+    beside = torch_calls.Beside(1)
+    with pytest.raises(runtime.B200Error):
+        beside.end()
+    assert left == [("enter", 1), ("exit", 1)]
