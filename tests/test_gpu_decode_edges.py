@@ -558,3 +558,83 @@ def test_a_wait_given_up_leaves_no_old_memory(lengths, nodes, heads, kv, d, cap,
         x.keys[b, :, n:] = math.nan
         x.values[b, :, n:] = math.nan
     x.check(*x.call())
+
+
+# ---------------------------------------------------------------- orders of calls, captured
+
+
+def test_a_padded_step_captured_on_the_runtimes_own_stream():
+    """Extension, acceptance and eviction of a padded batch in one graph, torch's stream capturing and
+    the launches on the runtime's: replays are the same calls made one by one."""
+    from ppy_b200 import runtime
+
+    model, cache = _model_and_cache(3, 64)
+    other = model.new_cache(3, capacity=64)
+    prompt, steps = _ids(3, 20, seed=1), _ids(3, 12, seed=2)
+    counts = [[4, 1, 3], [2, 4, 1], [1, 1, 4]]
+    for c in (cache, other):
+        model.extend(c, prompt)
+        c.accept()
+    ids = torch.zeros(3, 4, dtype=torch.int64, device="cuda")
+    real = torch.ones(3, dtype=torch.int32, device="cuda")
+    logits = model.new_logits(3, 4)
+    stream = torch.cuda.Stream()
+    try:
+        runtime.set_stream(None)
+        with torch.cuda.stream(stream):
+            warm = model.new_cache(3, capacity=64)
+            model.extend(warm, ids, counts=real, logits=logits)
+            warm.accept()
+            warm.evict(21, recent=2)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                model.extend(cache, ids, counts=real, logits=logits)
+                cache.accept()
+                kept = cache.evict(21, recent=2)
+        for i, n in enumerate(counts):
+            with torch.cuda.stream(stream):
+                ids.copy_(steps[:, 4 * i:4 * i + 4])
+                real.copy_(torch.tensor(n, dtype=torch.int32))
+                graph.replay()
+                got = logits.clone()
+                want = model.extend(other, steps[:, 4 * i:4 * i + 4],
+                                    counts=torch.tensor(n, dtype=torch.int32, device="cuda"))
+                other.accept()
+                want_kept = other.evict(21, recent=2)
+                for b in range(3):
+                    assert torch.equal(got[b, :n[b]], want[b, :n[b]])
+                assert torch.equal(kept, want_kept)
+                for name in ("lengths", "seen"):
+                    assert torch.equal(getattr(cache, name), getattr(other, name))
+                for b in range(3):
+                    length = int(cache.lengths[b])
+                    for name in ("keys", "values", "weights", "positions"):
+                        assert torch.equal(getattr(cache, name)[:, b, :, :length],
+                                           getattr(other, name)[:, b, :, :length]), name
+        cache.check()
+        other.check()
+        assert cache.seen.tolist() == [27, 26, 28]
+    finally:
+        torch.cuda.synchronize()
+        runtime.set_stream(torch.cuda.current_stream())
+
+
+def test_a_cache_without_weights_decodes_the_same():
+    model, cache = _model_and_cache(2, 120, layers=2)
+    bare = model.new_cache(2, capacity=120, weights=False)
+    prompt, tree = _ids(2, 80, seed=1), _ids(2, 4, seed=2)
+    parents = torch.tensor([-1, 0, 0, 2], dtype=torch.int32, device="cuda")
+    path = torch.tensor([[0, 2, 3], [0, 1, 3]], dtype=torch.int32, device="cuda")
+    accepted = torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    for step in range(2):
+        outs = []
+        for c in (cache, bare):
+            model.extend(c, prompt[:, 40 * step:40 * step + 40])
+            c.accept()
+            outs.append(model.extend(c, tree, parents))
+            c.accept(path, accepted)
+            c.check()
+        assert torch.equal(*outs)
+    assert torch.equal(cache.keys, bare.keys) and torch.equal(cache.values, bare.values)
+    assert torch.equal(cache.positions, bare.positions) and bare.weights is None
