@@ -6,8 +6,8 @@
 //   s_ij = scale q_i . k_j,  lse_i = log sum_visible e^{s_ij},  out_i = sum e^{s_ij - lse_i} v_j
 //
 // The rows of one key head (nodes x the query heads that share it) form the M side of the
-// products. Two kernels: the one here streams tiles of 64 keys through shared memory for 16 (or
-// 64) rows a CTA with warp-level products, and tree_attention_sm100.cuh holds the tensor-core
+// products. Two kernels: the one here streams tiles of 64 keys through shared memory for 16 rows
+// a CTA with warp-level products, and tree_attention_sm100.cuh holds the tensor-core
 // kernel for many rows. Both keep a running maximum and sum (f32). The key tiles of all sequences
 // are dealt to the CTAs in parts of equal size; a sequence of several parts is joined by a
 // second kernel in the order of its parts, so results do not depend on timing.

@@ -51,11 +51,13 @@ inline bool strides_fit(const int64_t (&strides)[3], int64_t n0, int64_t n1, int
 
 // Which kernel is the faster, by the bytes of a full cache (the lengths are on the device). The
 // narrow kernel starts and ends an item in about 2 us where the wide one takes 6, and reads the
-// cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.4. Measured, wide
-// against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 20.1 / 10.2,
-// 64 of 750 (144 MB) 101.6 / 51.9; 4 rows, 8 heads of 128, 64 of 1500 (384 MB) 117.9 / 93.3, 16 of
-// 8000 (504 MB) 98.6 / 110.1; 32 rows, 12 heads of 64, 8 of 1000 (26 MB) 29.6 / 26.5; 64 rows,
-// 2 sequences (6 MB) 23.4 / 23.0, 4 (13 MB) 25.4 / 28.8, 64 (204 MB) 161 / 240.
+// cache once per 16 rows at up to 4.6 TB/s, the wide one once at up to 5.5. Measured, wide
+// against narrow, us: one row, 12 heads of 64, 1 sequence of 1000 entries (3 MB) 19.7 / 10.0,
+// 64 of 750 (144 MB) 71.8 / 51.5; 4 rows, 8 heads of 128, 64 of 1500 (384 MB) 95.8 / 93.1, 16 of
+// 8000 (504 MB) 95.7 / 109.7; trees of 32 nodes, 12 heads of 64, 8 of 1000 (26 MB) 26.3 / 28.7; of
+// 64 nodes, 2 sequences (6 MB) 21.7 / 23.6, 4 (13 MB) 22.5 / 29.5, 64 (204 MB) 110 / 249. A cache
+// that is mostly empty counts as a full one: 64 of 750 entries in slots for 16384 go to the wide
+// kernel, 73.3 / 52.4.
 inline bool narrow_faster(const Args& a) {
   const int64_t rows = a.nodes * (a.heads / a.kv_heads), item = a.capacity * a.head_dim * 4;
   const int64_t cache = a.batch * a.kv_heads * item, tiles = (rows + kNarrowRows - 1) / kNarrowRows;

@@ -180,9 +180,13 @@ def _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accep
     for name, t in (("lengths", lengths), ("seen", seen), ("accepted", accepted)):
         whole(name, t, (batch,), torch.int32, device)
     whole("path", path, (batch, length) if path.dim() == 2 else (length,), torch.int32, device)
-    for name, t in (("taken", taken), ("taken", before), ("counts", counts)):
-        if t is not None:
-            whole(name, t, (batch,), torch.int32, device)
+    before_at = taken_at = counts_at = 0
+    if taken is not None:
+        taken_at = whole("taken", taken, (batch,), torch.int32, device)
+    if before is not None:
+        before_at = whole("taken", before, (batch,), torch.int32, device)
+    if counts is not None:
+        counts_at = whole("counts", counts, (batch,), torch.int32, device)
     tables = weights if weights is not None else positions
     strides = (0, 0, 0)
     for name, t, kept in (("weights", weights, torch.float32),
@@ -204,7 +208,7 @@ def _accept(q, lse, keys, values, weights, positions, lengths, seen, path, accep
                 steps, heads, kv_heads, d, capacity, *q_strides[:4], *keys_strides[:4],
                 *values_strides[:4], *strides,
                 1.0 / math.sqrt(d) if scale is None else scale), _PART.pack(
-                    _address(counts), _address(before), _address(taken), first, length,
+                    counts_at, before_at, taken_at, first, length,
                     length if path.dim() == 2 else 0)) != runtime.STATUS_OK:
             raise B200Error(runtime.last_error())
     finally:
