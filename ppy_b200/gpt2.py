@@ -338,7 +338,7 @@ class GPT2:
         # tokens behind the last are seen by none before them
         whole = (length + 127) // 128 * 128
         padded = torch.nn.functional.pad(ids, (0, whole - length))
-        following = torch.full_like(padded, -1)
+        following = torch.full_like(padded, -1, memory_format=torch.contiguous_format)
         following[:, :length - 1] = ids[:, 1:]
         beside = torch_calls.begin(ids.get_device())
         try:

@@ -425,6 +425,16 @@ def test_score_texts_of_any_length(batch, length):
         _near(rows, oracle_gpt2.forward(model, ids.contiguous())[:, :-1])
 
 
+def test_score_texts_that_lie_in_columns():
+    model, _ = _model_and_cache(1, 1)
+    for length in (100, 128):
+        ids = _ids(3, length)
+        columns = ids.t().contiguous().t()
+        assert not columns.is_contiguous()
+        got, want = model.score(columns, top=1), model.score(ids, top=1)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_score_beside_torchs_stream():
     """ids made on torch's stream while the launches go to another: no wait by the caller."""
     from ppy_b200 import runtime
